@@ -35,7 +35,7 @@ enum {
   INF_ERR_STATE = -4        /* plan not bound / wrong call order                */
 };
 
-enum { INF_DTYPE_F32 = 0, INF_DTYPE_BF16 = 1, INF_DTYPE_I32 = 2, INF_DTYPE_I64 = 3 };
+enum { INF_DTYPE_F32 = 0, INF_DTYPE_BF16 = 1, INF_DTYPE_I32 = 2, INF_DTYPE_I64 = 3, INF_DTYPE_I8 = 4 };
 /* GEMM arithmetic: FP32 exact f32 MFMA; BF16 bf16 operands (fp32 accumulation, fp32
  * master weights); BF16X3 fp32 operands multiplied as split bf16 (hi*hi + hi*lo + lo*hi,
  * ~2^-16 relative per product) -- every buffer and kernel of the fp32 mode, only the
@@ -194,6 +194,51 @@ int inf_ff_encode(int64_t n, int d, const float* x, const float* bands, int k, i
  * not in a plan arena: the plan update's arithmetic (adam_dev.hpp adam_elem). */
 int inf_adam_dense(int64_t n, float* param, const float* grad, float* exp_avg, float* exp_avg_sq, int step,
                    double lr, double beta1, double beta2, double eps, inf_stream_t stream);
+
+/* ---- dense layers in 8 bits ------------------------------------------------------ */
+/* Rows in 8 bits: scale[m] = fl32(max_k |x_mk| / 127), q_mk = the whole number nearest to
+ * 127 x_mk / max_k |x_mk| (the ratio itself; ties to even).  A row of zeros has scale 0; a
+ * row with an infinity or a NaN has scale NaN and q 0.  x: fp32 / bf16, ld_x any (0 repeats
+ * one row).  q rows start on 16 bytes: q 16-byte aligned, ld_q >= k a multiple of 16; what
+ * lies behind column k is neither read as a value nor written.                            */
+int inf_quantize_rows(const void* x, int x_dtype, int64_t rows, int k, int64_t ld_x, int8_t* q, int64_t ld_q,
+                      float* scale, inf_stream_t stream);
+/* out[m][j] = q[m][j] scale[m], rounded once to fp32 / bf16. */
+int inf_restore_rows(const int8_t* q, int64_t ld_q, const float* scale, int64_t rows, int k, void* out, int out_dtype,
+                     int64_t ld_out, inf_stream_t stream);
+/* 8-bit weights q[n][k] (any strides) laid out for inf_linear_int; `packed` 16-byte aligned,
+ * inf_packed_weight_bytes(n, k) bytes. */
+int64_t inf_packed_weight_bytes(int n, int k);
+int inf_pack_weight(const int8_t* q, int64_t stride_n, int64_t stride_k, int n, int k, int8_t* packed,
+                    inf_stream_t stream);
+/* out = act(fl(fl(acc) fl(x_scale[m] w_scale[n])) + bias[n] + add[m][n]), acc the exact sum
+ * of the 8-bit products (k <= 2^17), each operation rounded once to fp32; bias and add may
+ * be NULL.  x: fp32 / bf16 (put into 8 bits first, in the workspace), or INF_DTYPE_I8 rows
+ * with x_scale, behind whose last row 128 bytes may be read (their values do not matter).
+ * out: fp32 / bf16, or INF_DTYPE_I8 rows with out_scale (inf_quantize_rows of the result).
+ * act 0 none, 1 ReLU, 2 sigmoid.  workspace: inf_linear_int_workspace_bytes bytes.        */
+int64_t inf_linear_int_workspace_bytes(int64_t rows, int n, int k, int x_dtype, int out_dtype);
+int inf_linear_int(int64_t rows, int n, int k, const void* x, int x_dtype, int64_t ld_x, const float* x_scale,
+                   const int8_t* w, const float* w_scale, const float* bias, const float* add, int64_t ld_add, int act,
+                   void* out, int out_dtype, int64_t ld_out, float* out_scale, void* workspace, inf_stream_t stream);
+/* Linear layer that keeps its input in 8 bits: y = act(x W^T + bias + add) in fp32 from x
+ * (fp32 / bf16) as it is, W(n, k) = W[n stride_wn + k stride_wk]; bias and add may be NULL,
+ * add may be y.  q / scale (not NULL): the rows of x in 8 bits.  mask (not NULL): bit j of
+ * word w of row m (ceil(n / 32) words a row) = y[m][32 w + j] > 0.  workspace:
+ * inf_linear_ckpt_workspace_bytes(.., 0) bytes.                                            */
+int64_t inf_linear_ckpt_workspace_bytes(int64_t rows, int n, int k, int x_dtype, int backward);
+int inf_linear_ckpt_forward(int64_t rows, int n, int k, const void* x, int x_dtype, int64_t ld_x, const float* W,
+                            int64_t stride_wn, int64_t stride_wk, const float* bias, const float* add, int64_t ld_add,
+                            int act, float* y, int64_t ld_y, uint32_t* mask, int8_t* q, int64_t ld_q, float* scale,
+                            void* workspace, inf_stream_t stream);
+/* Its gradients: dz = dy (act 0), dy where the mask's bit is set (1), dy y (1 - y) (2);
+ * dx = dz W (fp32 / bf16), dW = dz^T (scale q), db = sum over the rows of dz.  dx, dW and db
+ * may each be NULL; with no rows dW and db are zero.  workspace:
+ * inf_linear_ckpt_workspace_bytes(.., 1) bytes.                                            */
+int inf_linear_ckpt_backward(int64_t rows, int n, int k, const float* dy, int64_t ld_dy, int act, const float* y,
+                             int64_t ld_y, const uint32_t* mask, const int8_t* q, int64_t ld_q, const float* scale,
+                             const float* W, int64_t stride_wn, int64_t stride_wk, void* dx, int dx_dtype,
+                             int64_t ld_dx, float* dW, int64_t ld_dw, float* db, void* workspace, inf_stream_t stream);
 
 /* ---- plan: one TextureField (model.py:12-112) + its training step ---------------- */
 typedef struct inf_plan inf_plan;

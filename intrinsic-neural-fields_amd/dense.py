@@ -8,10 +8,23 @@ in one output buffer: a plain nn.Linear (one segment), LinearWithConcatAndActiva
 (model.py:186-191: one weight split by column ranges) without materialising the concat.
 Every product, activation, gradient and bias sum runs in libinf_hip.so; torch only
 allocates.
+
+In 8 bits (csrc/quant.hpp: whole numbers q and one scale s a row, x ~ s q):
+`linear(..., checkpoint="int8")` keeps the inputs in 8 bits between forward and backward
+(a quarter of the memory; ReLU's outputs as one bit each), `linear8` multiplies 8-bit rows
+with 8-bit weights for rendering, and `quantize_rows` / `Rows8.restore` are the rows
+themselves.
+
+A training step of these layers that is captured into a HIP graph captures its forward too:
+autograd ties a leaf's gradient accumulation to the stream of its first live graph, so no
+eager graph of the same parameters may be alive while a backward pass is captured.
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
+from torch.autograd.function import once_differentiable
 
 ACT = {None: 0, "relu": 1, "sigmoid": 2}
 
@@ -90,14 +103,306 @@ class _Linear(torch.autograd.Function):
         return (None, None, *dxs, *dws, *dbs)
 
 
-def linear(segments, weights, biases, act=None):
-    """segments: [(x_s, weight index, column offset)]; weights / biases: lists of tensors."""
+def linear(segments, weights, biases, act=None, checkpoint=None):
+    """segments: [(x_s, weight index, column offset)]; weights / biases: lists of tensors.
+
+    checkpoint="int8": x_s (fp32, or bf16 taken as it is) is kept in 8 bits for the backward,
+    where dW_s = dz^T (s q)_s; the output, dx_s and the bias gradients do not depend on it.
+    A list names it for each segment: "int8", or the `Rows8` of that x_s where several layers
+    read the same tensor.  Products are exact to fp32, as without it, in another order of
+    summation; a row with an infinity or a NaN gives NaN."""
     for t in [x for x, _, _ in segments] + list(weights) + list(biases):
         if not t.is_cuda:
             raise RuntimeError("the dense layers run on the HIP device only; there is no CPU fallback")
     spec = tuple((wi, c0) for _, wi, c0 in segments)
+    if checkpoint is not None:
+        return _linear_ckpt(segments, spec, weights, biases, ACT[act], checkpoint)
     xs = [x.to(torch.float32) for x, _, _ in segments]
     return _Linear.apply(spec, ACT[act], *xs, *weights, *biases)
+
+
+# ---- 8 bits -------------------------------------------------------------------------
+
+def _on(device):
+    """The device of the tensors as the current one, for launches on its current stream."""
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _round_up(n, m):
+    return (n + m - 1) // m * m
+
+
+def _rows_of(x, what):
+    """x as rows whose values are next to each other (any distance between rows)."""
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"{what} must be a matrix [rows, k] with k >= 1, got {list(x.shape)}")
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"{what} must be fp32 or bf16, got {x.dtype}")
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+
+
+class Rows8:
+    """The rows of a matrix in 8 bits: `q` int8 [rows, k] (rows start on 16 bytes) and
+    `scale` fp32 [rows], standing for scale[:, None] * q.  Made by quantize_rows and linear8."""
+
+    __slots__ = ("q", "scale")
+
+    def __init__(self, rows, k, device):
+        ld = _round_up(k, 16)
+        # 128 bytes behind the last row: a product may read past it (include/inf_hip.h)
+        self.q = torch.empty(rows * ld + 128, dtype=torch.int8, device=device).as_strided((rows, k), (ld, 1))
+        self.scale = torch.empty(rows, dtype=torch.float32, device=device)
+
+    @classmethod
+    def _from(cls, q, scale):
+        r = cls.__new__(cls)
+        r.q, r.scale = q, scale
+        return r
+
+    @property
+    def shape(self):
+        return self.q.shape
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def restore(self, dtype=torch.float32):
+        """scale * q, rounded once to fp32 / bf16."""
+        rt = _rt()
+        from inf_hip import lib
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"8-bit rows are restored to fp32 or bf16, not {dtype}")
+        rows, k = self.q.shape
+        out = torch.empty((rows, k), dtype=dtype, device=self.q.device)
+        with _on(self.q.device):
+            rt.check(lib.inf_restore_rows(rt.ptr(self.q), self.q.stride(0), rt.ptr(self.scale), rows, k, rt.ptr(out),
+                                          rt.dtype_code(out), k, rt.stream_handle()), "restore_rows")
+        return out
+
+
+def quantize_rows(x):
+    """x [rows, k] fp32 / bf16 in 8 bits: scale = max|x| / 127 of each row, q the whole number
+    nearest to 127 x / max|x| (ties to even).  Rows of zeros have scale 0; a row with an
+    infinity or a NaN has scale NaN, and whatever is made of it is NaN.  No gradient."""
+    rt = _rt()
+    from inf_hip import lib
+    rt.require_hip(x)
+    x = _rows_of(x.detach(), "x")
+    rows, k = x.shape
+    r = Rows8(rows, k, x.device)
+    with _on(x.device):
+        rt.check(lib.inf_quantize_rows(rt.ptr(x), rt.dtype_code(x), rows, k, x.stride(0), rt.ptr(r.q), r.q.stride(0),
+                                       rt.ptr(r.scale), rt.stream_handle()), "quantize_rows")
+    return r
+
+
+class Weight8:
+    """A weight [n, k] in 8 bits with one scale a row, laid out for linear8 (`packed`)."""
+
+    __slots__ = ("packed", "scale", "n", "k")
+
+    def __init__(self, packed, scale, n, k):
+        self.packed, self.scale, self.n, self.k = packed, scale, n, k
+
+
+def pack_weight8(q, scale):
+    """8-bit weights q int8 [n, k] (any strides) with scales fp32 [n], laid out for linear8."""
+    rt = _rt()
+    from inf_hip import lib
+    rt.require_hip(q, scale)
+    if q.dim() != 2 or q.dtype != torch.int8 or min(q.shape) < 1:
+        raise ValueError("an 8-bit weight is an int8 matrix [n, k]")
+    n, k = q.shape
+    if scale.shape != (n,) or scale.dtype != torch.float32 or scale.device != q.device:
+        raise ValueError("an 8-bit weight has one fp32 scale a row, on its device")
+    packed = torch.empty(int(lib.inf_packed_weight_bytes(n, k)), dtype=torch.int8, device=q.device)
+    with _on(q.device):
+        rt.check(lib.inf_pack_weight(rt.ptr(q), q.stride(0), q.stride(1), n, k, rt.ptr(packed), rt.stream_handle()),
+                 "pack_weight")
+    return Weight8(packed, scale.contiguous().clone(), n, k)
+
+
+def quantize_weight(W, col0=0, cols=None):
+    """W[:, col0:col0 + cols] (fp32 / bf16) in 8 bits, laid out for linear8."""
+    cols = W.shape[1] - col0 if cols is None else cols
+    if col0 < 0 or cols < 1 or col0 + cols > W.shape[1]:
+        raise ValueError(f"columns {col0}..{col0 + cols} of a weight with {W.shape[1]}")
+    r = quantize_rows(W.detach()[:, col0:col0 + cols])
+    return pack_weight8(r.q, r.scale)
+
+
+def linear8(xs, weights, biases, act=None, out=torch.float32):
+    """act(sum_s x_s W_s^T + sum bias) with the rows of x_s and W_s in 8 bits: the sums of their
+    products are exact, and scales, bias and the sum over s are one fp32 rounding each.
+
+    xs: for each segment a matrix fp32 / bf16 (put into 8 bits on the way) or a Rows8;
+    weights: a Weight8 each; biases: fp32 [n], one for each of the first segments.
+    out: torch.float32, torch.bfloat16, or torch.int8 for a Rows8 of the result.
+    For rendering: it has no gradient, and refuses inputs that ask for one."""
+    rt = _rt()
+    from inf_hip import DTYPE_I8, lib
+    code = {torch.float32: rt.DTYPE_F32, torch.bfloat16: rt.DTYPE_BF16, torch.int8: DTYPE_I8}.get(out)
+    if code is None:
+        raise ValueError(f"linear8 gives fp32, bf16 or int8 rows, not {out}")
+    if len(xs) < 1 or len(xs) != len(weights) or len(biases) > len(xs):
+        raise ValueError("linear8 takes one weight and at most one bias for each segment")
+    rows, n, device = xs[0].shape[0], weights[0].n, xs[0].device
+    grad = torch.is_grad_enabled()
+    acc, last = None, len(xs) - 1
+    with _on(device) if device.type == "cuda" else contextlib.nullcontext():
+        for s, (x, w) in enumerate(zip(xs, weights)):
+            if isinstance(x, Rows8):
+                q, scale, xc = x.q, x.scale, DTYPE_I8
+            else:
+                rt.require_hip(x)
+                if grad and x.requires_grad:
+                    raise RuntimeError("linear8 has no gradient: call it under torch.no_grad(), or train with linear")
+                q, scale = _rows_of(x, "x"), None
+                xc = rt.dtype_code(q)
+            if q.shape != (rows, w.k) or w.n != n:
+                raise ValueError(f"segment {s}: x {list(q.shape)} and weight [{w.n}, {w.k}] do not fit [{rows}, {n}]")
+            b = biases[s] if s < len(biases) else None
+            if b is not None and (b.shape != (n,) or b.dtype != torch.float32 or not b.is_contiguous()):
+                raise ValueError("a bias is a contiguous fp32 [n] tensor")
+            if q.device != device or w.packed.device != device or (b is not None and b.device != device):
+                raise ValueError("linear8 takes its tensors on one device")
+            oc = code if s == last else rt.DTYPE_F32
+            if oc == DTYPE_I8:
+                y = Rows8(rows, n, device)
+                op, ldo, osc = y.q, y.q.stride(0), y.scale
+            else:
+                y = torch.empty((rows, n), dtype=out if s == last else torch.float32, device=device)
+                op, ldo, osc = y, n, None
+            nws = int(lib.inf_linear_int_workspace_bytes(rows, n, w.k, xc, oc))
+            ws = torch.empty(nws, dtype=torch.uint8, device=device) if nws else None
+            rt.check(lib.inf_linear_int(rows, n, w.k, rt.ptr(q), xc, q.stride(0), rt.ptr(scale), rt.ptr(w.packed),
+                                        rt.ptr(w.scale), rt.ptr(b), rt.ptr(acc), n, ACT[act] if s == last else 0,
+                                        rt.ptr(op), oc, ldo, rt.ptr(osc), rt.ptr(ws), rt.stream_handle()), "linear_int")
+            acc = y
+    return y
+
+
+class _LinearCkpt(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, spec, act, kept, *tensors):
+        # spec and tensors as _Linear; kept: per segment the Rows8 of x, or None to make them
+        rt = _rt()
+        from inf_hip import lib
+        nseg = len(spec)
+        nw = max(w for w, _ in spec) + 1
+        xs, ws, bs = tensors[:nseg], tensors[nseg:nseg + nw], tensors[nseg + nw:]
+        needs = ctx.needs_input_grad[3:]
+        rows, n, device = xs[0].shape[0], ws[0].shape[0], xs[0].device
+        save, y, mask = [], None, None
+        with _on(device):
+            st = rt.stream_handle()
+            y = torch.empty((rows, n), dtype=torch.float32, device=device)
+            if act == 1 and any(needs):
+                mask = torch.empty((rows, (n + 31) // 32), dtype=torch.int32, device=device)
+            for s, (wi, c0) in enumerate(spec):
+                x, W = xs[s], ws[wi]
+                k, last = x.shape[1], s == nseg - 1
+                rows8 = kept[s]
+                make = needs[nseg + wi] and rows8 is None
+                if make:
+                    rows8 = Rows8(rows, k, device)
+                xc = rt.dtype_code(x)
+                work = torch.empty(int(lib.inf_linear_ckpt_workspace_bytes(rows, n, k, xc, 0)), dtype=torch.uint8,
+                                   device=device)
+                b = bs[s] if s < len(bs) else None
+                rt.check(lib.inf_linear_ckpt_forward(
+                    rows, n, k, rt.ptr(x), xc, x.stride(0), W.data_ptr() + 4 * c0 * W.stride(1), W.stride(0),
+                    W.stride(1), rt.ptr(b), rt.ptr(y) if s else None, n, act if last else 0, rt.ptr(y), n,
+                    rt.ptr(mask) if last else None, rt.ptr(rows8.q) if make else None,
+                    rows8.q.stride(0) if make else 0, rt.ptr(rows8.scale) if make else None, rt.ptr(work), st),
+                    "linear_ckpt_forward")
+                save += [rows8.q, rows8.scale] if needs[nseg + wi] else [None, None]
+        ctx.spec, ctx.act, ctx.nw, ctx.nb = spec, act, nw, len(bs)
+        ctx.widths, ctx.dtypes = [x.shape[1] for x in xs], [x.dtype for x in xs]
+        ctx.rows, ctx.n = rows, n
+        ctx.save_for_backward(*save, *ws, mask, y if act == 2 else None)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        rt = _rt()
+        from inf_hip import lib
+        spec, act, nw, nb = ctx.spec, ctx.act, ctx.nw, ctx.nb
+        nseg, rows, n = len(spec), ctx.rows, ctx.n
+        saved = ctx.saved_tensors
+        ws, mask, y = saved[2 * nseg:2 * nseg + nw], saved[-2], saved[-1]
+        needs = ctx.needs_input_grad[3:]
+        dy = dy.to(torch.float32)
+        if dy.stride(1) != 1 or dy.stride(0) < n:
+            dy = dy.contiguous()
+        device = dy.device
+        dxs, dws, dbs = [None] * nseg, [None] * nw, [None] * nb
+        with _on(device):
+            st = rt.stream_handle()
+            for s, (wi, c0) in enumerate(spec):
+                q, scale, W, k = saved[2 * s], saved[2 * s + 1], ws[wi], ctx.widths[s]
+                dx = dwp = None
+                if needs[s]:
+                    dxs[s] = dx = torch.empty((rows, k), dtype=ctx.dtypes[s], device=device)
+                if needs[nseg + wi]:
+                    if dws[wi] is None:
+                        covered = sum(kk for (wj, _), kk in zip(spec, ctx.widths) if wj == wi) == W.shape[1]
+                        dws[wi] = (torch.empty if covered else torch.zeros)(W.shape, dtype=torch.float32,
+                                                                            device=device)
+                    dwp = dws[wi].data_ptr() + 4 * c0
+                if s < nb and needs[nseg + nw + s]:
+                    dbs[s] = torch.empty(n, dtype=torch.float32, device=device)
+                db = dbs[s] if s < nb else None
+                if dx is None and dwp is None and db is None:
+                    continue
+                xc = rt.dtype_code(dx) if dx is not None else rt.DTYPE_F32
+                work = torch.empty(int(lib.inf_linear_ckpt_workspace_bytes(rows, n, k, xc, 1)), dtype=torch.uint8,
+                                   device=device)
+                rt.check(lib.inf_linear_ckpt_backward(
+                    rows, n, k, rt.ptr(dy), dy.stride(0), act, rt.ptr(y), n, rt.ptr(mask), rt.ptr(q),
+                    q.stride(0) if q is not None else 0, rt.ptr(scale), W.data_ptr() + 4 * c0 * W.stride(1),
+                    W.stride(0), W.stride(1), rt.ptr(dx), xc, k, dwp, W.shape[1], rt.ptr(db), rt.ptr(work), st),
+                    "linear_ckpt_backward")
+        return (None, None, None, *dxs, *dws, *dbs)
+
+
+def _linear_ckpt(segments, spec, weights, biases, act, checkpoint):
+    kept = [checkpoint] * len(segments) if isinstance(checkpoint, str) else list(checkpoint)
+    if len(kept) != len(segments) or any(not isinstance(c, Rows8) and c != "int8" for c in kept):
+        raise ValueError('checkpoint is "int8", or for each segment "int8" or the Rows8 of its input')
+    if not segments or not weights or len(biases) > len(segments):
+        raise ValueError("linear takes at least one segment and at most one bias for each")
+    if max(w for w, _ in spec) + 1 != len(weights) or min(w for w, _ in spec) < 0:
+        raise ValueError("every weight belongs to a segment")
+    xs = [x if x.dtype in (torch.float32, torch.bfloat16) else x.to(torch.float32) for x, _, _ in segments]
+    xs = [_rows_of(x, "x") for x in xs]
+    rows, device = xs[0].shape[0], xs[0].device
+    n = weights[0].shape[0]
+    for t in (*xs, *weights, *biases):
+        if t.device != device:
+            raise ValueError("linear takes its tensors on one device")
+    for W in weights:
+        if W.dim() != 2 or W.dtype != torch.float32 or W.shape[0] != n or n < 1:
+            raise ValueError("weights are fp32 matrices with the same number of rows")
+    for b in biases:
+        if b.shape != (n,) or b.dtype != torch.float32 or not b.is_contiguous():
+            raise ValueError("a bias is a contiguous fp32 [n] tensor")
+    taken = {}
+    for (wi, c0), x, c in zip(spec, xs, kept):
+        k = x.shape[1]
+        if x.shape[0] != rows or c0 < 0 or c0 + k > weights[wi].shape[1]:
+            raise ValueError(f"x {list(x.shape)} at column {c0} does not fit weight {list(weights[wi].shape)}")
+        if any(c0 < b and a < c0 + k for a, b in taken.setdefault(wi, [])):
+            raise ValueError("segments of one weight take separate columns")
+        taken[wi].append((c0, c0 + k))
+        if isinstance(c, Rows8) and (c.shape != x.shape or c.device != device):
+            raise ValueError(f"checkpoint {list(c.shape)} is not of x {list(x.shape)}")
+    return _LinearCkpt.apply(spec, act, tuple(c if isinstance(c, Rows8) else None for c in kept), *xs, *weights,
+                             *biases)
 
 
 def view_angles(unit_dirs, face_idxs, face_normals):

@@ -15,7 +15,7 @@ LIB_PATH = os.environ.get("INF_LIB") or os.path.join(_HERE, "libinf_hip.so")
 
 # ---- constants (inf_hip.h) ---------------------------------------------------------
 INF_OK = 0
-DTYPE_F32, DTYPE_BF16, DTYPE_I32, DTYPE_I64 = 0, 1, 2, 3
+DTYPE_F32, DTYPE_BF16, DTYPE_I32, DTYPE_I64, DTYPE_I8 = 0, 1, 2, 3, 4
 MODE_FP32, MODE_BF16, MODE_BF16X3 = 0, 1, 2
 LOSS_L2, LOSS_L1, LOSS_CAUCHY = 0, 1, 2
 LOSS_CODES = {"L2": LOSS_L2, "L1": LOSS_L1, "cauchy": LOSS_CAUCHY}
@@ -85,6 +85,20 @@ _SIGNATURES = {
     "inf_ff_encode": (c_int, [c_int64, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_void_p]),
     "inf_uv_fill_holes": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "inf_masked_sse": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
+    "inf_quantize_rows": (c_int, [c_void_p, c_int, c_int64, c_int, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    "inf_restore_rows": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int, c_int64, c_void_p]),
+    "inf_packed_weight_bytes": (c_int64, [c_int, c_int]),
+    "inf_pack_weight": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p]),
+    "inf_linear_int_workspace_bytes": (c_int64, [c_int64, c_int, c_int, c_int, c_int]),
+    "inf_linear_int": (c_int, [c_int64, c_int, c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                               c_void_p, c_int64, c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p]),
+    "inf_linear_ckpt_workspace_bytes": (c_int64, [c_int64, c_int, c_int, c_int, c_int]),
+    "inf_linear_ckpt_forward": (c_int, [c_int64, c_int, c_int, c_void_p, c_int, c_int64, c_void_p, c_int64, c_int64,
+                                        c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p,
+                                        c_int64, c_void_p, c_void_p, c_void_p]),
+    "inf_linear_ckpt_backward": (c_int, [c_int64, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p,
+                                         c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int,
+                                         c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
     "inf_plan_create": (c_int, [ctypes.POINTER(MlpDesc), c_int, ctypes.POINTER(c_void_p)]),
     "inf_plan_destroy": (None, [c_void_p]),
     "inf_plan_get_info": (c_int, [c_void_p, ctypes.POINTER(PlanInfo)]),

@@ -75,6 +75,7 @@ class LinearWithConcatAndActivation(nn.Module):
         self.Lx = nn.Linear(x_in_dim, out_dim)
         self.Ly = nn.Linear(y_in_dim, out_dim)
         self.actn = activation()
+        self.checkpoint = None  # None or "int8": what dense.linear keeps of x and y until the backward
         self.batchnorm = None
         if batchnorm:
             self.batchnorm = nn.BatchNorm1d(out_dim)
@@ -89,5 +90,6 @@ class LinearWithConcatAndActivation(nn.Module):
             raise NotImplementedError("only the ReLU activation is implemented")
         lead = x.shape[:-1]
         out = dense.linear([(x.reshape(-1, x.shape[-1]), 0, 0), (y.reshape(-1, y.shape[-1]), 1, 0)],
-                           [self.Lx.weight, self.Ly.weight], [self.Lx.bias, self.Ly.bias], "relu")
+                           [self.Lx.weight, self.Ly.weight], [self.Lx.bias, self.Ly.bias], "relu",
+                           checkpoint=self.checkpoint)
         return out.view(*lead, out.shape[-1])

@@ -9,11 +9,17 @@ into it), the kernels read packed GEMM-dtype copies that are refreshed whenever 
 parameter changes, and a batch whose features were not materialised is gathered inside
 the same launch sequence (mesh.py:313-324 fused into the forward).
 
+The layers outside the fused plan (the view-dependent field; dense.py) take two more keys of
+`model_config["kernels"]`: `dense_checkpoints: int8` keeps their inputs in 8 bits between
+forward and backward, `dense_inference: int8` runs them on 8-bit rows and weights wherever no
+gradient is recorded (rendering, evaluation).
+
 Kernel arithmetic mode: `model_config["kernels"]["mode"]` ("fp32" exact f32 MFMA, the
 default, or "bf16" MFMA with fp32 accumulation), overridable by INF_MODE.
 """
 from __future__ import annotations
 
+import contextlib
 import os
 import weakref
 
@@ -106,6 +112,7 @@ class TextureField(nn.Module):
 
         self.kernel_mode = os.environ.get("INF_MODE", "fp32")
         self.max_batch_hint = 4096
+        self.dense_checkpoints = None   # None or "int8": the dense layers' inputs until the backward
         self._rt: _Runtime | None = None
 
     # ---- device binding ----------------------------------------------------------
@@ -211,14 +218,39 @@ class TextureField(nn.Module):
             raise RuntimeError("TextureField runs on MI355X (HIP) devices only. There is no CPU fallback.")
         h = x
         n = len(self.layers)
+        kept = self.dense_checkpoints
+        # two layers read the features: their 8-bit rows are made once
+        kept_x = dense.quantize_rows(x) if kept == "int8" and torch.is_grad_enabled() else kept
         for i, layer in enumerate(self.layers):
             if i == self.skip_layer_idx:
                 h = dense.linear([(h, 0, 0), (x, 1, 0)], [layer.Lx.weight, layer.Ly.weight],
-                                 [layer.Lx.bias, layer.Ly.bias], "relu")
+                                 [layer.Lx.bias, layer.Ly.bias], "relu", checkpoint=kept and [kept, kept_x])
             else:
                 lin = layer[0]
                 act = "relu" if i < n - 1 or not self.return_rgb else "sigmoid"
-                h = dense.linear([(h, 0, 0)], [lin.weight], [lin.bias], act)
+                h = dense.linear([(h, 0, 0)], [lin.weight], [lin.bias], act,
+                                 checkpoint=kept and [kept if i else kept_x])
+        return h
+
+    def weights8(self):
+        """The layers' weights in 8 bits, laid out for dense.linear8: a list for each layer."""
+        import dense
+        return [[dense.quantize_weight(layer.Lx.weight), dense.quantize_weight(layer.Ly.weight)]
+                if i == self.skip_layer_idx else [dense.quantize_weight(layer[0].weight)]
+                for i, layer in enumerate(self.layers)]
+
+    def _dense_forward8(self, batch, weights, out=torch.float32):
+        """_dense_forward on 8-bit rows between the layers; out: as dense.linear8."""
+        import dense
+        h = x = dense.quantize_rows(self._input_features(batch))
+        n = len(self.layers)
+        for i, (layer, w) in enumerate(zip(self.layers, weights)):
+            to = torch.int8 if i < n - 1 else out
+            if i == self.skip_layer_idx:
+                h = dense.linear8([h, x], w, [layer.Lx.bias, layer.Ly.bias], "relu", out=to)
+            else:
+                act = "relu" if i < n - 1 or not self.return_rgb else "sigmoid"
+                h = dense.linear8([h], w, [layer[0].bias], act, out=to)
         return h
 
     def forward(self, batch):
@@ -350,6 +382,45 @@ class TextureFieldWithViewDependency(nn.Module):
         self.directional_mlp = nn.Sequential(nn.Linear(bottleneck_vec_dim + embedding_size, directional_hidden_dim),
                                              activation(), nn.Linear(directional_hidden_dim, RGB_COLOR_DIM),
                                              nn.Sigmoid())
+        self.dense_inference = None   # None or "int8": the layers where no gradient is recorded
+        self._weights8 = None
+
+    def set_dense_options(self, checkpoints=None, inference=None):
+        """checkpoints="int8": inputs kept in 8 bits until the backward (dense.linear);
+        inference="int8": 8-bit rows and weights where no gradient is recorded (dense.linear8)."""
+        for what in (checkpoints, inference):
+            if what not in (None, "int8"):
+                raise ValueError(f'dense layers have "int8" or nothing for checkpoints and inference, not {what!r}')
+        self.spatial_mlp.dense_checkpoints = checkpoints
+        self.dense_inference = inference
+
+    @contextlib.contextmanager
+    def weights_laid_out(self):
+        """With dense_inference="int8", the weights put into 8 bits once for the calls inside (a
+        frame's chunks) instead of once a call.  They must not change meanwhile."""
+        before = self._weights8
+        try:
+            if self.dense_inference == "int8":
+                self._weights8 = self._make_weights8()
+            yield self
+        finally:
+            self._weights8 = before
+
+    def _make_weights8(self):
+        import dense
+        l0, l2 = self.directional_mlp[0], self.directional_mlp[2]
+        return (self.spatial_mlp.weights8(), [dense.quantize_weight(l0.weight, 0, self.bottleneck_vec_dim),
+                                              dense.quantize_weight(l0.weight, self.bottleneck_vec_dim)],
+                [dense.quantize_weight(l2.weight)])
+
+    @torch.no_grad()
+    def _forward8(self, batch):
+        import dense
+        spatial, w0, w2 = self._weights8 or self._make_weights8()
+        l0, l2 = self.directional_mlp[0], self.directional_mlp[2]
+        bottleneck = self.spatial_mlp._dense_forward8(batch, spatial, out=torch.int8)
+        h = dense.linear8([bottleneck, self._get_embedded_view_dir(batch)], w0, [l0.bias], "relu", out=torch.int8)
+        return dense.linear8([h], w2, [l2.bias], "sigmoid")
 
     def _get_embedded_view_dir(self, batch):
         """model.py:162-172."""
@@ -365,11 +436,15 @@ class TextureFieldWithViewDependency(nn.Module):
         """model.py:174-177; the concatenation is two column ranges of the first
         directional weight."""
         import dense
+        if self.dense_inference == "int8" and not torch.is_grad_enabled():
+            return self._forward8(batch)
+        kept = self.spatial_mlp.dense_checkpoints
         bottleneck = self.spatial_mlp(batch)
         view = self._get_embedded_view_dir(batch)
         l0, l2 = self.directional_mlp[0], self.directional_mlp[2]
-        h = dense.linear([(bottleneck, 0, 0), (view, 0, self.bottleneck_vec_dim)], [l0.weight], [l0.bias], "relu")
-        return dense.linear([(h, 0, 0)], [l2.weight], [l2.bias], "sigmoid")
+        h = dense.linear([(bottleneck, 0, 0), (view, 0, self.bottleneck_vec_dim)], [l0.weight], [l0.bias], "relu",
+                         checkpoint=kept)
+        return dense.linear([(h, 0, 0)], [l2.weight], [l2.bias], "sigmoid", checkpoint=kept)
 
 
 def init_weights(m):
@@ -416,6 +491,12 @@ def make_model(model_config, mesh=None):
                                                batchnorm=model_config.get("batchnorm", False), activation=nn.ReLU)
     model.apply(init_weights)
     kernels = model_config.get("kernels") or {}
+    dense_options = {k: kernels.get(f"dense_{k}") for k in ("checkpoints", "inference")}
+    if isinstance(model, TextureFieldWithViewDependency):
+        model.set_dense_options(**dense_options)
+    elif any(dense_options.values()):
+        raise ValueError("kernels.dense_checkpoints / dense_inference are for the view-dependent field; the others "
+                         "run on the fused plan (kernels.mode)")
     model.kernel_mode = os.environ.get("INF_MODE", kernels.get("mode", "fp32"))
     if kernels.get("max_batch"):
         model.max_batch_hint = int(kernels["max_batch"])

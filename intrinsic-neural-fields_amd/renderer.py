@@ -14,6 +14,7 @@ hit_ray_idxs) overrides it.
 """
 from __future__ import annotations
 
+import contextlib
 import os
 
 import torch
@@ -119,9 +120,10 @@ class Renderer:
         key = "eigenfunctions" if self.feature_strategy == "efuncs" else "xyz"
         fill = 1.0 if self.background == "white" else 0.0
         img = torch.full((self.H * self.W, 3), fill, dtype=torch.float32, device=dev)
-        preds = [self.model({key: feats[lo:lo + RENDER_CHUNK], "unit_ray_dirs": unit_dirs[lo:lo + RENDER_CHUNK],
-                             "hit_face_idxs": face[lo:lo + RENDER_CHUNK]})
-                 for lo in range(0, feats.shape[0], RENDER_CHUNK)]
+        with getattr(self.model, "weights_laid_out", contextlib.nullcontext)():
+            preds = [self.model({key: feats[lo:lo + RENDER_CHUNK], "unit_ray_dirs": unit_dirs[lo:lo + RENDER_CHUNK],
+                                 "hit_face_idxs": face[lo:lo + RENDER_CHUNK]})
+                     for lo in range(0, feats.shape[0], RENDER_CHUNK)]
         if preds:
             pix = hit if obj_mask_1d is None else torch.nonzero(torch.as_tensor(obj_mask_1d).to(dev)).reshape(-1)[hit]
             img[pix] = torch.cat(preds)
