@@ -196,11 +196,11 @@ int inf_adam_dense(int64_t n, float* param, const float* grad, float* exp_avg, f
                    double lr, double beta1, double beta2, double eps, inf_stream_t stream);
 
 /* ---- dense layers in 8 bits ------------------------------------------------------ */
-/* Rows in 8 bits: scale[m] = fl32(max_k |x_mk| / 127), q_mk = the whole number nearest to
+/* Rows in 8 bits: scale[m] = fl(max_k |x_mk| fl(1 / 127)), q_mk = the whole number nearest to
  * 127 x_mk / max_k |x_mk| (the ratio itself; ties to even).  A row of zeros has scale 0; a
  * row with an infinity or a NaN has scale NaN and q 0.  x: fp32 / bf16, ld_x any (0 repeats
- * one row).  q rows start on 16 bytes: q 16-byte aligned, ld_q >= k a multiple of 16; what
- * lies behind column k is neither read as a value nor written.                            */
+ * one row).  q is rows of whole 16 bytes: 16-byte aligned, ld_q >= k a multiple of 16; its
+ * bytes behind column k do not matter to any reader and may be written.                   */
 int inf_quantize_rows(const void* x, int x_dtype, int64_t rows, int k, int64_t ld_x, int8_t* q, int64_t ld_q,
                       float* scale, inf_stream_t stream);
 /* out[m][j] = q[m][j] scale[m], rounded once to fp32 / bf16. */

@@ -1,7 +1,7 @@
 // Rows in 8-bit whole numbers with a scale each: the arithmetic that csrc/rows8.hip,
 // linear8.hip and ckpt.hip share.
 //
-//   a_m = max_k |x_mk|    s_m = fl32(a_m / 127)    q_mk = nearest whole number to 127 x_mk / a_m
+//   a_m = max_k |x_mk|    s_m = fl(a_m fl(1 / 127))    q_mk = nearest whole number to 127 x_mk / a_m
 //
 // q goes by the ratio itself (ties to even), not by a rounded quotient: the same numbers
 // whichever kernel makes them.  A row of zeros has s = 0 and q = 0; a row with an infinity
@@ -37,7 +37,7 @@ __device__ __forceinline__ RowScale row_scale(unsigned amax_bits) {
   RowScale o;
   const float a = __uint_as_float(amax_bits);
   const bool finite = amax_bits < 0x7f800000u;
-  o.s = finite ? __fdiv_rn(a, 127.f) : __uint_as_float(0x7fc00000u);
+  o.s = finite ? a * (1.f / 127.f) : __uint_as_float(0x7fc00000u);
   o.up = a < 0x1p-90f ? 0x1p64f : 1.f;
   o.a = a * o.up;
   o.r = finite && amax_bits != 0 ? 127.f / o.a : 0.f;
@@ -58,6 +58,12 @@ __device__ __forceinline__ int quantize(float x, const RowScale& rs) {
     q = t < 0.f ? -m : m;
   }
   return q;
+}
+
+// four values as the bytes of a word
+__device__ __forceinline__ uint32_t quantize4(float x0, float x1, float x2, float x3, const RowScale& rs) {
+  return (uint32_t)(uint8_t)quantize(x0, rs) | (uint32_t)(uint8_t)quantize(x1, rs) << 8 |
+         (uint32_t)(uint8_t)quantize(x2, rs) << 16 | (uint32_t)quantize(x3, rs) << 24;
 }
 
 // relu keeps a NaN (fmaxf would make it 0); sigmoid as csrc/dense.hip

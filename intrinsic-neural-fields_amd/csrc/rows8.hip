@@ -11,34 +11,134 @@ namespace {
 
 using namespace q8;
 
+// A row is held in the registers of LPR lanes (4, 16 or 64), CH chunks of 16 bytes of x a
+// lane, between its maximum and its rounding: x is read once, with 16-byte loads, and the
+// rows of a wave's other lanes keep more loads on their way.  Bound by bytes.
+// Loads and stores of a whole chunk need their element's alignment only (rows of odd
+// lengths: k = 1023).
+template <typename T> struct Chunk;
+template <> struct Chunk<float> {
+  static constexpr int V = 4;
+  typedef float X __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <> struct Chunk<bf16> {
+  static constexpr int V = 8;
+  typedef bf16 X __attribute__((ext_vector_type(8), aligned(2)));
+};
+
+// columns [c, c + V) of a row; those from k on are zero
 template <typename T>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int k, int64_t ldx,
-                                                            int8_t* __restrict__ q, int64_t ldq,
-                                                            float* __restrict__ scale) {
-  __shared__ unsigned part[256];
-  for (int64_t m = blockIdx.x; m < rows; m += gridDim.x) {
-    unsigned a = 0;
-    for (int j = threadIdx.x; j < k; j += 256) a = max(a, abs_bits(to_f32(x[m * ldx + j])));
-    part[threadIdx.x] = a;
-    __syncthreads();
-    for (int h = 128; h > 0; h >>= 1) {
-      if (threadIdx.x < h) part[threadIdx.x] = max(part[threadIdx.x], part[threadIdx.x + h]);
-      __syncthreads();
-    }
-    const RowScale rs = row_scale(part[0]);
-    __syncthreads();
-    for (int j = threadIdx.x; j < k; j += 256) q[m * ldq + j] = (int8_t)quantize(to_f32(x[m * ldx + j]), rs);
-    if (threadIdx.x == 0) scale[m] = rs.s;
+__device__ __forceinline__ void load_chunk(const T* row, int c, int k, float (&v)[Chunk<T>::V]) {
+  constexpr int V = Chunk<T>::V;
+  if (c + V <= k) {
+    const typename Chunk<T>::X x = *reinterpret_cast<const typename Chunk<T>::X*>(row + c);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = (float)x[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = c + e < k ? to_f32(row[c + e]) : 0.f;
   }
 }
 
+template <int LPR>
+__device__ __forceinline__ unsigned row_max(unsigned a) {
+#pragma unroll
+  for (int h = LPR / 2; h > 0; h >>= 1) a = max(a, (unsigned)__shfl_xor((int)a, h));
+  return a;
+}
+
+template <typename T, int LPR, int CH>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int k, int64_t ldx,
+                                                            int8_t* __restrict__ q, int64_t ldq,
+                                                            float* __restrict__ scale) {
+  constexpr int V = Chunk<T>::V;
+  const int64_t m = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const int l = threadIdx.x % LPR;
+  if (m >= rows) return;  // whole rows of lanes: the exchanges below stay within a row
+  float v[CH][V];
+  unsigned a = 0;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) load_chunk(x + m * ldx, (i * LPR + l) * V, k, v[i]);
+#pragma unroll
+  for (int i = 0; i < CH; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) a = max(a, abs_bits(v[i][e]));
+  const RowScale rs = row_scale(row_max<LPR>(a));
+  if (l == 0) scale[m] = rs.s;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int c = (i * LPR + l) * V;
+    if (c >= k) break;
+    uint32_t w[V / 4];
+#pragma unroll
+    for (int e = 0; e < V; e += 4) w[e / 4] = quantize4(v[i][e], v[i][e + 1], v[i][e + 2], v[i][e + 3], rs);
+    int8_t* const to = q + m * ldq + c;
+    if (c + V <= k) {
+#pragma unroll
+      for (int e = 0; e < V / 4; ++e) reinterpret_cast<uint32_t*>(to)[e] = w[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (c + e < k) to[e] = (int8_t)(w[e / 4] >> (8 * (e % 4)));
+    }
+  }
+}
+
+// Rows too long for a wave's registers: a workgroup a row, which is read twice.
 template <typename T>
+__global__ __launch_bounds__(256) void quantize_long_rows_kernel(const T* __restrict__ x, int64_t rows, int k,
+                                                                 int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
+                                                                 float* __restrict__ scale) {
+  constexpr int V = Chunk<T>::V;
+  __shared__ unsigned part[4];
+  for (int64_t m = blockIdx.x; m < rows; m += gridDim.x) {
+    unsigned a = 0;
+    float v[V];
+    for (int c = threadIdx.x * V; c < k; c += 256 * V) {
+      load_chunk(x + m * ldx, c, k, v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) a = max(a, abs_bits(v[e]));
+    }
+    a = row_max<64>(a);
+    __syncthreads();  // the last row's maximum has been read
+    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = a;
+    __syncthreads();
+    const RowScale rs = row_scale(max(max(part[0], part[1]), max(part[2], part[3])));
+    if (threadIdx.x == 0) scale[m] = rs.s;
+    for (int c = threadIdx.x * V; c < k; c += 256 * V) {
+      load_chunk(x + m * ldx, c, k, v);
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (c + e < k) q[m * ldq + c + e] = (int8_t)quantize(v[e], rs);
+    }
+  }
+}
+
+// LPR lanes a row, each lane 4 values a turn (one 4-byte load, one 16- or 8-byte store).
+template <typename T, int LPR>
 __global__ __launch_bounds__(256) void restore_rows_kernel(const int8_t* __restrict__ q, int64_t ldq,
                                                            const float* __restrict__ scale, int64_t rows, int k,
                                                            T* __restrict__ out, int64_t ldo) {
-  for (int64_t m = blockIdx.x; m < rows; m += gridDim.x) {
-    const float s = scale[m];
-    for (int j = threadIdx.x; j < k; j += 256) out[m * ldo + j] = from_f32<T>((float)q[m * ldq + j] * s);
+  typedef T O __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  const int64_t m = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  if (m >= rows) return;
+  const float s = scale[m];
+  const int8_t* const from = q + m * ldq;
+  T* const to = out + m * ldo;
+#pragma unroll 4
+  for (int c = (threadIdx.x % LPR) * 4; c < k; c += LPR * 4) {
+    // q rows start on 16 bytes and their length is a multiple: a whole load stays in the row
+    const int w = *reinterpret_cast<const int*>(from + c);
+    O o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = from_f32<T>((float)(int8_t)(w >> (8 * e)) * s);
+    if (c + 4 <= k) {
+      *reinterpret_cast<O*>(to + c) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < k) to[c + e] = o[e];
+    }
   }
 }
 
@@ -55,12 +155,39 @@ unsigned blocks_of(int64_t n) { return (unsigned)std::min<int64_t>(std::max<int6
 
 }  // namespace
 
+template <typename T>
+static void quantize_rows_any(const T* x, int64_t rows, int k, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
+                              hipStream_t st) {
+  constexpr int V = Chunk<T>::V;
+  const int chunks = (int)ceil_div(k, V);
+  auto grid = [&](int lpr) { return (unsigned)ceil_div(rows, 256 / lpr); };
+#define INF_Q(LPR, CH) quantize_rows_kernel<T, LPR, CH><<<grid(LPR), 256, 0, st>>>(x, rows, k, ldx, q, ldq, scale)
+  // the fewest lanes that hold a row in one chunk each, then more chunks a lane; 64 values a
+  // lane is the most that still leaves several waves a SIMD
+  if (chunks <= 4) INF_Q(4, 1);
+  else if (chunks <= 16) INF_Q(16, 1);
+  else if (chunks <= 64) INF_Q(64, 1);
+  else if (chunks <= 128) INF_Q(64, 2);
+  else if (chunks <= 256) INF_Q(64, 4);
+  else if (chunks <= 512) INF_Q(64, 8);
+  else if (V == 4 && chunks <= 1024) INF_Q(64, V == 4 ? 16 : 8);
+  else quantize_long_rows_kernel<<<blocks_of(rows), 256, 0, st>>>(x, rows, k, ldx, q, ldq, scale);
+#undef INF_Q
+}
+
+template <typename T>
+static void restore_rows_any(const int8_t* q, int64_t ldq, const float* scale, int64_t rows, int k, T* out,
+                             int64_t ldo, hipStream_t st) {
+  if (k <= 16) restore_rows_kernel<T, 4><<<(unsigned)ceil_div(rows, 64), 256, 0, st>>>(q, ldq, scale, rows, k, out, ldo);
+  else if (k <= 64) restore_rows_kernel<T, 16><<<(unsigned)ceil_div(rows, 16), 256, 0, st>>>(q, ldq, scale, rows, k, out, ldo);
+  else if (k <= 4096) restore_rows_kernel<T, 64><<<(unsigned)ceil_div(rows, 4), 256, 0, st>>>(q, ldq, scale, rows, k, out, ldo);
+  else restore_rows_kernel<T, 256><<<(unsigned)rows, 256, 0, st>>>(q, ldq, scale, rows, k, out, ldo);
+}
+
 int launch_quantize_rows(const void* x, int dtype, int64_t rows, int k, int64_t ldx, int8_t* q, int64_t ldq,
                          float* scale, hipStream_t stream) {
-  if (dtype == INF_DTYPE_F32)
-    quantize_rows_kernel<<<blocks_of(rows), 256, 0, stream>>>((const float*)x, rows, k, ldx, q, ldq, scale);
-  else
-    quantize_rows_kernel<<<blocks_of(rows), 256, 0, stream>>>((const bf16*)x, rows, k, ldx, q, ldq, scale);
+  if (dtype == INF_DTYPE_F32) quantize_rows_any((const float*)x, rows, k, ldx, q, ldq, scale, stream);
+  else quantize_rows_any((const bf16*)x, rows, k, ldx, q, ldq, scale, stream);
   INF_LAUNCH_CHECK();
   return INF_OK;
 }
@@ -76,6 +203,7 @@ int inf_quantize_rows(const void* x, int x_dtype, int64_t rows, int k, int64_t l
   INF_CHECK_ARG(rows >= 0 && k >= 1 && ld_x >= 0, "quantize_rows: bad shape");
   INF_CHECK_ARG(x_dtype == INF_DTYPE_F32 || x_dtype == INF_DTYPE_BF16, "quantize_rows: x must be fp32 or bf16");
   INF_CHECK_ARG(ld_q >= k && ld_q % q8::Q_ALIGN == 0, "quantize_rows: q rows must start on 16 bytes");
+  INF_CHECK_ARG(rows < (int64_t)1 << 31, "quantize_rows: too many rows");
   if (rows == 0) return INF_OK;
   INF_CHECK_ARG(x != nullptr && q != nullptr && scale != nullptr && (uintptr_t)q % 16 == 0,
                 "quantize_rows: null or unaligned argument");
@@ -87,13 +215,12 @@ int inf_restore_rows(const int8_t* q, int64_t ld_q, const float* scale, int64_t 
   INF_CHECK_ARG(rows >= 0 && k >= 1 && ld_out >= k, "restore_rows: bad shape");
   INF_CHECK_ARG(out_dtype == INF_DTYPE_F32 || out_dtype == INF_DTYPE_BF16, "restore_rows: out must be fp32 or bf16");
   INF_CHECK_ARG(ld_q >= k && ld_q % q8::Q_ALIGN == 0, "restore_rows: q rows must start on 16 bytes");
+  INF_CHECK_ARG(rows < (int64_t)1 << 31, "restore_rows: too many rows");
   if (rows == 0) return INF_OK;
   INF_CHECK_ARG(q != nullptr && scale != nullptr && out != nullptr && (uintptr_t)q % 16 == 0,
                 "restore_rows: null or unaligned argument");
-  if (out_dtype == INF_DTYPE_F32)
-    restore_rows_kernel<<<blocks_of(rows), 256, 0, (hipStream_t)stream>>>(q, ld_q, scale, rows, k, (float*)out, ld_out);
-  else
-    restore_rows_kernel<<<blocks_of(rows), 256, 0, (hipStream_t)stream>>>(q, ld_q, scale, rows, k, (bf16*)out, ld_out);
+  if (out_dtype == INF_DTYPE_F32) restore_rows_any(q, ld_q, scale, rows, k, (float*)out, ld_out, (hipStream_t)stream);
+  else restore_rows_any(q, ld_q, scale, rows, k, (bf16*)out, ld_out, (hipStream_t)stream);
   INF_LAUNCH_CHECK();
   return INF_OK;
 }

@@ -3,8 +3,8 @@ implementations in 64 bits.
 
 Tolerances.  u = 2^-24 is half a step of fp32, relative; U that of the output's type (bf16
 2^-8 / 2 = 2^-9 of a value's own power of two, at most 2^-8 / 2 relative: finfo.eps / 2).
-  rows in 8 bits: q equal; scale and restored values one rounding each (scale: 1 u, value:
-    2 u more with the scale's, then U).
+  rows in 8 bits: q equal; the scale has two roundings (1 / 127 and its product with the
+    maximum): 2 u and u^2; a restored value, from the scale as it is, one: u or U.
   linear8: acc is exact, then fl(acc), fl(sx sw), their product, the bias, the sum over
     segments: |error| <= 5 u (sum_s |acc t| + |bias|) a segment, plus U |y| for the output;
     sx and sw have one rounding each, which the oracle takes over (it reads the scales).
@@ -54,7 +54,7 @@ def check_rows(x, r):
     assert torch.equal(r.q.cpu(), torch.from_numpy(q))
     got = r.scale.cpu().double().numpy()
     assert np.array_equal(np.isnan(got), np.isnan(s))
-    np.testing.assert_allclose(got, s, rtol=U32, atol=2.0 ** -150)
+    np.testing.assert_allclose(got, s, rtol=2 * U32 + U32 ** 2, atol=2.0 ** -150)
 
 
 SHAPES = [(1, 1), (1, 3), (7, 3), (5, 15), (3, 16), (2, 17), (9, 63), (4, 64), (33, 65), (3, 127), (2, 256), (5, 255),

@@ -62,7 +62,7 @@ def layers64(m, batch):
 
     def put(z):  # fp32 rows into 8 bits
         q, _ = oracle_rows(z)
-        s = (z.abs().amax(1) / 127.0).float()
+        s = z.abs().amax(1).float() * torch.tensor(1.0 / 127.0, dtype=torch.float32)
         return torch.from_numpy(q).double(), s
 
     def lin(xs, ws, bs, act):
