@@ -4,14 +4,19 @@
 //   y      = act(z), as fp32, bf16, or in 8-bit rows again
 // The roundings are written out one by one and never contracted: a row that goes into 8
 // bits again has the same numbers whichever kernel made it.
+//
+// Two kernels.  Up to 16 rows: linear8_few_kernel, one launch, bound by its latency and by
+// reading the weights once.  More: x goes into 8 bits in a launch of its own (rows8.hip: a
+// row's maximum is needed before its first product), then linear8_tile_kernel.
 #include <algorithm>
 
-#include "quant.hpp"
+#include "mtile.hpp"
 
 namespace inf {
 namespace {
 
 using namespace q8;
+using namespace mt;
 
 struct Linear8Args {
   int64_t rows;
@@ -28,6 +33,7 @@ struct Linear8Args {
   int act;
   void* out;
   int64_t ldo;
+  float* os;  // scales of an int8 result
 };
 
 __device__ __forceinline__ float combine(int acc, float sx, float sw, float bias, float add, int act) {
@@ -38,54 +44,311 @@ __device__ __forceinline__ float combine(int acc, float sx, float sw, float bias
   return activate(z, act);
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void linear8_kernel(Linear8Args a) {
-  __shared__ int As[64][17], Bs[64][17];  // 64 rows of 64 values each
-  const int t = threadIdx.x;
-  const int tm = (t / 16) * 4, tn = (t % 16) * 4;
-  const int n0 = blockIdx.x * 64;
-  for (int64_t m0 = (int64_t)blockIdx.y * 64; m0 < a.rows; m0 += (int64_t)gridDim.y * 64) {
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < a.k; k0 += 64) {
-      for (int i = t; i < 64 * 16; i += 256) {
-        const int r = i / 16, c = i % 16;
-        int av = 0, bv = 0;
-        for (int e = 0; e < 4; ++e) {
-          const int kk = k0 + 4 * c + e;
-          if (kk < a.k && m0 + r < a.rows) av |= (int)(uint8_t)a.q[(m0 + r) * a.ldq + kk] << (8 * e);
-          if (kk < a.k && n0 + r < a.n) bv |= (int)(uint8_t)a.w[(int64_t)(n0 + r) * a.ldw + kk] << (8 * e);
-        }
-        As[r][c] = av;
-        Bs[r][c] = bv;
-      }
-      __syncthreads();
-      for (int c = 0; c < 16; ++c)
+// four neighbouring results of a row, as they are stored
+template <typename T> struct Four;
+template <> struct Four<float> { typedef float V __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Four<bf16> { typedef bf16 V __attribute__((ext_vector_type(4), aligned(2))); };
+
+// ---- tiles ---------------------------------------------------------------------------
+// BM rows of x by BN rows of the weight a workgroup, WM x WN waves, v_mfma_i32_16x16x64_i8.
+// The weight is the instruction's first operand, so that a lane holds four neighbouring
+// outputs of one row.  Per turn 128 values of k: both operands go straight from memory to LDS
+// (two stages: the next one is on its way while this one is multiplied).  Behind k the
+// weight's rows are zero, so what x's side reads there does not matter; rows past the end are
+// the last row again and are not stored.
+// T = int8_t: a row of the result goes into 8 bits here; BN holds all of its n values.
+template <int BM, int BN, int WM, int WN>
+struct L8 {
+  static constexpr int THREADS = 64 * WM * WN;
+  static constexpr int WROWS = BM / WM, WCOLS = BN / WN, TI = WROWS / 16, TJ = WCOLS / 16;
+  static constexpr int STAGE = (BM + BN) * 128, LDS = 2 * STAGE;
+  static constexpr int LOADS = STAGE / (THREADS * 16);
+  static_assert(STAGE % (THREADS * 16) == 0 && LDS <= 160 * 1024 && TI >= 1 && TJ >= 1, "tile");
+  static_assert(BM * WN * 4 + BM * BN <= LDS, "the result's image fits the stages");
+};
+
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void linear8_tile_kernel(Linear8Args a, int tiles_n, int nblocks) {
+  using P = L8<BM, BN, WM, WN>;
+  constexpr int TI = P::TI, TJ = P::TJ;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int bid = xcd_order((int)blockIdx.x, nblocks);
+  const int64_t m0 = (int64_t)(bid / tiles_n) * BM;
+  const int n0 = (bid % tiles_n) * BN;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave / WN, wc = wave % WN, r16 = lane & 15, g4 = lane >> 4;
+
+  const char* src[P::LOADS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            acc[i][j] = __builtin_amdgcn_sdot4(As[tm + i][c], Bs[tn + j][c], acc[i][j], false);
-      __syncthreads();
+  for (int i = 0; i < P::LOADS; ++i) {
+    const int p = tid + P::THREADS * i, row = p >> 3;
+    const int c = (p & 7) ^ swz(row);  // LDS is filled in order: the swizzle is the source's
+    if (row < BN) {
+      src[i] = reinterpret_cast<const char*>(a.w + min(n0 + row, a.n - 1) * a.ldw) + c * 16;
+    } else {
+      src[i] = reinterpret_cast<const char*>(a.q + min(m0 + row - BN, a.rows - 1) * a.ldq) + c * 16;
     }
-    for (int i = 0; i < 4; ++i)
-      for (int j = 0; j < 4; ++j) {
-        const int64_t m = m0 + tm + i;
-        const int n = n0 + tn + j;
-        if (m >= a.rows || n >= a.n) continue;
-        const float y = combine(acc[i][j], a.qs[m], a.ws[n], a.bias != nullptr ? a.bias[n] : 0.f,
-                                a.add != nullptr ? a.add[m * a.ldadd + n] : 0.f, a.act);
-        reinterpret_cast<T*>(a.out)[m * a.ldo + n] = from_f32<T>(y);
+  }
+  auto issue = [&](int t) {
+    char* st = smem + (t & 1) * P::STAGE;
+#pragma unroll
+    for (int i = 0; i < P::LOADS; ++i) {
+      const char* from = src[i] + t * 128;
+      __builtin_amdgcn_global_load_lds(from, (lds_void*)(st + (wave + (P::THREADS / 64) * i) * 1024), 16, 0, 0);
+    }
+  };
+  i32x4 acc[TJ][TI];
+#pragma unroll
+  for (int j = 0; j < TJ; ++j)
+#pragma unroll
+    for (int i = 0; i < TI; ++i) acc[j][i] = i32x4{0, 0, 0, 0};
+
+  const int turns = (int)(a.ldw / 128);
+  issue(0);
+#pragma unroll 1
+  for (int t = 0; t < turns; ++t) {
+    wait_all_barrier();
+    if (t + 1 < turns) issue(t + 1);
+    const char* st = smem + (t & 1) * P::STAGE;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      i32x4 wf[TJ], xf[TI];
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+        wf[j] = *reinterpret_cast<const i32x4*>(st + chunk_at(wc * P::WCOLS + 16 * j + r16, 4 * h + g4));
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+        xf[i] = *reinterpret_cast<const i32x4*>(st + chunk_at(BN + wr * P::WROWS + 16 * i + r16, 4 * h + g4));
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+#pragma unroll
+        for (int i = 0; i < TI; ++i)
+          acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[i], acc[j][i], 0, 0, 0);
+    }
+  }
+
+  // lane: row wr WROWS + 16 i + r16, columns wc WCOLS + 16 j + 4 g4 + (0..3)
+  float z[TJ][TI][4];
+  float sx[TI];
+#pragma unroll
+  for (int i = 0; i < TI; ++i) sx[i] = a.qs[min(m0 + wr * P::WROWS + 16 * i + r16, a.rows - 1)];
+#pragma unroll
+  for (int j = 0; j < TJ; ++j) {
+    const int n = n0 + wc * P::WCOLS + 16 * j + 4 * g4;
+    float sw[4], bias[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sw[e] = a.ws[min(n + e, a.n - 1)];
+      bias[e] = a.bias != nullptr ? a.bias[min(n + e, a.n - 1)] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      const int64_t m = m0 + wr * P::WROWS + 16 * i + r16;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float add = a.add != nullptr && m < a.rows && n + e < a.n ? a.add[m * a.ldadd + n + e] : 0.f;
+        z[j][i][e] = combine(acc[j][i][e], sx[i], sw[e], bias[e], add, a.act);
       }
+    }
+  }
+  if constexpr (sizeof(T) == 1) {
+    unsigned* const top = reinterpret_cast<unsigned*>(smem);  // [BM][WN]
+    char* const image = smem + BM * WN * 4;                    // [BM][BN]
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      unsigned b = 0;
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (wc * P::WCOLS + 16 * j + 4 * g4 + e < a.n) b = max(b, abs_bits(z[j][i][e]));
+      b = max(b, (unsigned)__shfl_xor((int)b, 16));
+      b = max(b, (unsigned)__shfl_xor((int)b, 32));
+      if (g4 == 0) top[(wr * P::WROWS + 16 * i + r16) * WN + wc] = b;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      const int row = wr * P::WROWS + 16 * i + r16;
+      unsigned b = 0;
+#pragma unroll
+      for (int v = 0; v < WN; ++v) b = max(b, top[row * WN + v]);
+      const RowScale rs = row_scale(b);
+      if (wc == 0 && g4 == 0 && m0 + row < a.rows) a.os[m0 + row] = rs.s;
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) {
+        const int col = wc * P::WCOLS + 16 * j + 4 * g4;
+        *reinterpret_cast<uint32_t*>(image + row * BN + (((col >> 4) ^ (row & (BN / 16 - 1))) << 4) + (col & 15)) =
+            quantize4(z[j][i][0], z[j][i][1], z[j][i][2], z[j][i][3], rs);
+      }
+    }
+    __syncthreads();
+    // whole 16-byte pieces: q rows are multiples of 16, so a piece that begins before n fits
+    for (int p = tid; p < BM * (BN / 16); p += P::THREADS) {
+      const int row = p / (BN / 16), c = p % (BN / 16);
+      if (m0 + row < a.rows && c * 16 < a.n)
+        *reinterpret_cast<u32x4*>((int8_t*)a.out + (m0 + row) * a.ldo + c * 16) =
+            *reinterpret_cast<const u32x4*>(image + row * BN + ((c ^ (row & (BN / 16 - 1))) << 4));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+      const int n = n0 + wc * P::WCOLS + 16 * j + 4 * g4;
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        const int64_t m = m0 + wr * P::WROWS + 16 * i + r16;
+        if (m >= a.rows) continue;
+        T* const to = reinterpret_cast<T*>(a.out) + m * a.ldo + n;
+        if (n + 4 <= a.n) {
+          typename Four<T>::V v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = from_f32<T>(z[j][i][e]);
+          *reinterpret_cast<typename Four<T>::V*>(to) = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < a.n) to[e] = from_f32<T>(z[j][i][e]);
+        }
+      }
+    }
   }
 }
 
-int launch_linear8(const Linear8Args& a, int out_dtype, hipStream_t stream) {
-  const dim3 grid((unsigned)ceil_div(a.n, 64), (unsigned)std::min<int64_t>(ceil_div(a.rows, 64), 65535));
-  if (out_dtype == INF_DTYPE_BF16) linear8_kernel<bf16><<<grid, 256, 0, stream>>>(a);
-  else linear8_kernel<float><<<grid, 256, 0, stream>>>(a);
+// ---- up to 16 rows -------------------------------------------------------------------
+// A workgroup makes 16 columns of every row, its four waves a quarter of the turns each, and
+// adds their sums in LDS.  It puts x into 8 bits itself (all workgroups the same numbers):
+// one launch, and x is small next to the weight.  X: float, bf16, or int8_t rows.
+constexpr int FEW = 16;
+constexpr int FEW_LDS = 128 * 1024;  // x in 8 bits: 16 rows of up to 8 K
+
+template <typename X, typename T>
+__global__ __launch_bounds__(256) void linear8_few_kernel(Linear8Args a, const X* __restrict__ x, int64_t ldx,
+                                                          int log_rows) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ unsigned top[FEW];
+  __shared__ int part[4][16][FEW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g4 = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const int ld = (int)a.ldw + 16;  // LDS rows: 16 bytes apart in the banks
+  const int rows = (int)a.rows;
+  const int turns = (int)(a.ldw / 64);
+  const int8_t* const wrow = a.w + min(n0 + r16, a.n - 1) * a.ldw + 16 * g4;
+  constexpr int AHEAD = 4;
+  i32x4 wf[AHEAD];
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u) {  // on their way while x is put into 8 bits
+    const int t = wave + 4 * u;
+    if (t < turns) wf[u] = *reinterpret_cast<const i32x4*>(wrow + t * 64);
+  }
+  // 256 >> log_rows threads a row, 16 bytes of the result each
+  const int per = 256 >> log_rows, m = tid / per, l = tid % per;
+  if constexpr (sizeof(X) == 1) {
+    if (m < rows)
+      for (int c = l * 16; c < a.ldw; c += per * 16)
+        *reinterpret_cast<i32x4*>(smem + m * ld + c) =
+            c < a.k ? *reinterpret_cast<const i32x4*>(x + m * ldx + c) : i32x4{0, 0, 0, 0};
+  } else {
+    if (tid < FEW) top[tid] = 0;
+    __syncthreads();
+    if (m < rows) {
+      unsigned b = 0;
+      for (int c = l; c < a.k; c += per) b = max(b, abs_bits(to_f32(x[m * ldx + c])));
+      atomicMax(&top[m], b);
+    }
+    __syncthreads();
+    if (m < rows) {
+      const RowScale rs = row_scale(top[m]);
+      for (int c = l * 4; c < a.ldw; c += per * 4) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = c + e < a.k ? to_f32(x[m * ldx + c + e]) : 0.f;
+        *reinterpret_cast<uint32_t*>(smem + m * ld + c) = quantize4(v[0], v[1], v[2], v[3], rs);
+      }
+    }
+  }
+  __syncthreads();
+  i32x4 acc = {0, 0, 0, 0};
+  // rows past the end read row 0; their sums are not stored
+  const char* const xrow = smem + (r16 < rows ? r16 : 0) * ld + 16 * g4;
+  for (int t0 = wave; t0 < turns; t0 += 4 * AHEAD) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int t = t0 + 4 * u;
+      if (t < turns) {
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], *reinterpret_cast<const i32x4*>(xrow + t * 64), acc, 0, 0, 0);
+        if (t + 4 * AHEAD < turns) wf[u] = *reinterpret_cast<const i32x4*>(wrow + (t + 4 * AHEAD) * 64);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) part[wave][4 * g4 + e][r16] = acc[e];
+  __syncthreads();
+  const int r = tid / 16, n = n0 + tid % 16;
+  if (r < rows && n < a.n) {
+    const int sum = part[0][tid % 16][r] + part[1][tid % 16][r] + part[2][tid % 16][r] + part[3][tid % 16][r];
+    const float sx = sizeof(X) == 1 ? a.qs[r] : row_scale(top[r]).s;
+    const float y = combine(sum, sx, a.ws[n], a.bias != nullptr ? a.bias[n] : 0.f,
+                            a.add != nullptr ? a.add[r * a.ldadd + n] : 0.f, a.act);
+    reinterpret_cast<T*>(a.out)[r * a.ldo + n] = from_f32<T>(y);
+  }
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+int launch_tile(const Linear8Args& a, hipStream_t stream) {
+  using P = L8<BM, BN, WM, WN>;
+  const int tiles_n = (int)ceil_div(a.n, BN);
+  const int64_t nblocks = ceil_div(a.rows, BM) * tiles_n;
+  INF_CHECK_ARG(nblocks < (int64_t)1 << 31, "linear_int: too many tiles");
+  static const hipError_t attr = hipFuncSetAttribute((const void*)linear8_tile_kernel<T, BM, BN, WM, WN>,
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
+  INF_HIP_TRY(attr);
+  linear8_tile_kernel<T, BM, BN, WM, WN>
+      <<<(unsigned)nblocks, P::THREADS, P::LDS, stream>>>(a, tiles_n, (int)nblocks);
   INF_LAUNCH_CHECK();
   return INF_OK;
 }
+
+// The widest tile that still gives every CU a workgroup (256 of them); a result in 8 bits
+// needs whole rows (n <= 256).
+template <typename T>
+int launch_tiles(const Linear8Args& a, hipStream_t stream) {
+  const int64_t wide = ceil_div(a.rows, 256);
+  if (a.n <= 32) return launch_tile<T, 256, 32, 4, 1>(a, stream);
+  if (a.n <= 128 && wide >= 256) return launch_tile<T, 256, 128, 4, 2>(a, stream);
+  if (a.n > 128 && wide * ceil_div(a.n, 256) >= 256) return launch_tile<T, 256, 256, 2, 4>(a, stream);
+  if (sizeof(T) == 1 && a.n > 64) return launch_tile<T, 64, 256, 1, 4>(a, stream);
+  return launch_tile<T, 64, 64, 2, 2>(a, stream);
+}
+
+int launch_linear8(const Linear8Args& a, int out_dtype, hipStream_t stream) {
+  if (out_dtype == INF_DTYPE_I8) return launch_tiles<int8_t>(a, stream);
+  if (out_dtype == INF_DTYPE_BF16) return launch_tiles<bf16>(a, stream);
+  return launch_tiles<float>(a, stream);
+}
+
+template <typename X, typename T>
+int launch_few(const Linear8Args& a, const X* x, int64_t ldx, hipStream_t stream) {
+  static const hipError_t attr = hipFuncSetAttribute((const void*)linear8_few_kernel<X, T>,
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, FEW_LDS);
+  INF_HIP_TRY(attr);
+  int log_rows = 0;
+  while ((1 << log_rows) < a.rows) ++log_rows;
+  linear8_few_kernel<X, T><<<(unsigned)ceil_div(a.n, 16), 256, (size_t)(a.rows * (a.ldw + 16)), stream>>>(a, x, ldx,
+                                                                                                       log_rows);
+  INF_LAUNCH_CHECK();
+  return INF_OK;
+}
+
+template <typename X>
+int launch_few_out(const Linear8Args& a, int out_dtype, const void* x, int64_t ldx, hipStream_t stream) {
+  if (out_dtype == INF_DTYPE_BF16) return launch_few<X, bf16>(a, (const X*)x, ldx, stream);
+  return launch_few<X, float>(a, (const X*)x, ldx, stream);
+}
+
+bool is_few(int64_t rows, int k) { return rows <= FEW && rows * (round_up(k, W_ALIGN) + 16) <= FEW_LDS; }
+// whether a result in 8 bits is made by the product's own kernel
+bool rows_whole(int64_t rows, int n, int k) { return n <= 256 && !is_few(rows, k); }
 
 struct Workspace {
   int64_t q, qs, y, bytes;  // offsets: x in 8 bits, its scales, the fp32 rows that go into 8 bits
@@ -93,13 +356,13 @@ struct Workspace {
 
 Workspace workspace_of(int64_t rows, int n, int k, int x_dtype, int out_dtype) {
   Workspace w{0, 0, 0, 0};
-  if (x_dtype != INF_DTYPE_I8) {
+  if (x_dtype != INF_DTYPE_I8 && !is_few(rows, k)) {
     w.q = w.bytes;
     w.bytes += round_up(rows * round_up(k, Q_ALIGN) + Q_SLACK, 256);
     w.qs = w.bytes;
     w.bytes += round_up(rows * 4, 256);
   }
-  if (out_dtype == INF_DTYPE_I8) {
+  if (out_dtype == INF_DTYPE_I8 && !rows_whole(rows, n, k)) {
     w.y = w.bytes;
     w.bytes += round_up(rows * n * 4, 256);
   }
@@ -122,6 +385,7 @@ int inf_linear_int(int64_t rows, int n, int k, const void* x, int x_dtype, int64
                    const int8_t* w, const float* w_scale, const float* bias, const float* add, int64_t ld_add, int act,
                    void* out, int out_dtype, int64_t ld_out, float* out_scale, void* workspace, inf_stream_t stream) {
   INF_CHECK_ARG(rows >= 0 && n >= 1 && k >= 1 && ld_x >= 0 && ld_out >= n, "linear_int: bad shape");
+  INF_CHECK_ARG(rows < (int64_t)1 << 31, "linear_int: too many rows");
   INF_CHECK_ARG(k <= 1 << 17, "linear_int: k is at most 2^17 (the sums are held in 32 bits)");
   INF_CHECK_ARG(act >= 0 && act <= 2, "linear_int: act must be 0 (none), 1 (ReLU) or 2 (sigmoid)");
   INF_CHECK_ARG(x_dtype == INF_DTYPE_F32 || x_dtype == INF_DTYPE_BF16 || x_dtype == INF_DTYPE_I8,
@@ -141,21 +405,32 @@ int inf_linear_int(int64_t rows, int n, int k, const void* x, int x_dtype, int64
   INF_CHECK_ARG(o.bytes == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0),
                 "linear_int: null or unaligned workspace");
   char* const wsp = (char*)workspace;
+  const hipStream_t st = (hipStream_t)stream;
   Linear8Args a{rows, n, k, (const int8_t*)x, ld_x, x_scale, w, round_up(k, q8::W_ALIGN), w_scale, bias, add, ld_add,
-                act, out, ld_out};
-  if (!x8) {
-    a.q = (int8_t*)(wsp + o.q);
-    a.ldq = round_up(k, q8::Q_ALIGN);
-    a.qs = (float*)(wsp + o.qs);
-    const int rc = launch_quantize_rows(x, x_dtype, rows, k, ld_x, (int8_t*)a.q, a.ldq, (float*)a.qs, (hipStream_t)stream);
-    if (rc != INF_OK) return rc;
+                act, out, ld_out, out_scale};
+  const bool put_after = y8 && !rows_whole(rows, n, k);
+  if (put_after) {
+    a.out = wsp + o.y;
+    a.ldo = n;
   }
-  if (!y8) return launch_linear8(a, out_dtype, (hipStream_t)stream);
-  a.out = wsp + o.y;
-  a.ldo = n;
-  const int rc = launch_linear8(a, INF_DTYPE_F32, (hipStream_t)stream);
-  if (rc != INF_OK) return rc;
-  return launch_quantize_rows(a.out, INF_DTYPE_F32, rows, n, n, (int8_t*)out, ld_out, out_scale, (hipStream_t)stream);
+  const int product_dtype = put_after ? INF_DTYPE_F32 : out_dtype;
+  int rc;
+  if (is_few(rows, k)) {
+    rc = x8 ? launch_few_out<int8_t>(a, product_dtype, x, ld_x, st)
+            : x_dtype == INF_DTYPE_BF16 ? launch_few_out<bf16>(a, product_dtype, x, ld_x, st)
+                                        : launch_few_out<float>(a, product_dtype, x, ld_x, st);
+  } else {
+    if (!x8) {
+      a.q = (int8_t*)(wsp + o.q);
+      a.ldq = round_up(k, q8::Q_ALIGN);
+      a.qs = (float*)(wsp + o.qs);
+      rc = launch_quantize_rows(x, x_dtype, rows, k, ld_x, (int8_t*)a.q, a.ldq, (float*)a.qs, st);
+      if (rc != INF_OK) return rc;
+    }
+    rc = launch_linear8(a, product_dtype, st);
+  }
+  if (rc != INF_OK || !put_after) return rc;
+  return launch_quantize_rows(a.out, INF_DTYPE_F32, rows, n, n, (int8_t*)out, ld_out, out_scale, st);
 }
 
 }  // extern "C"

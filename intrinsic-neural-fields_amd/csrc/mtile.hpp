@@ -1,0 +1,35 @@
+// The parts that the matrix tiles of linear8.hip and ckpt.hip share: LDS stages of 128-byte
+// rows, filled straight from memory, and their fragments.
+#pragma once
+
+#include "quant.hpp"
+
+namespace inf {
+namespace mt {
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// Chunk c (16 bytes) of a stage row lies at c ^ ((row >> 1) & 7): the 16 rows that a
+// fragment read touches at one c fall into all 64 banks evenly.
+__device__ __forceinline__ int swz(int row) { return (row >> 1) & 7; }
+__device__ __forceinline__ int chunk_at(int row, int c) { return row * 128 + ((c ^ swz(row)) << 4); }
+
+// the workgroup's barrier after all of this wave's loads (to registers and to LDS) and LDS
+// writes have arrived
+__device__ __forceinline__ void wait_all_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// Workgroups that one XCD receives (every eighth) take consecutive tiles, so that tiles which
+// share rows find them in that XCD's L2.
+__device__ __forceinline__ int xcd_order(int orig, int nblocks) {
+  const int q = nblocks / 8, r = nblocks % 8, xcd = orig % 8;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + orig / 8;
+}
+
+}  // namespace mt
+}  // namespace inf
