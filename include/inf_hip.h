@@ -223,7 +223,8 @@ int inf_linear_int(int64_t rows, int n, int k, const void* x, int x_dtype, int64
                    void* out, int out_dtype, int64_t ld_out, float* out_scale, void* workspace, inf_stream_t stream);
 /* Linear layer that keeps its input in 8 bits: y = act(x W^T + bias + add) in fp32 from x
  * (fp32 / bf16) as it is, W(n, k) = W[n stride_wn + k stride_wk]; bias and add may be NULL,
- * add may be y.  q / scale (not NULL): the rows of x in 8 bits.  mask (not NULL): bit j of
+ * add may be y.  q and scale: the rows of x in 8 bits, written; scale alone: x's own scales,
+ * read (q made before); both NULL: nothing is kept.  mask (not NULL): bit j of
  * word w of row m (ceil(n / 32) words a row) = y[m][32 w + j] > 0.  workspace:
  * inf_linear_ckpt_workspace_bytes(.., 0) bytes.                                            */
 int64_t inf_linear_ckpt_workspace_bytes(int64_t rows, int n, int k, int x_dtype, int backward);

@@ -3,109 +3,527 @@
 //             kept: q, s of x; one bit y > 0 (ReLU); y itself is the layer's output (sigmoid)
 //   backward  dz = dy [y > 0] | dy y (1 - y) | dy
 //             dx = dz W     dW = dz^T (s q)     db = sum_m dz
+//
+// Products of fp32 on the 16-bit matrix instructions.
+//   x W^T and dz W: each row of either side is scaled by a power of two so that its largest
+//   value lies in [2^14, 2^15), and a value is two fp16 pieces, hi = fp16(v), lo = fp16(v - hi):
+//   22 bits and a sign, rounded to nearest at 2^-24 of the value (2^-40 of the row's largest
+//   for the smallest ones, whose lo is subnormal).  hi hi + hi lo + lo hi, summed in fp32;
+//   lo lo is below 2^-24 and left out.  A bf16 x is one piece: two products.  The powers of two
+//   leave the result exactly.
+//   dW: q is exact in bf16 and dz s is three bf16 pieces, all 24 bits of it: three products, no
+//   scale (a column of dz has no scale that a sum over its rows could be divided by).
+// A value that is not finite makes NaN of the rows (and columns) that it enters.
 #include <algorithm>
 
-#include "quant.hpp"
+#include "mtile.hpp"
 
 namespace inf {
 namespace {
 
 using namespace q8;
+using namespace mt;
 
-constexpr int CT = 64, CK = 16;  // output tile, k tile
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8u __attribute__((ext_vector_type(8), aligned(4)));
+typedef bf16 bf16x8u __attribute__((ext_vector_type(8), aligned(2)));
 
-// C(m, n) = act(sum_k A(m, k) B(n, k) + bias[n] + beta C(m, n)); A and B by functor, stored by functor
-template <class FA, class FB, class ST>
-__device__ __forceinline__ void tile_product(int64_t m0, int64_t n0, int64_t M, int64_t N, int64_t K, const FA& fa,
-                                             const FB& fb, const ST& store) {
-  __shared__ float As[CK][CT + 1], Bs[CK][CT + 1];
-  const int t = threadIdx.x, tm = (t / 16) * 4, tn = (t % 16) * 4;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < K; k0 += CK) {
-    for (int i = t; i < CK * CT; i += 256) {
-      const int kk = i / CT, r = i % CT;
-      As[kk][r] = m0 + r < M && k0 + kk < K ? fa(m0 + r, k0 + kk) : 0.f;
-      Bs[kk][r] = n0 + r < N && k0 + kk < K ? fb(n0 + r, k0 + kk) : 0.f;
+enum { DZ_NONE = 0, DZ_RELU = 1, DZ_SIGMOID = 2 };  // act
+
+// the power of two that takes a row of largest value a below 2^15
+__device__ __forceinline__ int shift_of(float a) { return 15 - __builtin_amdgcn_frexp_expf(a); }
+__device__ __forceinline__ float by_power(float v, int e) { return __builtin_amdgcn_ldexpf(v, e); }
+
+__device__ __forceinline__ void split8(const float (&v)[8], int shift, f16x8* hi, f16x8* lo) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x = by_power(v[e], shift);
+    (*hi)[e] = (_Float16)x;
+    (*lo)[e] = (_Float16)(x - (float)(*hi)[e]);
+  }
+}
+
+// ---- the weight's rows as fp16 pieces ---------------------------------------------------
+// Row r of the product's side: V(r, k) = W[r sr + k sk], k < K, as blocks of 32 k: 64 bytes hi,
+// 64 bytes lo, zero behind K.  by_row: a wave a row, its lanes along k (sk is the short
+// stride); by column: a workgroup 64 rows, its lanes along the rows.
+__global__ __launch_bounds__(256) void split_rows_kernel(const float* __restrict__ W, int64_t sr, int64_t sk, int rows,
+                                                         int K, char* __restrict__ out, int* __restrict__ shift) {
+  const int r = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x % 64;
+  if (r >= rows) return;
+  const float* const w = W + r * sr;
+  unsigned a = 0;
+  for (int k = lane; k < K; k += 64) a = max(a, abs_bits(w[k * sk]));
+#pragma unroll
+  for (int h = 32; h > 0; h >>= 1) a = max(a, (unsigned)__shfl_xor((int)a, h));
+  const int e = shift_of(__uint_as_float(a));
+  if (lane == 0) shift[r] = e;
+  const int Kp = (K + 31) / 32 * 32;
+  for (int k = lane * 8; k < Kp; k += 512) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? w[(k + i) * sk] : 0.f;
+    f16x8 hi, lo;
+    split8(v, e, &hi, &lo);
+    char* const to = out + (int64_t)r * Kp * 4 + (k / 32) * 128 + (k % 32) * 2;
+    *reinterpret_cast<f16x8*>(to) = hi;
+    *reinterpret_cast<f16x8*>(to + 64) = lo;
+  }
+}
+
+__global__ __launch_bounds__(256) void split_columns_kernel(const float* __restrict__ W, int64_t sr, int64_t sk,
+                                                            int rows, int K, char* __restrict__ out,
+                                                            int* __restrict__ shift) {
+  __shared__ unsigned top[4][64];
+  const int l = threadIdx.x % 64, g = threadIdx.x / 64, r = blockIdx.x * 64 + l;
+  const float* const w = W + min(r, rows - 1) * sr;
+  unsigned a = 0;
+  for (int k = g; k < K; k += 4) a = max(a, abs_bits(w[k * sk]));
+  top[g][l] = a;
+  __syncthreads();
+  const int e = shift_of(__uint_as_float(max(max(top[0][l], top[1][l]), max(top[2][l], top[3][l]))));
+  if (r >= rows) return;
+  if (g == 0) shift[r] = e;
+  const int Kp = (K + 31) / 32 * 32;
+  for (int k = g * 8; k < Kp; k += 32) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? w[(k + i) * sk] : 0.f;
+    f16x8 hi, lo;
+    split8(v, e, &hi, &lo);
+    char* const to = out + (int64_t)r * Kp * 4 + (k / 32) * 128 + (k % 32) * 2;
+    *reinterpret_cast<f16x8*>(to) = hi;
+    *reinterpret_cast<f16x8*>(to + 64) = lo;
+  }
+}
+
+// ---- dz -------------------------------------------------------------------------------
+struct Dz {
+  const float* dy;
+  int64_t lddy;
+  const float* y;
+  int64_t ldy;
+  const uint32_t* mask;
+  int words;  // of the mask, a row
+};
+
+template <int ACT>
+__device__ __forceinline__ float dz_at(const Dz& d, int64_t m, int c) {
+  const float g = d.dy[m * d.lddy + c];
+  if (ACT == DZ_RELU) return (d.mask[m * d.words + c / 32] >> (c % 32)) & 1 ? g : 0.f;
+  if (ACT == DZ_SIGMOID) {
+    const float y = d.y[m * d.ldy + c];
+    return g * (y * (1.f - y));
+  }
+  return g;
+}
+
+// each row's shift; LPR lanes a row
+template <int ACT, int LPR>
+__global__ __launch_bounds__(256) void dz_shift_kernel(Dz d, int64_t rows, int n, int* __restrict__ shift) {
+  const int64_t m = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  if (m >= rows) return;
+  unsigned a = 0;
+  for (int c = threadIdx.x % LPR; c < n; c += LPR) a = max(a, abs_bits(dz_at<ACT>(d, m, c)));
+#pragma unroll
+  for (int h = LPR / 2; h > 0; h >>= 1) a = max(a, (unsigned)__shfl_xor((int)a, h));
+  if (threadIdx.x % LPR == 0) shift[m] = shift_of(__uint_as_float(a));
+}
+
+// ---- x W^T and dz W -----------------------------------------------------------------------
+// out(m, c) = sum_k side(m, k) V(c, k): BM rows by BN columns a workgroup, WM x WN waves,
+// v_mfma_f32_16x16x32_f16 with V as its first operand (a lane holds four neighbouring
+// columns of one row).  Per turn 32 k: V's pieces go straight from memory to LDS, the rows of
+// x or dz through registers, where they are split, one turn ahead.  Two LDS stages of
+// 128-byte rows (64 hi, 64 lo).
+struct SideArgs {
+  int64_t rows;
+  int cols, K;          // output columns; length of the sums
+  const void* x;        // forward: x
+  int64_t ldx;
+  const float* scale;   // forward: the rows' 8-bit scales (their largest value / 127)
+  const int* shift;     // dx: the rows' shifts
+  Dz dz;
+  const char* V;        // pieces of the weight's rows
+  const int* vshift;
+  const float* bias;    // forward
+  const float* add;
+  int64_t ldadd;
+  int act;
+  void* out;
+  int64_t ldo;
+  uint32_t* mask;
+};
+
+template <int BM, int BN, int WM, int WN>
+struct ST {
+  static constexpr int THREADS = 64 * WM * WN;
+  static constexpr int WROWS = BM / WM, WCOLS = BN / WN, TI = WROWS / 16, TJ = WCOLS / 16;
+  static constexpr int STAGE = (BM + BN) * 128, LDS = 2 * STAGE;
+  static constexpr int LOADS = BN * 128 / (THREADS * 16);
+  static constexpr int PASS = BM / (THREADS / 4);  // rows that a thread splits a turn (8 values each)
+  static_assert(BN * 128 % (THREADS * 16) == 0 && BM % (THREADS / 4) == 0 && LDS <= 160 * 1024, "tile");
+  static_assert(WCOLS % 32 == 0, "a wave holds whole words of the mask");
+};
+
+// MODE 0: forward, the side is X rows; 1: dx, the side is dz (ACT)
+template <int MODE, int ACT, typename X, typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, int tiles_n, int nblocks) {
+  using P = ST<BM, BN, WM, WN>;
+  constexpr int TI = P::TI, TJ = P::TJ, PASS = P::PASS;
+  constexpr bool LO = sizeof(X) == 4;  // a bf16 value is one piece
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int bid = xcd_order((int)blockIdx.x, nblocks);
+  const int64_t m0 = (int64_t)(bid / tiles_n) * BM;
+  const int n0 = (bid % tiles_n) * BN;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave / WN, wc = wave % WN, r16 = lane & 15, g4 = lane >> 4;
+  const int turns = (a.K + 31) / 32;
+  const int64_t ldv = (int64_t)turns * 128;
+
+  const char* src[P::LOADS];
+#pragma unroll
+  for (int i = 0; i < P::LOADS; ++i) {
+    const int p = tid + P::THREADS * i, row = p >> 3;
+    src[i] = a.V + min(n0 + row, a.cols - 1) * ldv + (((p & 7) ^ swz(row)) << 4);
+  }
+  auto issue = [&](int t) {
+    char* st = smem + (t & 1) * P::STAGE;
+#pragma unroll
+    for (int i = 0; i < P::LOADS; ++i) {
+      const char* from = src[i] + t * 128;
+      __builtin_amdgcn_global_load_lds(from, (lds_void*)(st + (wave + (P::THREADS / 64) * i) * 1024), 16, 0, 0);
     }
-    __syncthreads();
-    for (int kk = 0; kk < CK; ++kk)
+  };
+  const int c8 = (tid & 3) * 8;
+  int shift[PASS];
+  int64_t row[PASS];
+#pragma unroll
+  for (int p = 0; p < PASS; ++p) {
+    row[p] = min(m0 + (tid >> 2) + p * (P::THREADS / 4), a.rows - 1);
+    shift[p] = MODE == 0 ? shift_of(a.scale[row[p]] * 127.f) : a.shift[row[p]];
+  }
+  float v[PASS][8];
+  auto fetch = [&](int t) {
+    const int k = t * 32 + c8;
+#pragma unroll
+    for (int p = 0; p < PASS; ++p) {
+      const X* const from = MODE == 0 ? (const X*)a.x + row[p] * a.ldx : (const X*)a.dz.dy + row[p] * a.dz.lddy;
+      if (k + 8 <= a.K) {
+        if constexpr (sizeof(X) == 4) {
+          const f32x8u x = *reinterpret_cast<const f32x8u*>(from + k);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[p][e] = x[e];
+        } else {
+          const bf16x8u x = *reinterpret_cast<const bf16x8u*>(from + k);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[p][e] = (float)x[e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[p][e] = k + e < a.K ? to_f32(from[k + e]) : 0.f;
+      }
+      if constexpr (MODE == 1 && ACT == DZ_RELU) {
+        const uint32_t w = a.dz.mask[row[p] * a.dz.words + t] >> c8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[p][e] = (w >> e) & 1 ? v[p][e] : 0.f;
+      }
+      if constexpr (MODE == 1 && ACT == DZ_SIGMOID) {
+        const float* const yr = a.dz.y + row[p] * a.dz.ldy;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = k + e < a.K ? yr[k + e] : 0.f;
+          v[p][e] = v[p][e] * (y * (1.f - y));
+        }
+      }
+    }
+  };
+  auto put = [&](int t) {
+    char* st = smem + (t & 1) * P::STAGE;
+#pragma unroll
+    for (int p = 0; p < PASS; ++p) {
+      const int r = BN + (tid >> 2) + p * (P::THREADS / 4), c = tid & 3;
+      f16x8 hi, lo;
+      split8(v[p], shift[p], &hi, &lo);
+      *reinterpret_cast<f16x8*>(st + chunk_at(r, c)) = hi;
+      if (LO) *reinterpret_cast<f16x8*>(st + chunk_at(r, 4 + c)) = lo;
+    }
+  };
+
+  f32x4 acc[TJ][TI];
+#pragma unroll
+  for (int j = 0; j < TJ; ++j)
+#pragma unroll
+    for (int i = 0; i < TI; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  issue(0);
+  fetch(0);
+  put(0);
+  wait_all_barrier();
+#pragma unroll 1
+  for (int t = 0; t < turns; ++t) {
+    const bool more = t + 1 < turns;
+    if (more) {
+      issue(t + 1);
+      fetch(t + 1);
+    }
+    const char* st = smem + (t & 1) * P::STAGE;
+    f16x8 xh[TI], xl[TI];
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      const int r = BN + wr * P::WROWS + 16 * i + r16;
+      xh[i] = *reinterpret_cast<const f16x8*>(st + chunk_at(r, g4));
+      if (LO) xl[i] = *reinterpret_cast<const f16x8*>(st + chunk_at(r, 4 + g4));
+    }
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+      const int r = wc * P::WCOLS + 16 * j + r16;
+      const f16x8 wh = *reinterpret_cast<const f16x8*>(st + chunk_at(r, g4));
+      const f16x8 wl = *reinterpret_cast<const f16x8*>(st + chunk_at(r, 4 + g4));
+#pragma unroll
+      for (int i = 0; i < TI; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl, xh[i], acc[j][i], 0, 0, 0);
+      if (LO)
+#pragma unroll
+        for (int i = 0; i < TI; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, xl[i], acc[j][i], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < TI; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, xh[i], acc[j][i], 0, 0, 0);
+    }
+    if (more) put(t + 1);
+    wait_all_barrier();
+  }
+
+  // lane: row wr WROWS + 16 i + r16, columns wc WCOLS + 16 j + 4 g4 + (0..3)
+  int sm[TI];
+#pragma unroll
+  for (int i = 0; i < TI; ++i) {
+    const int64_t m = min(m0 + wr * P::WROWS + 16 * i + r16, a.rows - 1);
+    sm[i] = MODE == 0 ? shift_of(a.scale[m] * 127.f) : a.shift[m];
+  }
+  uint32_t bits[TI];
+#pragma unroll
+  for (int j = 0; j < TJ; ++j) {
+    const int n = n0 + wc * P::WCOLS + 16 * j + 4 * g4;
+    int sn[4];
+    float bias[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sn[e] = a.vshift[min(n + e, a.cols - 1)];
+      bias[e] = MODE == 0 && a.bias != nullptr ? a.bias[min(n + e, a.cols - 1)] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      const int64_t m = m0 + wr * P::WROWS + 16 * i + r16;
+      float z[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        z[e] = by_power(acc[j][i][e], -(sm[i] + sn[e]));
+        if (MODE == 0) {
+          z[e] += bias[e];
+          if (a.add != nullptr && m < a.rows && n + e < a.cols) z[e] += a.add[m * a.ldadd + n + e];
+          z[e] = activate(z[e], a.act);
+        }
+      }
+      if (m < a.rows) {
+        T* const to = reinterpret_cast<T*>(a.out) + m * a.ldo + n;
+        if (n + 4 <= a.cols) {
+          typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+          V4 o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(z[e]);
+          *reinterpret_cast<V4*>(to) = o;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < a.cols) to[e] = from_f32<T>(z[e]);
+        }
+      }
+      if (MODE == 0 && a.mask != nullptr) {
+        uint32_t b = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b |= (uint32_t)(z[e] > 0.f && n + e < a.cols) << (4 * g4 + e);
+        b |= (uint32_t)__shfl_xor((int)b, 16);
+        b |= (uint32_t)__shfl_xor((int)b, 32);
+        if (j % 2 == 0) {
+          bits[i] = b;
+        } else if (g4 == 0 && m < a.rows && n - 16 < a.cols) {
+          a.mask[m * ((a.cols + 31) / 32) + (n - 16) / 32] = bits[i] | b << 16;
+        }
+      }
+    }
+  }
+}
+
+// ---- dW and db ------------------------------------------------------------------------
+// dW(n, k) = sum_m dz(m, n) s_m q(m, k): 128 n by 256 k a workgroup, 2 x 4 waves, 32 rows m a
+// turn, v_mfma_f32_16x16x32_bf16 with q as its first operand (a lane holds four neighbouring
+// k of one n).  Both sides are turned on the way to LDS: a thread loads one column of 8 (4)
+// rows, neighbouring threads neighbouring columns.  The rows are divided over `splits`
+// workgroups a tile, whose sums add_slabs_kernel adds in order: no atomics.
+constexpr int DW_N = 128, DW_K = 256, DW_THREADS = 512;
+constexpr int DW_STAGE = DW_K * 64 + 3 * DW_N * 64;  // q rows, then the pieces of dz: hi, mid, lo
+constexpr int DW_LDS = 2 * DW_STAGE;
+
+__device__ __forceinline__ int at64(int row, int c) { return row * 64 + ((c ^ ((row >> 2) & 3)) << 4); }
+__device__ __forceinline__ uint32_t top_halves(float a, float b) {  // bf16 of a (low) and b, both exact
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+}
+
+struct DwArgs {
+  int64_t rows;
+  int n, k;
+  Dz dz;
+  const int8_t* q;
+  int64_t ldq;
+  const float* s;
+  int tiles_k, tiles, splits;
+  int64_t rows_a_split;  // a multiple of 32
+  float* out;            // [splits][n][ldw]
+  int64_t ldw;
+  float* db;             // [splits][n], or null
+};
+
+template <int ACT>
+__global__ __launch_bounds__(DW_THREADS) void dw_tile_kernel(DwArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  // the tiles of one split next to each other on one XCD: they read the same rows
+  const int bid = xcd_order((int)blockIdx.x, a.tiles * a.splits);
+  const int split = bid / a.tiles, tile = bid % a.tiles;
+  const int n0 = tile / a.tiles_k * DW_N, k0 = tile % a.tiles_k * DW_K;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave / 4, wk = wave % 4, r16 = lane & 15, g4 = lane >> 4;
+  const int64_t mb = split * a.rows_a_split, me = min(mb + a.rows_a_split, a.rows);
+  const int turns = (int)((me - mb + 31) / 32);
+
+  const int zc = tid & 127, zg = tid >> 7;  // dz: column, group of 8 rows
+  const int n = n0 + zc;
+  const bool in_n = n < a.n;
+  const int qc = tid & 63, qg = tid >> 6;   // q: 4 columns, group of 4 rows
+  const int64_t kq = min((int64_t)(k0 + 4 * qc), a.ldq - 4);
+  float z[8];
+  float dbsum = 0.f;
+  int q[4];
+  float s[8];
+  auto fetch = [&](int t) {
+    const int64_t mz = mb + t * 32 + zg * 8, mq = mb + t * 32 + qg * 4;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool in = in_n && mz + e < me;
+      z[e] = in ? dz_at<ACT>(a.dz, mz + e, n) : 0.f;
+      s[e] = in ? a.s[mz + e] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = *reinterpret_cast<const int*>(a.q + min(mq + e, a.rows - 1) * a.ldq + kq);
+  };
+  auto put = [&](int t) {
+    char* st = smem + (t & 1) * DW_STAGE;
+    u32x4 piece[3];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      float v[2] = {z[e] * s[e], z[e + 1] * s[e + 1]};
+      dbsum += z[e];
+      dbsum += z[e + 1];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        piece[p][e / 2] = top_halves(v[0], v[1]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) v[u] -= __uint_as_float(__float_as_uint(v[u]) & 0xffff0000u);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+      *reinterpret_cast<u32x4*>(st + DW_K * 64 + p * DW_N * 64 + at64(zc, zg)) = piece[p];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      u32x2 w;
+      w[0] = top_halves((float)(int8_t)(q[0] >> (8 * c)), (float)(int8_t)(q[1] >> (8 * c)));
+      w[1] = top_halves((float)(int8_t)(q[2] >> (8 * c)), (float)(int8_t)(q[3] >> (8 * c)));
+      *reinterpret_cast<u32x2*>(st + at64(4 * qc + c, qg / 2) + (qg & 1) * 8) = w;
+    }
+  };
+  f32x4 acc[4][4];  // [k tile][n tile]
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (turns > 0) {
+    fetch(0);
+    put(0);
+  }
+  wait_all_barrier();
+#pragma unroll 1
+  for (int t = 0; t < turns; ++t) {
+    if (t + 1 < turns) fetch(t + 1);
+    const char* st = smem + (t & 1) * DW_STAGE;
+    bf16x8 qf[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) qf[j] = *reinterpret_cast<const bf16x8*>(st + at64(wk * 64 + 16 * j + r16, g4));
+#pragma unroll
+    for (int p = 2; p >= 0; --p) {
+      bf16x8 zf[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
+        zf[i] = *reinterpret_cast<const bf16x8*>(st + DW_K * 64 + p * DW_N * 64 + at64(wn * 64 + 16 * i + r16, g4));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(As[kk][tm + i], Bs[kk][tn + j], acc[i][j]);
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[j], zf[i], acc[j][i], 0, 0, 0);
+    }
+    if (t + 1 < turns) put(t + 1);
+    wait_all_barrier();
+  }
+  float* const out = a.out + (int64_t)split * a.n * a.ldw;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = n0 + wn * 64 + 16 * i + r16;
+    if (c >= a.n) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = k0 + wk * 64 + 16 * j + 4 * g4;
+      float* const to = out + c * a.ldw + k;
+      if (k + 4 <= a.k) {
+        f32x4u o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = acc[j][i][e];
+        *reinterpret_cast<f32x4u*>(to) = o;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (k + e < a.k) to[e] = acc[j][i][e];
+      }
+    }
+  }
+  if (a.db != nullptr && k0 == 0) {
+    float* const part = reinterpret_cast<float*>(smem);  // every wave has read its last stage
+    part[zg * DW_N + zc] = dbsum;
     __syncthreads();
-  }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j)
-      if (m0 + tm + i < M && n0 + tn + j < N) store(m0 + tm + i, n0 + tn + j, acc[i][j]);
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void forward_kernel(int64_t rows, int n, int k, const T* __restrict__ x, int64_t ldx,
-                                                      const float* __restrict__ W, int64_t swn, int64_t swk,
-                                                      const float* __restrict__ bias, const float* __restrict__ add,
-                                                      int64_t ldadd, int act, float* __restrict__ y, int64_t ldy) {
-  for (int64_t m0 = (int64_t)blockIdx.y * CT; m0 < rows; m0 += (int64_t)gridDim.y * CT)
-    tile_product(m0, (int64_t)blockIdx.x * CT, rows, n, k, [&](int64_t m, int64_t c) { return to_f32(x[m * ldx + c]); },
-                 [&](int64_t r, int64_t c) { return W[r * swn + c * swk]; },
-                 [&](int64_t m, int64_t c, float v) {
-                   if (bias != nullptr) v += bias[c];
-                   if (add != nullptr) v += add[m * ldadd + c];
-                   y[m * ldy + c] = activate(v, act);
-                 });
-}
-
-// bit j of word w of a row: y[32 w + j] > 0
-__global__ __launch_bounds__(256) void mask_kernel(int64_t rows, int n, const float* __restrict__ y, int64_t ldy,
-                                                   uint32_t* __restrict__ mask) {
-  const int words = (n + 31) / 32;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * words; i += (int64_t)gridDim.x * 256) {
-    const int64_t m = i / words;
-    const int w = (int)(i % words);
-    uint32_t b = 0;
-    for (int j = 0; j < 32 && 32 * w + j < n; ++j) b |= (uint32_t)(y[m * ldy + 32 * w + j] > 0.f) << j;
-    mask[i] = b;
+    if (tid < DW_N && in_n)
+      a.db[(int64_t)split * a.n + n] = (part[zc] + part[DW_N + zc]) + (part[2 * DW_N + zc] + part[3 * DW_N + zc]);
   }
 }
 
-__global__ __launch_bounds__(256) void dz_kernel(int64_t rows, int n, const float* __restrict__ dy, int64_t lddy,
-                                                 int act, const float* __restrict__ y, int64_t ldy,
-                                                 const uint32_t* __restrict__ mask, float* __restrict__ dz) {
-  const int words = (n + 31) / 32;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * n; i += (int64_t)gridDim.x * 256) {
-    const int64_t m = i / n;
-    const int c = (int)(i % n);
-    float g = dy[m * lddy + c];
-    if (act == 1) g = (mask[m * words + c / 32] >> (c % 32)) & 1 ? g : 0.f;
-    if (act == 2) g = g * (y[m * ldy + c] * (1.f - y[m * ldy + c]));
-    dz[i] = g;
+// dW and db from the splits' sums, in order
+__global__ __launch_bounds__(256) void add_slabs_kernel(const float* __restrict__ slabs, int64_t count, int k,
+                                                        int splits, float* __restrict__ dW, int64_t lddw,
+                                                        const float* __restrict__ dbs, int n, float* __restrict__ db) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < count) {
+    float v = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) v += slabs[s * count + i];
+    dW[i / k * lddw + i % k] = v;
+  } else if (i - count < n && db != nullptr) {
+    float v = 0.f;
+    for (int s = 0; s < splits; ++s) v += dbs[(int64_t)s * n + (i - count)];
+    db[i - count] = v;
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void dx_kernel(int64_t rows, int n, int k, const float* __restrict__ dz,
-                                                 const float* __restrict__ W, int64_t swn, int64_t swk,
-                                                 T* __restrict__ dx, int64_t lddx) {
-  for (int64_t m0 = (int64_t)blockIdx.y * CT; m0 < rows; m0 += (int64_t)gridDim.y * CT)
-    tile_product(m0, (int64_t)blockIdx.x * CT, rows, k, n, [&](int64_t m, int64_t c) { return dz[m * n + c]; },
-                 [&](int64_t r, int64_t c) { return W[c * swn + r * swk]; },
-                 [&](int64_t m, int64_t c, float v) { dx[m * lddx + c] = from_f32<T>(v); });
-}
-
-__global__ __launch_bounds__(256) void dw_kernel(int64_t rows, int n, int k, const float* __restrict__ dz,
-                                                 const int8_t* __restrict__ q, int64_t ldq,
-                                                 const float* __restrict__ s, float* __restrict__ dW, int64_t lddw) {
-  tile_product((int64_t)blockIdx.y * CT, (int64_t)blockIdx.x * CT, n, k, rows,
-               [&](int64_t r, int64_t m) { return dz[m * n + r]; },
-               [&](int64_t c, int64_t m) { return (float)q[m * ldq + c] * s[m]; },
-               [&](int64_t r, int64_t c, float v) { dW[r * lddw + c] = v; });
-}
-
-__global__ __launch_bounds__(256) void db_kernel(int64_t rows, int n, const float* __restrict__ dz,
-                                                 float* __restrict__ db) {
+// db alone (no weight gradient asked for)
+template <int ACT>
+__global__ __launch_bounds__(256) void db_kernel(Dz d, int64_t rows, int n, float* __restrict__ db) {
   __shared__ float part[256];
   float v = 0.f;
-  for (int64_t m = threadIdx.x; m < rows; m += 256) v += dz[m * n + blockIdx.x];
+  for (int64_t m = threadIdx.x; m < rows; m += 256) v += dz_at<ACT>(d, m, blockIdx.x);
   part[threadIdx.x] = v;
   __syncthreads();
   for (int h = 128; h > 0; h >>= 1) {
@@ -115,9 +533,149 @@ __global__ __launch_bounds__(256) void db_kernel(int64_t rows, int n, const floa
   if (threadIdx.x == 0) db[blockIdx.x] = part[0];
 }
 
-unsigned blocks_of(int64_t n) { return (unsigned)std::min<int64_t>(std::max<int64_t>(ceil_div(n, 256), 1), 1 << 16); }
-dim3 tiles(int64_t m, int64_t n) {
-  return dim3((unsigned)ceil_div(n, CT), (unsigned)std::min<int64_t>(std::max<int64_t>(ceil_div(m, CT), 1), 65535));
+// ---- launches -------------------------------------------------------------------------
+template <int MODE, int ACT, typename X, typename T, int BM, int BN, int WM, int WN>
+int launch_tile(const SideArgs& a, hipStream_t stream) {
+  using P = ST<BM, BN, WM, WN>;
+  const int tiles_n = (int)ceil_div(a.cols, BN);
+  const int64_t nblocks = ceil_div(a.rows, BM) * tiles_n;
+  INF_CHECK_ARG(nblocks < (int64_t)1 << 31, "linear_ckpt: too many tiles");
+  const auto kernel = split_tile_kernel<MODE, ACT, X, T, BM, BN, WM, WN>;
+  static const hipError_t attr =
+      hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
+  INF_HIP_TRY(attr);
+  kernel<<<(unsigned)nblocks, P::THREADS, P::LDS, stream>>>(a, tiles_n, (int)nblocks);
+  INF_LAUNCH_CHECK();
+  return INF_OK;
+}
+
+// The widest tile that still gives every CU a workgroup.
+template <int MODE, int ACT, typename X, typename T>
+int launch_tiles(const SideArgs& a, hipStream_t stream) {
+  const int64_t wide = ceil_div(a.rows, 256);
+  if (a.cols <= 32 && wide >= 128) return launch_tile<MODE, ACT, X, T, 256, 32, 4, 1>(a, stream);
+  if (a.cols <= 128 && wide >= 256) return launch_tile<MODE, ACT, X, T, 256, 128, 4, 2>(a, stream);
+  if (a.cols > 128 && wide * ceil_div(a.cols, 256) >= 256) return launch_tile<MODE, ACT, X, T, 256, 256, 2, 4>(a, stream);
+  return launch_tile<MODE, ACT, X, T, 64, 64, 2, 2>(a, stream);
+}
+
+int launch_split(const float* W, int64_t sr, int64_t sk, int rows, int K, char* out, int* shift, hipStream_t stream) {
+  if (std::abs(sk) <= std::abs(sr))
+    split_rows_kernel<<<(unsigned)ceil_div(rows, 4), 256, 0, stream>>>(W, sr, sk, rows, K, out, shift);
+  else
+    split_columns_kernel<<<(unsigned)ceil_div(rows, 64), 256, 0, stream>>>(W, sr, sk, rows, K, out, shift);
+  INF_LAUNCH_CHECK();
+  return INF_OK;
+}
+
+template <int ACT>
+int launch_dz_shift(const Dz& d, int64_t rows, int n, int* shift, hipStream_t stream) {
+  if (n <= 16) dz_shift_kernel<ACT, 4><<<(unsigned)ceil_div(rows, 64), 256, 0, stream>>>(d, rows, n, shift);
+  else dz_shift_kernel<ACT, 64><<<(unsigned)ceil_div(rows, 4), 256, 0, stream>>>(d, rows, n, shift);
+  INF_LAUNCH_CHECK();
+  return INF_OK;
+}
+
+template <int ACT>
+int launch_dw(const DwArgs& a, hipStream_t stream) {
+  static const hipError_t attr =
+      hipFuncSetAttribute((const void*)dw_tile_kernel<ACT>, hipFuncAttributeMaxDynamicSharedMemorySize, DW_LDS);
+  INF_HIP_TRY(attr);
+  dw_tile_kernel<ACT><<<(unsigned)(a.tiles * a.splits), DW_THREADS, DW_LDS, stream>>>(a);
+  INF_LAUNCH_CHECK();
+  return INF_OK;
+}
+
+struct DwShape {
+  int tiles_k, tiles, splits;
+  int64_t rows_a_split;
+};
+
+// as many splits as give each CU a workgroup, of eight turns at least
+DwShape dw_shape(int64_t rows, int n, int k) {
+  DwShape d;
+  d.tiles_k = (int)ceil_div(k, DW_K);
+  d.tiles = d.tiles_k * (int)ceil_div(n, DW_N);
+  const int64_t turns = std::max<int64_t>(ceil_div(rows, 32), 1);
+  const int64_t splits = std::min<int64_t>(std::max<int64_t>(256 / d.tiles, 1), ceil_div(turns, 8));
+  d.rows_a_split = ceil_div(turns, splits) * 32;
+  d.splits = (int)std::max<int64_t>(ceil_div(rows, d.rows_a_split), 1);
+  return d;
+}
+
+// offsets in the workspace
+struct ForwardSpace {
+  int64_t scale, V, vshift, bytes;
+};
+ForwardSpace forward_space(int64_t rows, int n, int k) {
+  ForwardSpace w;
+  w.scale = 0;
+  w.V = w.scale + round_up(rows * 4, 256);
+  w.vshift = w.V + round_up(n * round_up(k, 32) * 4, 256);
+  w.bytes = w.vshift + round_up((int64_t)n * 4, 256);
+  return w;
+}
+struct BackwardSpace {
+  int64_t shift, V, vshift, slabs, db, bytes;
+};
+BackwardSpace backward_space(int64_t rows, int n, int k) {
+  const DwShape d = dw_shape(rows, n, k);
+  BackwardSpace w;
+  w.shift = 0;
+  w.V = w.shift + round_up(rows * 4, 256);
+  w.vshift = w.V + round_up(k * round_up(n, 32) * 4, 256);
+  w.slabs = w.vshift + round_up((int64_t)k * 4, 256);
+  w.db = w.slabs + round_up((int64_t)d.splits * n * k * 4, 256);
+  w.bytes = w.db + round_up((int64_t)d.splits * n * 4, 256);
+  return w;
+}
+
+template <int ACT>
+int backward(int64_t rows, int n, int k, const Dz& dz, const int8_t* q, int64_t ldq, const float* scale, const float* W,
+             int64_t swn, int64_t swk, void* dx, int dx_dtype, int64_t lddx, float* dW, int64_t lddw, float* db,
+             char* ws, hipStream_t st) {
+  const BackwardSpace o = backward_space(rows, n, k);
+  int rc;
+  if (dx != nullptr && rows > 0) {
+    rc = launch_dz_shift<ACT>(dz, rows, n, (int*)(ws + o.shift), st);
+    if (rc != INF_OK) return rc;
+    rc = launch_split(W, swk, swn, k, n, ws + o.V, (int*)(ws + o.vshift), st);
+    if (rc != INF_OK) return rc;
+    SideArgs a{};
+    a.rows = rows;
+    a.cols = k;
+    a.K = n;
+    a.shift = (int*)(ws + o.shift);
+    a.dz = dz;
+    a.V = ws + o.V;
+    a.vshift = (int*)(ws + o.vshift);
+    a.out = dx;
+    a.ldo = lddx;
+    rc = dx_dtype == INF_DTYPE_F32 ? launch_tiles<1, ACT, float, float>(a, st) : launch_tiles<1, ACT, float, bf16>(a, st);
+    if (rc != INF_OK) return rc;
+  }
+  if (dW != nullptr) {
+    const DwShape d = dw_shape(rows, n, k);
+    DwArgs a{rows, n, k, dz, q, ldq, scale, d.tiles_k, d.tiles, d.splits, d.rows_a_split, (float*)(ws + o.slabs), k,
+             db != nullptr ? (float*)(ws + o.db) : nullptr};
+    if (d.splits == 1) {  // nothing to add
+      a.out = dW;
+      a.ldw = lddw;
+      a.db = db;
+    }
+    rc = launch_dw<ACT>(a, st);
+    if (rc != INF_OK) return rc;
+    if (d.splits > 1) {
+      const int64_t count = (int64_t)n * k;
+      add_slabs_kernel<<<(unsigned)ceil_div(count + n, 256), 256, 0, st>>>(a.out, count, k, d.splits, dW, lddw, a.db, n,
+                                                                           db);
+      INF_LAUNCH_CHECK();
+    }
+  } else if (db != nullptr) {
+    db_kernel<ACT><<<n, 256, 0, st>>>(dz, rows, n, db);
+    INF_LAUNCH_CHECK();
+  }
+  return INF_OK;
 }
 
 }  // namespace
@@ -130,7 +688,7 @@ extern "C" {
 int64_t inf_linear_ckpt_workspace_bytes(int64_t rows, int n, int k, int x_dtype, int backward) {
   if (rows < 0 || n < 1 || k < 1) return -1;
   (void)x_dtype;
-  return backward ? round_up(std::max<int64_t>(rows * n * 4, 256), 256) : 256;
+  return backward ? backward_space(rows, n, k).bytes : forward_space(rows, n, k).bytes;
 }
 
 int inf_linear_ckpt_forward(int64_t rows, int n, int k, const void* x, int x_dtype, int64_t ld_x, const float* W,
@@ -138,6 +696,7 @@ int inf_linear_ckpt_forward(int64_t rows, int n, int k, const void* x, int x_dty
                             int act, float* y, int64_t ld_y, uint32_t* mask, int8_t* q, int64_t ld_q, float* scale,
                             void* workspace, inf_stream_t stream) {
   INF_CHECK_ARG(rows >= 0 && n >= 1 && k >= 1 && ld_x >= 0 && ld_y >= n, "linear_ckpt: bad shape");
+  INF_CHECK_ARG(rows < (int64_t)1 << 31, "linear_ckpt: too many rows");
   INF_CHECK_ARG(act >= 0 && act <= 2, "linear_ckpt: act must be 0 (none), 1 (ReLU) or 2 (sigmoid)");
   INF_CHECK_ARG(x_dtype == INF_DTYPE_F32 || x_dtype == INF_DTYPE_BF16, "linear_ckpt: x must be fp32 or bf16");
   if (rows == 0) return INF_OK;
@@ -146,22 +705,37 @@ int inf_linear_ckpt_forward(int64_t rows, int n, int k, const void* x, int x_dty
   INF_CHECK_ARG(q == nullptr || (scale != nullptr && ld_q >= k && ld_q % q8::Q_ALIGN == 0 && (uintptr_t)q % 16 == 0),
                 "linear_ckpt: q rows must start on 16 bytes and have scales");
   const hipStream_t st = (hipStream_t)stream;
+  char* const ws = (char*)workspace;
+  const ForwardSpace o = forward_space(rows, n, k);
+  SideArgs a{};
+  a.scale = scale;
+  int rc;
   if (q != nullptr) {
-    const int rc = launch_quantize_rows(x, x_dtype, rows, k, ld_x, q, ld_q, scale, st);
-    if (rc != INF_OK) return rc;
+    rc = launch_quantize_rows(x, x_dtype, rows, k, ld_x, q, ld_q, scale, st);
+  } else if (scale == nullptr) {
+    a.scale = (float*)(ws + o.scale);
+    rc = launch_quantize_rows(x, x_dtype, rows, k, ld_x, nullptr, 0, (float*)(ws + o.scale), st);
+  } else {
+    rc = INF_OK;
   }
-  if (x_dtype == INF_DTYPE_F32)
-    forward_kernel<<<tiles(rows, n), 256, 0, st>>>(rows, n, k, (const float*)x, ld_x, W, stride_wn, stride_wk, bias,
-                                                    add, ld_add, act, y, ld_y);
-  else
-    forward_kernel<<<tiles(rows, n), 256, 0, st>>>(rows, n, k, (const bf16*)x, ld_x, W, stride_wn, stride_wk, bias, add,
-                                                    ld_add, act, y, ld_y);
-  INF_LAUNCH_CHECK();
-  if (mask != nullptr) {
-    mask_kernel<<<blocks_of(rows * ((n + 31) / 32)), 256, 0, st>>>(rows, n, y, ld_y, mask);
-    INF_LAUNCH_CHECK();
-  }
-  return INF_OK;
+  if (rc != INF_OK) return rc;
+  rc = launch_split(W, stride_wn, stride_wk, n, k, ws + o.V, (int*)(ws + o.vshift), st);
+  if (rc != INF_OK) return rc;
+  a.rows = rows;
+  a.cols = n;
+  a.K = k;
+  a.x = x;
+  a.ldx = ld_x;
+  a.V = ws + o.V;
+  a.vshift = (int*)(ws + o.vshift);
+  a.bias = bias;
+  a.add = add;
+  a.ldadd = ld_add;
+  a.act = act;
+  a.out = y;
+  a.ldo = ld_y;
+  a.mask = mask;
+  return x_dtype == INF_DTYPE_F32 ? launch_tiles<0, 0, float, float>(a, st) : launch_tiles<0, 0, bf16, float>(a, st);
 }
 
 int inf_linear_ckpt_backward(int64_t rows, int n, int k, const float* dy, int64_t ld_dy, int act, const float* y,
@@ -170,6 +744,7 @@ int inf_linear_ckpt_backward(int64_t rows, int n, int k, const float* dy, int64_
                              int64_t ld_dx, float* dW, int64_t ld_dw, float* db, void* workspace,
                              inf_stream_t stream) {
   INF_CHECK_ARG(rows >= 0 && n >= 1 && k >= 1 && ld_dy >= 0, "linear_ckpt backward: bad shape");
+  INF_CHECK_ARG(rows < (int64_t)1 << 31, "linear_ckpt backward: too many rows");
   INF_CHECK_ARG(act >= 0 && act <= 2, "linear_ckpt backward: act must be 0 (none), 1 (ReLU) or 2 (sigmoid)");
   INF_CHECK_ARG(dx == nullptr || (W != nullptr && ld_dx >= k && (dx_dtype == INF_DTYPE_F32 || dx_dtype == INF_DTYPE_BF16)),
                 "linear_ckpt backward: dx needs the weight and is fp32 or bf16");
@@ -181,27 +756,12 @@ int inf_linear_ckpt_backward(int64_t rows, int n, int k, const float* dy, int64_
                                                ld_q % q8::Q_ALIGN == 0 && (uintptr_t)q % 16 == 0),
                 "linear_ckpt backward: dW needs the 8-bit rows");
   const hipStream_t st = (hipStream_t)stream;
-  float* dz = (float*)workspace;
-  if (rows > 0) {
-    dz_kernel<<<blocks_of(rows * n), 256, 0, st>>>(rows, n, dy, ld_dy, act, y, ld_y, mask, dz);
-    INF_LAUNCH_CHECK();
-  }
-  if (dx != nullptr && rows > 0) {
-    if (dx_dtype == INF_DTYPE_F32)
-      dx_kernel<<<tiles(rows, k), 256, 0, st>>>(rows, n, k, dz, W, stride_wn, stride_wk, (float*)dx, ld_dx);
-    else
-      dx_kernel<<<tiles(rows, k), 256, 0, st>>>(rows, n, k, dz, W, stride_wn, stride_wk, (bf16*)dx, ld_dx);
-    INF_LAUNCH_CHECK();
-  }
-  if (dW != nullptr) {
-    dw_kernel<<<tiles(n, k), 256, 0, st>>>(rows, n, k, dz, q, ld_q, scale, dW, ld_dw);
-    INF_LAUNCH_CHECK();
-  }
-  if (db != nullptr) {
-    db_kernel<<<n, 256, 0, st>>>(rows, n, dz, db);
-    INF_LAUNCH_CHECK();
-  }
-  return INF_OK;
+  const Dz dz{dy, ld_dy, y, ld_y, mask, (n + 31) / 32};
+  char* const ws = (char*)workspace;
+#define INF_BACKWARD(ACT) \
+  backward<ACT>(rows, n, k, dz, q, ld_q, scale, W, stride_wn, stride_wk, dx, dx_dtype, ld_dx, dW, ld_dw, db, ws, st)
+  return act == 1 ? INF_BACKWARD(DZ_RELU) : act == 2 ? INF_BACKWARD(DZ_SIGMOID) : INF_BACKWARD(DZ_NONE);
+#undef INF_BACKWARD
 }
 
 }  // extern "C"

@@ -65,6 +65,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
     for (int e = 0; e < V; ++e) a = max(a, abs_bits(v[i][e]));
   const RowScale rs = row_scale(row_max<LPR>(a));
   if (l == 0) scale[m] = rs.s;
+  if (q == nullptr) return;  // the scales alone
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int c = (i * LPR + l) * V;
@@ -105,6 +106,7 @@ __global__ __launch_bounds__(256) void quantize_long_rows_kernel(const T* __rest
     __syncthreads();
     const RowScale rs = row_scale(max(max(part[0], part[1]), max(part[2], part[3])));
     if (threadIdx.x == 0) scale[m] = rs.s;
+    if (q == nullptr) continue;
     for (int c = threadIdx.x * V; c < k; c += 256 * V) {
       load_chunk(x + m * ldx, c, k, v);
 #pragma unroll

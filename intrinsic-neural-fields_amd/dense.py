@@ -317,7 +317,7 @@ class _LinearCkpt(torch.autograd.Function):
                     rows, n, k, rt.ptr(x), xc, x.stride(0), W.data_ptr() + 4 * c0 * W.stride(1), W.stride(0),
                     W.stride(1), rt.ptr(b), rt.ptr(y) if s else None, n, act if last else 0, rt.ptr(y), n,
                     rt.ptr(mask) if last else None, rt.ptr(rows8.q) if make else None,
-                    rows8.q.stride(0) if make else 0, rt.ptr(rows8.scale) if make else None, rt.ptr(work), st),
+                    rows8.q.stride(0) if make else 0, rt.ptr(rows8.scale) if rows8 is not None else None, rt.ptr(work), st),
                     "linear_ckpt_forward")
                 save += [rows8.q, rows8.scale] if needs[nseg + wi] else [None, None]
         ctx.spec, ctx.act, ctx.nw, ctx.nb = spec, act, nw, len(bs)
