@@ -226,7 +226,8 @@ int inf_linear_int(int64_t rows, int n, int k, const void* x, int x_dtype, int64
  * add may be y.  q and scale: the rows of x in 8 bits, written; scale alone: x's own scales,
  * read (q made before); both NULL: nothing is kept.  mask (not NULL): bit j of
  * word w of row m (ceil(n / 32) words a row) = y[m][32 w + j] > 0.  workspace:
- * inf_linear_ckpt_workspace_bytes(.., 0) bytes.                                            */
+ * inf_linear_ckpt_workspace_bytes(.., 0) bytes.  n k below 2^29 (n and k padded to 256), rows
+ * of x, dy and y less than 2^21 values apart.                                              */
 int64_t inf_linear_ckpt_workspace_bytes(int64_t rows, int n, int k, int x_dtype, int backward);
 int inf_linear_ckpt_forward(int64_t rows, int n, int k, const void* x, int x_dtype, int64_t ld_x, const float* W,
                             int64_t stride_wn, int64_t stride_wk, const float* bias, const float* add, int64_t ld_add,

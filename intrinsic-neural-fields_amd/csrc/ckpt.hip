@@ -15,6 +15,7 @@
 //   scale (a column of dz has no scale that a sum over its rows could be divided by).
 // A value that is not finite makes NaN of the rows (and columns) that it enters.
 #include <algorithm>
+#include <cstdlib>
 
 #include "mtile.hpp"
 
@@ -25,76 +26,83 @@ using namespace q8;
 using namespace mt;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x8u __attribute__((ext_vector_type(8), aligned(4)));
-typedef bf16 bf16x8u __attribute__((ext_vector_type(8), aligned(2)));
 
 enum { DZ_NONE = 0, DZ_RELU = 1, DZ_SIGMOID = 2 };  // act
+
+// An offset that the compiler adds to its uniform base in the load itself: left to it, it adds
+// them before the loop, into two registers each, and spills.
+__device__ __forceinline__ unsigned pinned(unsigned o) {
+  asm volatile("" : "+v"(o));
+  return o;
+}
 
 // the power of two that takes a row of largest value a below 2^15
 __device__ __forceinline__ int shift_of(float a) { return 15 - __builtin_amdgcn_frexp_expf(a); }
 __device__ __forceinline__ float by_power(float v, int e) { return __builtin_amdgcn_ldexpf(v, e); }
 
-__device__ __forceinline__ void split8(const float (&v)[8], int shift, f16x8* hi, f16x8* lo) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float x = by_power(v[e], shift);
-    (*hi)[e] = (_Float16)x;
-    (*lo)[e] = (_Float16)(x - (float)(*hi)[e]);
-  }
-}
+// x = hi + lo, each rounded to nearest
+__device__ __forceinline__ _Float16 piece_hi(float x) { return (_Float16)x; }
+__device__ __forceinline__ _Float16 piece_lo(float x, _Float16 hi) { return (_Float16)(x - (float)hi); }
 
 // ---- the weight's rows as fp16 pieces ---------------------------------------------------
 // Row r of the product's side: V(r, k) = W[r sr + k sk], k < K, as blocks of 32 k: 64 bytes hi,
-// 64 bytes lo, zero behind K.  by_row: a wave a row, its lanes along k (sk is the short
-// stride); by column: a workgroup 64 rows, its lanes along the rows.
-__global__ __launch_bounds__(256) void split_rows_kernel(const float* __restrict__ W, int64_t sr, int64_t sk, int rows,
-                                                         int K, char* __restrict__ out, int* __restrict__ shift) {
-  const int r = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x % 64;
-  if (r >= rows) return;
-  const float* const w = W + r * sr;
-  unsigned a = 0;
-  for (int k = lane; k < K; k += 64) a = max(a, abs_bits(w[k * sk]));
+// 64 bytes lo, zero behind K.
+__device__ __forceinline__ void put_pieces(char* row, const float* w, int64_t sk, int c, int K, int e) {
+  float v[8];
 #pragma unroll
-  for (int h = 32; h > 0; h >>= 1) a = max(a, (unsigned)__shfl_xor((int)a, h));
-  const int e = shift_of(__uint_as_float(a));
-  if (lane == 0) shift[r] = e;
-  const int Kp = (K + 31) / 32 * 32;
-  for (int k = lane * 8; k < Kp; k += 512) {
-    float v[8];
+  for (int i = 0; i < 8; ++i) v[i] = c * 8 + i < K ? w[(c * 8 + i) * sk] : 0.f;
+  f16x8 hi, lo;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? w[(k + i) * sk] : 0.f;
-    f16x8 hi, lo;
-    split8(v, e, &hi, &lo);
-    char* const to = out + (int64_t)r * Kp * 4 + (k / 32) * 128 + (k % 32) * 2;
-    *reinterpret_cast<f16x8*>(to) = hi;
-    *reinterpret_cast<f16x8*>(to + 64) = lo;
+  for (int i = 0; i < 8; ++i) {
+    const float x = by_power(v[i], e);
+    hi[i] = piece_hi(x);
+    lo[i] = piece_lo(x, hi[i]);
   }
+  char* const to = row + c / 4 * 128 + c % 4 * 16;
+  *reinterpret_cast<f16x8*>(to) = hi;
+  *reinterpret_cast<f16x8*>(to + 64) = lo;
 }
 
-__global__ __launch_bounds__(256) void split_columns_kernel(const float* __restrict__ W, int64_t sr, int64_t sk,
-                                                            int rows, int K, char* __restrict__ out,
-                                                            int* __restrict__ shift) {
-  __shared__ unsigned top[4][64];
-  const int l = threadIdx.x % 64, g = threadIdx.x / 64, r = blockIdx.x * 64 + l;
-  const float* const w = W + min(r, rows - 1) * sr;
+// sk is the short stride: a workgroup a row, its threads along k
+__global__ __launch_bounds__(256) void split_rows_kernel(const float* __restrict__ W, int64_t sr, int64_t sk, int rows,
+                                                         int K, char* __restrict__ out, int* __restrict__ shift) {
+  __shared__ unsigned top[4];
+  const int r = blockIdx.x, tid = threadIdx.x;
+  const float* const w = W + r * sr;
   unsigned a = 0;
-  for (int k = g; k < K; k += 4) a = max(a, abs_bits(w[k * sk]));
-  top[g][l] = a;
+#pragma unroll 4
+  for (int k = tid; k < K; k += 256) a = max(a, abs_bits(w[k * sk]));
+#pragma unroll
+  for (int h = 32; h > 0; h >>= 1) a = max(a, (unsigned)__shfl_xor((int)a, h));
+  if (tid % 64 == 0) top[tid / 64] = a;
   __syncthreads();
-  const int e = shift_of(__uint_as_float(max(max(top[0][l], top[1][l]), max(top[2][l], top[3][l]))));
+  const int e = shift_of(__uint_as_float(max(max(top[0], top[1]), max(top[2], top[3]))));
+  if (tid == 0) shift[r] = e;
+  const int Kp = (K + 31) / 32 * 32;
+  for (int c = tid; c < Kp / 8; c += 256) put_pieces(out + (int64_t)r * Kp * 4, w, sk, c, K, e);
+}
+
+// sr is the short stride: a workgroup 16 rows, 16 threads along them and 64 along k
+__global__ __launch_bounds__(1024) void split_columns_kernel(const float* __restrict__ W, int64_t sr, int64_t sk,
+                                                             int rows, int K, char* __restrict__ out,
+                                                             int* __restrict__ shift) {
+  __shared__ unsigned top[16];
+  const int l = threadIdx.x % 16, g = threadIdx.x / 16, r = blockIdx.x * 16 + l;
+  const float* const w = W + min(r, rows - 1) * sr;
+  if (threadIdx.x < 16) top[threadIdx.x] = 0;
+  __syncthreads();
+  unsigned a = 0;
+#pragma unroll 4
+  for (int k = g; k < K; k += 64) a = max(a, abs_bits(w[k * sk]));
+  a = max(a, (unsigned)__shfl_xor((int)a, 16));
+  a = max(a, (unsigned)__shfl_xor((int)a, 32));
+  if (threadIdx.x % 64 < 16) atomicMax(&top[l], a);  // a maximum: in any order the same
+  __syncthreads();
   if (r >= rows) return;
+  const int e = shift_of(__uint_as_float(top[l]));
   if (g == 0) shift[r] = e;
   const int Kp = (K + 31) / 32 * 32;
-  for (int k = g * 8; k < Kp; k += 32) {
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? w[(k + i) * sk] : 0.f;
-    f16x8 hi, lo;
-    split8(v, e, &hi, &lo);
-    char* const to = out + (int64_t)r * Kp * 4 + (k / 32) * 128 + (k % 32) * 2;
-    *reinterpret_cast<f16x8*>(to) = hi;
-    *reinterpret_cast<f16x8*>(to + 64) = lo;
-  }
+  for (int c = g; c < Kp / 8; c += 64) put_pieces(out + (int64_t)r * Kp * 4, w, sk, c, K, e);
 }
 
 // ---- dz -------------------------------------------------------------------------------
@@ -133,9 +141,9 @@ __global__ __launch_bounds__(256) void dz_shift_kernel(Dz d, int64_t rows, int n
 // ---- x W^T and dz W -----------------------------------------------------------------------
 // out(m, c) = sum_k side(m, k) V(c, k): BM rows by BN columns a workgroup, WM x WN waves,
 // v_mfma_f32_16x16x32_f16 with V as its first operand (a lane holds four neighbouring
-// columns of one row).  Per turn 32 k: V's pieces go straight from memory to LDS, the rows of
-// x or dz through registers, where they are split, one turn ahead.  Two LDS stages of
-// 128-byte rows (64 hi, 64 lo).
+// columns of one row).  Per turn 32 k.  LDS: two stages of 128-byte rows (64 hi, 64 lo), V's
+// filled straight from memory one turn ahead.  The rows of x or dz are read in whole lines
+// into registers two turns ahead and split on their way to LDS, each value once.
 struct SideArgs {
   int64_t rows;
   int cols, K;          // output columns; length of the sums
@@ -161,8 +169,7 @@ struct ST {
   static constexpr int WROWS = BM / WM, WCOLS = BN / WN, TI = WROWS / 16, TJ = WCOLS / 16;
   static constexpr int STAGE = (BM + BN) * 128, LDS = 2 * STAGE;
   static constexpr int LOADS = BN * 128 / (THREADS * 16);
-  static constexpr int PASS = BM / (THREADS / 4);  // rows that a thread splits a turn (8 values each)
-  static_assert(BN * 128 % (THREADS * 16) == 0 && BM % (THREADS / 4) == 0 && LDS <= 160 * 1024, "tile");
+  static_assert(BN * 128 % (THREADS * 16) == 0 && LDS <= 160 * 1024, "tile");
   static_assert(WCOLS % 32 == 0, "a wave holds whole words of the mask");
 };
 
@@ -170,8 +177,14 @@ struct ST {
 template <int MODE, int ACT, typename X, typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, int tiles_n, int nblocks) {
   using P = ST<BM, BN, WM, WN>;
-  constexpr int TI = P::TI, TJ = P::TJ, PASS = P::PASS;
-  constexpr bool LO = sizeof(X) == 4;  // a bf16 value is one piece
+  constexpr int TI = P::TI, TJ = P::TJ;
+  constexpr bool LO = sizeof(X) == 4;         // a bf16 value is one piece
+  constexpr int V = 16 / sizeof(X);           // values of a 16-byte load
+  constexpr int LANES = 32 / V;               // lanes that load a row's 32 values
+  constexpr int PASS = BM * LANES / P::THREADS;
+  constexpr bool MASK = MODE == 1 && ACT == DZ_RELU, WITH_Y = MODE == 1 && ACT == DZ_SIGMOID;
+  constexpr int ROW_LOADS = PASS * (MASK || WITH_Y ? 2 : 1);  // at least so many loads a turn
+  static_assert(PASS * P::THREADS == BM * LANES, "tile");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int bid = xcd_order((int)blockIdx.x, nblocks);
   const int64_t m0 = (int64_t)(bid / tiles_n) * BM;
@@ -179,74 +192,91 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wave / WN, wc = wave % WN, r16 = lane & 15, g4 = lane >> 4;
   const int turns = (a.K + 31) / 32;
-  const int64_t ldv = (int64_t)turns * 128;
 
-  const char* src[P::LOADS];
-#pragma unroll
-  for (int i = 0; i < P::LOADS; ++i) {
-    const int p = tid + P::THREADS * i, row = p >> 3;
-    src[i] = a.V + min(n0 + row, a.cols - 1) * ldv + (((p & 7) ^ swz(row)) << 4);
-  }
-  auto issue = [&](int t) {
-    char* st = smem + (t & 1) * P::STAGE;
+  // (offsets of 32 bits from uniform bases: with 128 registers a lane each address counts)
+  // rows of V behind the last are in the workspace, whatever they hold: their columns are not stored
+  const unsigned src = (unsigned)(n0 + (tid >> 3)) * (unsigned)turns * 128u + (unsigned)(((tid & 7) ^ swz(tid >> 3)) << 4);
+  static_assert(P::THREADS / 8 % 16 == 0, "the swizzle of a thread's rows is the same");
+  auto issue = [&](int t, int stage) {
+    char* st = smem + (stage & 1) * P::STAGE;
 #pragma unroll
     for (int i = 0; i < P::LOADS; ++i) {
-      const char* from = src[i] + t * 128;
+      const char* const V = a.V + (int64_t)t * 128 + (int64_t)i * (P::THREADS / 8) * turns * 128;
+      const char* from = V + pinned(src);
       __builtin_amdgcn_global_load_lds(from, (lds_void*)(st + (wave + (P::THREADS / 64) * i) * 1024), 16, 0, 0);
     }
   };
-  const int c8 = (tid & 3) * 8;
-  int shift[PASS];
-  int64_t row[PASS];
+  // this thread's rows (PASS of them) and its values of each turn: k = V (tid % LANES) + (0..V)
+  const int kc = (tid % LANES) * V;
+  auto row_of = [&](int p) { return tid / LANES + p * (P::THREADS / LANES); };
+  const X* const side = MODE == 0 ? (const X*)a.x + m0 * a.ldx : (const X*)a.dz.dy + m0 * a.dz.lddy;
+  const float* const ys = WITH_Y ? a.dz.y + m0 * a.dz.ldy : nullptr;
+  const uint32_t* const words = MASK ? a.dz.mask + m0 * a.dz.words : nullptr;
+  int shift[PASS], off[PASS], yoff[WITH_Y ? PASS : 1], woff[MASK ? PASS : 1];
 #pragma unroll
   for (int p = 0; p < PASS; ++p) {
-    row[p] = min(m0 + (tid >> 2) + p * (P::THREADS / 4), a.rows - 1);
-    shift[p] = MODE == 0 ? shift_of(a.scale[row[p]] * 127.f) : a.shift[row[p]];
+    const int r = (int)min((int64_t)row_of(p), a.rows - 1 - m0);
+    shift[p] = MODE == 0 ? shift_of(a.scale[m0 + r] * 127.f) : a.shift[m0 + r];
+    off[p] = r * (int)(MODE == 0 ? a.ldx : a.dz.lddy);
+    if constexpr (WITH_Y) yoff[p] = r * (int)a.dz.ldy;
+    if constexpr (MASK) woff[p] = r * a.dz.words;
   }
-  float v[PASS][8];
-  auto fetch = [&](int t) {
-    const int k = t * 32 + c8;
+  struct Raw {
+    X v[PASS][V];
+    float y[WITH_Y ? PASS : 1][4];
+    uint32_t w[MASK ? PASS : 1];
+  };
+  typedef X XV __attribute__((ext_vector_type(V), aligned(sizeof(X))));
+  // The last 32 k, which may be fewer, are the first turn: the loop has whole ones alone.
+  auto block_of = [&](int t) { return t == 0 ? turns - 1 : min(t, turns - 1) - 1; };
+  // Nothing here uses what it loads: the waits belong to put(), a turn later.
+  auto fetch = [&](Raw& r, int block) {
+    const int k = block * 32 + kc;
 #pragma unroll
     for (int p = 0; p < PASS; ++p) {
-      const X* const from = MODE == 0 ? (const X*)a.x + row[p] * a.ldx : (const X*)a.dz.dy + row[p] * a.dz.lddy;
-      if (k + 8 <= a.K) {
-        if constexpr (sizeof(X) == 4) {
-          const f32x8u x = *reinterpret_cast<const f32x8u*>(from + k);
+      const XV x = *reinterpret_cast<const XV*>((const char*)side + pinned((unsigned)(off[p] + k) * sizeof(X)));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[p][e] = x[e];
-        } else {
-          const bf16x8u x = *reinterpret_cast<const bf16x8u*>(from + k);
+      for (int e = 0; e < V; ++e) r.v[p][e] = x[e];
+      if constexpr (WITH_Y) {
+        const f32x4u y = *reinterpret_cast<const f32x4u*>((const char*)ys + pinned((unsigned)(yoff[p] + k) * 4u));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[p][e] = (float)x[e];
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[p][e] = k + e < a.K ? to_f32(from[k + e]) : 0.f;
+        for (int e = 0; e < 4; ++e) r.y[p][e] = y[e];
       }
-      if constexpr (MODE == 1 && ACT == DZ_RELU) {
-        const uint32_t w = a.dz.mask[row[p] * a.dz.words + t] >> c8;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[p][e] = (w >> e) & 1 ? v[p][e] : 0.f;
-      }
-      if constexpr (MODE == 1 && ACT == DZ_SIGMOID) {
-        const float* const yr = a.dz.y + row[p] * a.dz.ldy;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y = k + e < a.K ? yr[k + e] : 0.f;
-          v[p][e] = v[p][e] * (y * (1.f - y));
-        }
-      }
+      if constexpr (MASK)
+        r.w[p] = *reinterpret_cast<const uint32_t*>((const char*)words + pinned((unsigned)(woff[p] + block) * 4u));
     }
   };
-  auto put = [&](int t) {
+  auto fetch_last = [&](Raw& r) {
+    const int k = (turns - 1) * 32 + kc;
+#pragma unroll
+    for (int p = 0; p < PASS; ++p) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int ke = min(k + e, a.K - 1);
+        r.v[p][e] = k + e < a.K ? side[off[p] + ke] : (X)0.f;
+        if constexpr (WITH_Y) r.y[p][e] = ys[yoff[p] + ke];
+      }
+      if constexpr (MASK) r.w[p] = words[woff[p] + turns - 1];
+    }
+  };
+  auto put = [&](const Raw& r, int t) {
     char* st = smem + (t & 1) * P::STAGE;
 #pragma unroll
     for (int p = 0; p < PASS; ++p) {
-      const int r = BN + (tid >> 2) + p * (P::THREADS / 4), c = tid & 3;
-      f16x8 hi, lo;
-      split8(v[p], shift[p], &hi, &lo);
-      *reinterpret_cast<f16x8*>(st + chunk_at(r, c)) = hi;
-      if (LO) *reinterpret_cast<f16x8*>(st + chunk_at(r, 4 + c)) = lo;
+      typedef _Float16 Piece __attribute__((ext_vector_type(V)));
+      Piece hi, lo;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float v = to_f32(r.v[p][e]);
+        if constexpr (WITH_Y) v *= r.y[p][e] * (1.f - r.y[p][e]);
+        if constexpr (MASK) v = (r.w[p] >> (kc + e)) & 1 ? v : 0.f;
+        const float x = by_power(v, shift[p]);
+        hi[e] = piece_hi(x);
+        if (LO) lo[e] = piece_lo(x, hi[e]);
+      }
+      const int row = BN + row_of(p);
+      *reinterpret_cast<Piece*>(st + chunk_at(row, kc / 8) + (kc % 8) * 2) = hi;
+      if (LO) *reinterpret_cast<Piece*>(st + chunk_at(row, 4 + kc / 8) + (kc % 8) * 2) = lo;
     }
   };
 
@@ -255,41 +285,55 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
   for (int j = 0; j < TJ; ++j)
 #pragma unroll
     for (int i = 0; i < TI; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  issue(0);
-  fetch(0);
-  put(0);
-  wait_all_barrier();
-#pragma unroll 1
-  for (int t = 0; t < turns; ++t) {
-    const bool more = t + 1 < turns;
-    if (more) {
-      issue(t + 1);
-      fetch(t + 1);
-    }
+  // Two passes over the products, so that one of V's pieces at a time is held: hi of V by both
+  // pieces of the rows, then lo of V by hi of the rows.
+  auto turn_products = [&](int t) {
     const char* st = smem + (t & 1) * P::STAGE;
-    f16x8 xh[TI], xl[TI];
+    f16x8 w[TJ];
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) w[j] = *reinterpret_cast<const f16x8*>(st + chunk_at(wc * P::WCOLS + 16 * j + r16, g4));
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
       const int r = BN + wr * P::WROWS + 16 * i + r16;
-      xh[i] = *reinterpret_cast<const f16x8*>(st + chunk_at(r, g4));
-      if (LO) xl[i] = *reinterpret_cast<const f16x8*>(st + chunk_at(r, 4 + g4));
+      if (LO) {
+        const f16x8 xl = *reinterpret_cast<const f16x8*>(st + chunk_at(r, 4 + g4));
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], xl, acc[j][i], 0, 0, 0);
+      }
+      const f16x8 xh = *reinterpret_cast<const f16x8*>(st + chunk_at(r, g4));
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], xh, acc[j][i], 0, 0, 0);
     }
 #pragma unroll
-    for (int j = 0; j < TJ; ++j) {
-      const int r = wc * P::WCOLS + 16 * j + r16;
-      const f16x8 wh = *reinterpret_cast<const f16x8*>(st + chunk_at(r, g4));
-      const f16x8 wl = *reinterpret_cast<const f16x8*>(st + chunk_at(r, 4 + g4));
+    for (int j = 0; j < TJ; ++j)
+      w[j] = *reinterpret_cast<const f16x8*>(st + chunk_at(wc * P::WCOLS + 16 * j + r16, 4 + g4));
 #pragma unroll
-      for (int i = 0; i < TI; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl, xh[i], acc[j][i], 0, 0, 0);
-      if (LO)
+    for (int i = 0; i < TI; ++i) {
+      const f16x8 xh = *reinterpret_cast<const f16x8*>(st + chunk_at(BN + wr * P::WROWS + 16 * i + r16, g4));
 #pragma unroll
-        for (int i = 0; i < TI; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, xl[i], acc[j][i], 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < TI; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, xh[i], acc[j][i], 0, 0, 0);
+      for (int j = 0; j < TJ; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], xh, acc[j][i], 0, 0, 0);
     }
-    if (more) put(t + 1);
-    wait_all_barrier();
+  };
+  Raw raw;
+  issue(block_of(0), 0);
+  fetch_last(raw);
+  put(raw, 0);
+  if (turns > 1) fetch(raw, block_of(1));
+  wait_barrier<0>();
+#pragma unroll 1
+  for (int t = 0; t + 1 < turns; ++t) {
+    issue(block_of(t + 1), t + 1);
+    // the parts stay apart: interleaved they need more registers than there are
+    __builtin_amdgcn_sched_barrier(0);
+    turn_products(t);
+    __builtin_amdgcn_sched_barrier(0);
+    put(raw, t + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(raw, block_of(t + 2));  // past the last: the last again, so that the waits can be counted
+    wait_barrier<ROW_LOADS>();    // V's loads are older than the rows'
   }
+  turn_products(turns - 1);
+  wait_barrier<0>();
 
   // lane: row wr WROWS + 16 i + r16, columns wc WCOLS + 16 j + 4 g4 + (0..3)
   int sm[TI];
@@ -298,34 +342,55 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
     const int64_t m = min(m0 + wr * P::WROWS + 16 * i + r16, a.rows - 1);
     sm[i] = MODE == 0 ? shift_of(a.scale[m] * 127.f) : a.shift[m];
   }
-  uint32_t bits[TI];
+  int sn[TJ][4];
+  float bias[TJ][4];
 #pragma unroll
-  for (int j = 0; j < TJ; ++j) {
-    const int n = n0 + wc * P::WCOLS + 16 * j + 4 * g4;
-    int sn[4];
-    float bias[4];
+  for (int j = 0; j < TJ; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      sn[e] = a.vshift[min(n + e, a.cols - 1)];
-      bias[e] = MODE == 0 && a.bias != nullptr ? a.bias[min(n + e, a.cols - 1)] : 0.f;
+      const int n = min(n0 + wc * P::WCOLS + 16 * j + 4 * g4 + e, a.cols - 1);
+      sn[j][e] = a.vshift[n];
+      bias[j][e] = MODE == 0 && a.bias != nullptr ? a.bias[n] : 0.f;
     }
+  // Rows that all start on 16 bytes are stored from the registers.  Others (k = 1023) go through
+  // this wave's own piece of LDS, so that a store is one run of a row: 16-byte stores across
+  // lines took 224 us where these take 163 (65,536 x 1023 x 256, dx).
+  const bool direct = ((uintptr_t)a.out | (uintptr_t)(a.ldo * sizeof(T))) % 16 == 0;
+  constexpr int RS = P::WCOLS * 4 + 16;
+  static_assert(WM * WN * 16 * RS <= P::LDS, "the waves' pieces fit the stages");
+  char* const mine = smem + wave * 16 * RS;
 #pragma unroll
-    for (int i = 0; i < TI; ++i) {
-      const int64_t m = m0 + wr * P::WROWS + 16 * i + r16;
+  for (int i = 0; i < TI; ++i) {
+    const int64_t m = m0 + wr * P::WROWS + 16 * i + r16;
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+      const int n = n0 + wc * P::WCOLS + 16 * j + 4 * g4;
       float z[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        z[e] = by_power(acc[j][i][e], -(sm[i] + sn[e]));
-        if (MODE == 0) {
-          z[e] += bias[e];
-          if (a.add != nullptr && m < a.rows && n + e < a.cols) z[e] += a.add[m * a.ldadd + n + e];
-          z[e] = activate(z[e], a.act);
+      for (int e = 0; e < 4; ++e) z[e] = by_power(acc[j][i][e], -(sm[i] + sn[j][e])) + bias[j][e];
+      if (MODE == 0) {
+        if (a.add != nullptr && m < a.rows) {
+          const float* const from = a.add + m * a.ldadd + n;
+          if (n + 4 <= a.cols) {
+            const f32x4u v = *reinterpret_cast<const f32x4u*>(from);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] += v[e];
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n + e < a.cols) z[e] += from[e];
+          }
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = activate(z[e], a.act);
       }
-      if (m < a.rows) {
+      if (!direct) {
+        *reinterpret_cast<f32x4*>(mine + r16 * RS + (16 * j + 4 * g4) * 4) = f32x4{z[0], z[1], z[2], z[3]};
+      } else if (m < a.rows) {
         T* const to = reinterpret_cast<T*>(a.out) + m * a.ldo + n;
         if (n + 4 <= a.cols) {
-          typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+          typedef T V4 __attribute__((ext_vector_type(4)));
           V4 o;
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(z[e]);
@@ -343,26 +408,43 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
         b |= (uint32_t)__shfl_xor((int)b, 16);
         b |= (uint32_t)__shfl_xor((int)b, 32);
         if (j % 2 == 0) {
-          bits[i] = b;
+          bits = b;
         } else if (g4 == 0 && m < a.rows && n - 16 < a.cols) {
-          a.mask[m * ((a.cols + 31) / 32) + (n - 16) / 32] = bits[i] | b << 16;
+          a.mask[m * ((a.cols + 31) / 32) + (n - 16) / 32] = bits | b << 16;
         }
+      }
+    }
+    if (!direct) {
+      constexpr int AT_ONCE = 64 / P::WCOLS;  // rows of a store
+      const int c = lane % P::WCOLS, n = n0 + wc * P::WCOLS + c;
+#pragma unroll
+      for (int r = 0; r < 16; r += AT_ONCE) {
+        const int row = r + lane / P::WCOLS;
+        const int64_t mr = m0 + wr * P::WROWS + 16 * i + row;
+        const float v = *reinterpret_cast<const float*>(mine + row * RS + c * 4);
+        if (mr < a.rows && n < a.cols) reinterpret_cast<T*>(a.out)[mr * a.ldo + n] = from_f32<T>(v);
       }
     }
   }
 }
 
 // ---- dW and db ------------------------------------------------------------------------
-// dW(n, k) = sum_m dz(m, n) s_m q(m, k): 128 n by 256 k a workgroup, 2 x 4 waves, 32 rows m a
+// dW(n, k) = sum_m dz(m, n) s_m q(m, k): 128 n by 256 k a workgroup, 4 x 4 waves, 32 rows m a
 // turn, v_mfma_f32_16x16x32_bf16 with q as its first operand (a lane holds four neighbouring
-// k of one n).  Both sides are turned on the way to LDS: a thread loads one column of 8 (4)
-// rows, neighbouring threads neighbouring columns.  The rows are divided over `splits`
+// k of one n).  Both sides are turned on the way to LDS: a thread loads one column (four of q) of
+// 4 (2) rows, neighbouring threads neighbouring columns.  Bound by these conversions next to
+// the products: 16 waves, so that one's run beside another's.  The rows are divided over `splits`
 // workgroups a tile, whose sums add_slabs_kernel adds in order: no atomics.
-constexpr int DW_N = 128, DW_K = 256, DW_THREADS = 512;
+constexpr int DW_N = 128, DW_K = 256, DW_THREADS = 1024;
 constexpr int DW_STAGE = DW_K * 64 + 3 * DW_N * 64;  // q rows, then the pieces of dz: hi, mid, lo
 constexpr int DW_LDS = 2 * DW_STAGE;
 
-__device__ __forceinline__ int at64(int row, int c) { return row * 64 + ((c ^ ((row >> 2) & 3)) << 4); }
+// Chunk c (16 bytes) of a 64-byte LDS row.  A 16-byte read serves 16 lanes at a time, rows 0-3 and
+// 12-15 of one c with rows 4-11 of the next: the last term but one sends them to 16 places.  The
+// turn of four rows and the last term do the same for writes to every fourth row.
+__device__ __forceinline__ int at64(int r, int c) {
+  return (r >> 2) * 256 + (((r + (r >> 2)) & 3) << 6) + (((c ^ -(r >> 2) ^ (r >> 4)) & 3) << 4);
+}
 __device__ __forceinline__ uint32_t top_halves(float a, float b) {  // bf16 of a (low) and b, both exact
   return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
 }
@@ -389,92 +471,124 @@ __global__ __launch_bounds__(DW_THREADS) void dw_tile_kernel(DwArgs a) {
   const int split = bid / a.tiles, tile = bid % a.tiles;
   const int n0 = tile / a.tiles_k * DW_N, k0 = tile % a.tiles_k * DW_K;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wn = wave / 4, wk = wave % 4, r16 = lane & 15, g4 = lane >> 4;
+  const int wn = wave / 4, wk = wave % 4, r16 = lane & 15, g4 = lane >> 4;  // 32 n by 64 k a wave
   const int64_t mb = split * a.rows_a_split, me = min(mb + a.rows_a_split, a.rows);
   const int turns = (int)((me - mb + 31) / 32);
 
-  const int zc = tid & 127, zg = tid >> 7;  // dz: column, group of 8 rows
-  const int n = n0 + zc;
-  const bool in_n = n < a.n;
-  const int qc = tid & 63, qg = tid >> 6;   // q: 4 columns, group of 4 rows
-  const int64_t kq = min((int64_t)(k0 + 4 * qc), a.ldq - 4);
-  float z[8];
+  const int zc = tid & 127, zg = tid >> 7;  // dz: column, group of 4 rows
+  const int n = n0 + zc, nc = min(n, a.n - 1);
+  const bool in_n = n < a.n, with_db = a.db != nullptr && k0 == 0;
+  const int qc = tid & 63, qg = tid >> 6;   // q: 4 columns, group of 2 rows
+  const int kq = (int)min((int64_t)(k0 + 4 * qc), a.ldq - 4);
+  float z[4], y[ACT == DZ_SIGMOID ? 4 : 1], s[4];
+  uint32_t w[ACT == DZ_RELU ? 4 : 1];
   float dbsum = 0.f;
-  int q[4];
-  float s[8];
-  auto fetch = [&](int t) {
-    const int64_t mz = mb + t * 32 + zg * 8, mq = mb + t * 32 + qg * 4;
+  int q[2];
+  // The rows of a split's last turn, which may be fewer, are the first: the loop has whole turns
+  // alone, whose addresses are a uniform base each and one offset of 32 bits.
+  const auto block_of = [&](int t) { return t == 0 ? turns - 1 : t - 1; };
+  const unsigned zoff = (unsigned)(zg * 4) * (unsigned)a.dz.lddy + nc, yoff = (unsigned)(zg * 4) * (unsigned)a.dz.ldy + nc;
+  const unsigned woff = (unsigned)(zg * 4 * a.dz.words + nc / 32), qoff = (unsigned)(qg * 2) * (unsigned)a.ldq + kq;
+  auto fetch = [&](int block) {
+    const int64_t m = mb + block * 32;
+    const float* const dy = a.dz.dy + m * a.dz.lddy;
+    const f32x4u s0 = *reinterpret_cast<const f32x4u*>(a.s + m + zg * 4);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bool in = in_n && mz + e < me;
-      z[e] = in ? dz_at<ACT>(a.dz, mz + e, n) : 0.f;
-      s[e] = in ? a.s[mz + e] : 0.f;
+    for (int e = 0; e < 4; ++e) {
+      z[e] = (dy + e * a.dz.lddy)[pinned(zoff)];
+      s[e] = s0[e];
+      if constexpr (ACT == DZ_RELU) w[e] = (a.dz.mask + (m + e) * a.dz.words)[pinned(woff)];
+      if constexpr (ACT == DZ_SIGMOID) y[e] = (a.dz.y + (m + e) * a.dz.ldy)[pinned(yoff)];
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[e] = *reinterpret_cast<const int*>(a.q + min(mq + e, a.rows - 1) * a.ldq + kq);
+    for (int e = 0; e < 2; ++e) q[e] = *reinterpret_cast<const int*>(a.q + (m + e) * a.ldq + pinned(qoff));
+  };
+  auto fetch_last = [&]() {  // rows past the end: the last row, times zero
+    const int64_t mz = mb + (turns - 1) * 32 + zg * 4, mq = mb + (turns - 1) * 32 + qg * 2;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t m = min(mz + e, me - 1);
+      z[e] = mz + e < me ? a.dz.dy[m * a.dz.lddy + nc] : 0.f;
+      s[e] = mz + e < me ? a.s[m] : 0.f;
+      if constexpr (ACT == DZ_RELU) w[e] = a.dz.mask[m * a.dz.words + nc / 32];
+      if constexpr (ACT == DZ_SIGMOID) y[e] = mz + e < me ? a.dz.y[m * a.dz.ldy + nc] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) q[e] = *reinterpret_cast<const int*>(a.q + min(mq + e, me - 1) * a.ldq + kq);
   };
   auto put = [&](int t) {
     char* st = smem + (t & 1) * DW_STAGE;
-    u32x4 piece[3];
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (ACT == DZ_RELU)  // the mask's bit as all bits
+        z[e] = __uint_as_float(__float_as_uint(z[e]) & (unsigned)__builtin_amdgcn_sbfe((int)w[e], nc & 31, 1));
+      if constexpr (ACT == DZ_SIGMOID) z[e] *= y[e] * (1.f - y[e]);
+    }
+    if (with_db)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dbsum += z[e];
+    u32x2 piece[3];
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
       float v[2] = {z[e] * s[e], z[e + 1] * s[e + 1]};
-      dbsum += z[e];
-      dbsum += z[e + 1];
 #pragma unroll
       for (int p = 0; p < 3; ++p) {
         piece[p][e / 2] = top_halves(v[0], v[1]);
+        if (p < 2)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) v[u] -= __uint_as_float(__float_as_uint(v[u]) & 0xffff0000u);
+          for (int u = 0; u < 2; ++u) v[u] -= __uint_as_float(__float_as_uint(v[u]) & 0xffff0000u);
       }
     }
 #pragma unroll
     for (int p = 0; p < 3; ++p)
-      *reinterpret_cast<u32x4*>(st + DW_K * 64 + p * DW_N * 64 + at64(zc, zg)) = piece[p];
+      *reinterpret_cast<u32x2*>(st + DW_K * 64 + p * DW_N * 64 + at64(zc, zg / 2) + (zg & 1) * 8) = piece[p];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      u32x2 w;
-      w[0] = top_halves((float)(int8_t)(q[0] >> (8 * c)), (float)(int8_t)(q[1] >> (8 * c)));
-      w[1] = top_halves((float)(int8_t)(q[2] >> (8 * c)), (float)(int8_t)(q[3] >> (8 * c)));
-      *reinterpret_cast<u32x2*>(st + at64(4 * qc + c, qg / 2) + (qg & 1) * 8) = w;
-    }
+    for (int c = 0; c < 4; ++c)
+      *reinterpret_cast<uint32_t*>(st + at64(4 * qc + c, qg / 4) + (qg & 3) * 4) =
+          top_halves((float)(int8_t)(q[0] >> (8 * c)), (float)(int8_t)(q[1] >> (8 * c)));
   };
-  f32x4 acc[4][4];  // [k tile][n tile]
+  f32x4 acc[4][2];  // [k tile][n tile]
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (turns > 0) {
-    fetch(0);
-    put(0);
-  }
-  wait_all_barrier();
-#pragma unroll 1
-  for (int t = 0; t < turns; ++t) {
-    if (t + 1 < turns) fetch(t + 1);
+    for (int i = 0; i < 2; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto turn_products = [&](int t) {
     const char* st = smem + (t & 1) * DW_STAGE;
     bf16x8 qf[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) qf[j] = *reinterpret_cast<const bf16x8*>(st + at64(wk * 64 + 16 * j + r16, g4));
 #pragma unroll
     for (int p = 2; p >= 0; --p) {
-      bf16x8 zf[4];
+      bf16x8 zf[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        zf[i] = *reinterpret_cast<const bf16x8*>(st + DW_K * 64 + p * DW_N * 64 + at64(wn * 64 + 16 * i + r16, g4));
+      for (int i = 0; i < 2; ++i)
+        zf[i] = *reinterpret_cast<const bf16x8*>(st + DW_K * 64 + p * DW_N * 64 + at64(wn * 32 + 16 * i + r16, g4));
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
           acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[j], zf[i], acc[j][i], 0, 0, 0);
     }
-    if (t + 1 < turns) put(t + 1);
+  };
+  if (turns > 0) {
+    fetch_last();
+    put(0);
+    if (turns > 1) fetch(block_of(1));
+    wait_all_barrier();
+#pragma unroll 1
+    for (int t = 0; t + 1 < turns; ++t) {
+      turn_products(t);
+      put(t + 1);
+      if (t + 2 < turns) fetch(block_of(t + 2));
+      wait_lds_barrier();
+    }
+    turn_products(turns - 1);
     wait_all_barrier();
   }
   float* const out = a.out + (int64_t)split * a.n * a.ldw;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = n0 + wn * 64 + 16 * i + r16;
+  for (int i = 0; i < 2; ++i) {
+    const int c = n0 + wn * 32 + 16 * i + r16;
     if (c >= a.n) continue;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -493,11 +607,16 @@ __global__ __launch_bounds__(DW_THREADS) void dw_tile_kernel(DwArgs a) {
     }
   }
   if (a.db != nullptr && k0 == 0) {
-    float* const part = reinterpret_cast<float*>(smem);  // every wave has read its last stage
+    float* const part = reinterpret_cast<float*>(smem);
     part[zg * DW_N + zc] = dbsum;
     __syncthreads();
     if (tid < DW_N && in_n)
-      a.db[(int64_t)split * a.n + n] = (part[zc] + part[DW_N + zc]) + (part[2 * DW_N + zc] + part[3 * DW_N + zc]);
+    {
+      float v = 0.f;
+#pragma unroll
+      for (int g = 0; g < 8; ++g) v += part[g * DW_N + zc];
+      a.db[(int64_t)split * a.n + n] = v;
+    }
   }
 }
 
@@ -549,21 +668,26 @@ int launch_tile(const SideArgs& a, hipStream_t stream) {
   return INF_OK;
 }
 
-// The widest tile that still gives every CU a workgroup.
+// The widest tile that still fills the CUs.  65,536 x 1024 x 256: forward 108 us with 256 x 256
+// (one of 16 waves a CU), 128 with 128 x 128 (two of 8); dx, whose sums are short and whose
+// results are many, 163 with 128 x 128, where one's stores run beside the other's products, 172
+// with 256 x 128.
 template <int MODE, int ACT, typename X, typename T>
 int launch_tiles(const SideArgs& a, hipStream_t stream) {
   const int64_t wide = ceil_div(a.rows, 256);
-  if (a.cols <= 32 && wide >= 128) return launch_tile<MODE, ACT, X, T, 256, 32, 4, 1>(a, stream);
-  if (a.cols <= 128 && wide >= 256) return launch_tile<MODE, ACT, X, T, 256, 128, 4, 2>(a, stream);
-  if (a.cols > 128 && wide * ceil_div(a.cols, 256) >= 256) return launch_tile<MODE, ACT, X, T, 256, 256, 2, 4>(a, stream);
+  if (a.cols <= 32) return launch_tile<MODE, ACT, X, T, 64, 32, 4, 1>(a, stream);
+  if constexpr (MODE == 0)
+    if (a.cols > 128 && wide * ceil_div(a.cols, 256) >= 256)
+      return launch_tile<MODE, ACT, X, T, 256, 256, 4, 4>(a, stream);
+  if (ceil_div(a.rows, 128) * ceil_div(a.cols, 128) >= 512) return launch_tile<MODE, ACT, X, T, 128, 128, 4, 2>(a, stream);
   return launch_tile<MODE, ACT, X, T, 64, 64, 2, 2>(a, stream);
 }
 
 int launch_split(const float* W, int64_t sr, int64_t sk, int rows, int K, char* out, int* shift, hipStream_t stream) {
   if (std::abs(sk) <= std::abs(sr))
-    split_rows_kernel<<<(unsigned)ceil_div(rows, 4), 256, 0, stream>>>(W, sr, sk, rows, K, out, shift);
+    split_rows_kernel<<<(unsigned)rows, 256, 0, stream>>>(W, sr, sk, rows, K, out, shift);
   else
-    split_columns_kernel<<<(unsigned)ceil_div(rows, 64), 256, 0, stream>>>(W, sr, sk, rows, K, out, shift);
+    split_columns_kernel<<<(unsigned)ceil_div(rows, 16), 1024, 0, stream>>>(W, sr, sk, rows, K, out, shift);
   INF_LAUNCH_CHECK();
   return INF_OK;
 }
@@ -603,6 +727,12 @@ DwShape dw_shape(int64_t rows, int n, int k) {
   return d;
 }
 
+// what the products' 32-bit offsets reach: a weight's pieces, and 256 rows
+bool fits(int n, int k, int64_t ld) {
+  return round_up(n, 256) * round_up(k, 32) < (int64_t)1 << 29 && round_up(k, 256) * round_up(n, 32) < (int64_t)1 << 29 &&
+         ld < (int64_t)1 << 21;
+}
+
 // offsets in the workspace
 struct ForwardSpace {
   int64_t scale, V, vshift, bytes;
@@ -611,7 +741,7 @@ ForwardSpace forward_space(int64_t rows, int n, int k) {
   ForwardSpace w;
   w.scale = 0;
   w.V = w.scale + round_up(rows * 4, 256);
-  w.vshift = w.V + round_up(n * round_up(k, 32) * 4, 256);
+  w.vshift = w.V + round_up(n, 256) * round_up(k, 32) * 4;
   w.bytes = w.vshift + round_up((int64_t)n * 4, 256);
   return w;
 }
@@ -623,7 +753,7 @@ BackwardSpace backward_space(int64_t rows, int n, int k) {
   BackwardSpace w;
   w.shift = 0;
   w.V = w.shift + round_up(rows * 4, 256);
-  w.vshift = w.V + round_up(k * round_up(n, 32) * 4, 256);
+  w.vshift = w.V + round_up(k, 256) * round_up(n, 32) * 4;
   w.slabs = w.vshift + round_up((int64_t)k * 4, 256);
   w.db = w.slabs + round_up((int64_t)d.splits * n * k * 4, 256);
   w.bytes = w.db + round_up((int64_t)d.splits * n * 4, 256);
@@ -696,7 +826,7 @@ int inf_linear_ckpt_forward(int64_t rows, int n, int k, const void* x, int x_dty
                             int act, float* y, int64_t ld_y, uint32_t* mask, int8_t* q, int64_t ld_q, float* scale,
                             void* workspace, inf_stream_t stream) {
   INF_CHECK_ARG(rows >= 0 && n >= 1 && k >= 1 && ld_x >= 0 && ld_y >= n, "linear_ckpt: bad shape");
-  INF_CHECK_ARG(rows < (int64_t)1 << 31, "linear_ckpt: too many rows");
+  INF_CHECK_ARG(rows < (int64_t)1 << 31 && fits(n, k, ld_x), "linear_ckpt: too large");
   INF_CHECK_ARG(act >= 0 && act <= 2, "linear_ckpt: act must be 0 (none), 1 (ReLU) or 2 (sigmoid)");
   INF_CHECK_ARG(x_dtype == INF_DTYPE_F32 || x_dtype == INF_DTYPE_BF16, "linear_ckpt: x must be fp32 or bf16");
   if (rows == 0) return INF_OK;
@@ -744,7 +874,7 @@ int inf_linear_ckpt_backward(int64_t rows, int n, int k, const float* dy, int64_
                              int64_t ld_dx, float* dW, int64_t ld_dw, float* db, void* workspace,
                              inf_stream_t stream) {
   INF_CHECK_ARG(rows >= 0 && n >= 1 && k >= 1 && ld_dy >= 0, "linear_ckpt backward: bad shape");
-  INF_CHECK_ARG(rows < (int64_t)1 << 31, "linear_ckpt backward: too many rows");
+  INF_CHECK_ARG(rows < (int64_t)1 << 31 && fits(n, k, ld_dy) && fits(n, k, ld_y), "linear_ckpt backward: too large");
   INF_CHECK_ARG(act >= 0 && act <= 2, "linear_ckpt backward: act must be 0 (none), 1 (ReLU) or 2 (sigmoid)");
   INF_CHECK_ARG(dx == nullptr || (W != nullptr && ld_dx >= k && (dx_dtype == INF_DTYPE_F32 || dx_dtype == INF_DTYPE_BF16)),
                 "linear_ckpt backward: dx needs the weight and is fp32 or bf16");

@@ -315,8 +315,8 @@ template <typename T>
 int launch_tiles(const Linear8Args& a, hipStream_t stream) {
   const int64_t wide = ceil_div(a.rows, 256);
   if (a.n <= 32) return launch_tile<T, 256, 32, 4, 1>(a, stream);
-  if (a.n <= 128 && wide >= 256) return launch_tile<T, 256, 128, 4, 2>(a, stream);
-  if (a.n > 128 && wide * ceil_div(a.n, 256) >= 256) return launch_tile<T, 256, 256, 2, 4>(a, stream);
+  if (a.n <= 128 && wide >= 256) return launch_tile<T, 256, 128, 8, 2>(a, stream);
+  if (a.n > 128 && wide * ceil_div(a.n, 256) >= 256) return launch_tile<T, 256, 256, 4, 4>(a, stream);
   if (sizeof(T) == 1 && a.n > 64) return launch_tile<T, 64, 256, 1, 4>(a, stream);
   return launch_tile<T, 64, 64, 2, 2>(a, stream);
 }

@@ -18,10 +18,26 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 __device__ __forceinline__ int swz(int row) { return (row >> 1) & 7; }
 __device__ __forceinline__ int chunk_at(int row, int c) { return row * 128 + ((c ^ swz(row)) << 4); }
 
-// the workgroup's barrier after all of this wave's loads (to registers and to LDS) and LDS
-// writes have arrived
-__device__ __forceinline__ void wait_all_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+// The workgroup's barrier once this wave's LDS writes, and its loads (to registers and to LDS)
+// but the last N that it issued, have arrived.  The wait is the builtin, not inline assembly:
+// the compiler then knows which registers are there, and does not wait for later loads to use
+// them (s_waitcnt vmcnt(N) expcnt(7) lgkmcnt(0)).
+template <int N>
+__device__ __forceinline__ void wait_barrier() {
+  static_assert(N < 16, "vmcnt's low field");
+  asm volatile("" ::: "memory");  // (a fence would wait for every load)
+  __builtin_amdgcn_s_waitcnt(0x0070 | N);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wait_all_barrier() { wait_barrier<0>(); }
+
+// The same where nothing but LDS writes is waited for: the loads are registers'.
+__device__ __forceinline__ void wait_lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // vmcnt(63) expcnt(7) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // Workgroups that one XCD receives (every eighth) take consecutive tiles, so that tiles which
