@@ -63,46 +63,73 @@ __device__ __forceinline__ void put_pieces(char* row, const float* w, int64_t sk
   *reinterpret_cast<f16x8*>(to + 64) = lo;
 }
 
+struct Weight {
+  const float* W;
+  int64_t sr, sk;
+  int rows, K;
+  char* out;
+  int* shift;
+};
+
+// Workgroups of 256 threads; scratch: 16 words of LDS.
 // sk is the short stride: a workgroup a row, its threads along k
-__global__ __launch_bounds__(256) void split_rows_kernel(const float* __restrict__ W, int64_t sr, int64_t sk, int rows,
-                                                         int K, char* __restrict__ out, int* __restrict__ shift) {
-  __shared__ unsigned top[4];
-  const int r = blockIdx.x, tid = threadIdx.x;
-  const float* const w = W + r * sr;
-  unsigned a = 0;
+__device__ __forceinline__ void split_row(int block, const Weight& a, unsigned* scratch) {
+  const int r = block, tid = threadIdx.x;
+  const float* const w = a.W + r * a.sr;
+  unsigned t = 0;
 #pragma unroll 4
-  for (int k = tid; k < K; k += 256) a = max(a, abs_bits(w[k * sk]));
-#pragma unroll
-  for (int h = 32; h > 0; h >>= 1) a = max(a, (unsigned)__shfl_xor((int)a, h));
-  if (tid % 64 == 0) top[tid / 64] = a;
+  for (int k = tid; k < a.K; k += 256) t = max(t, abs_bits(w[k * a.sk]));
+  t = row_max<64>(t);
+  if (tid % 64 == 0) scratch[tid / 64] = t;
   __syncthreads();
-  const int e = shift_of(__uint_as_float(max(max(top[0], top[1]), max(top[2], top[3]))));
-  if (tid == 0) shift[r] = e;
-  const int Kp = (K + 31) / 32 * 32;
-  for (int c = tid; c < Kp / 8; c += 256) put_pieces(out + (int64_t)r * Kp * 4, w, sk, c, K, e);
+  const int e = shift_of(__uint_as_float(max(max(scratch[0], scratch[1]), max(scratch[2], scratch[3]))));
+  if (tid == 0) a.shift[r] = e;
+  const int Kp = (a.K + 31) / 32 * 32;
+  for (int c = tid; c < Kp / 8; c += 256) put_pieces(a.out + (int64_t)r * Kp * 4, w, a.sk, c, a.K, e);
 }
 
-// sr is the short stride: a workgroup 16 rows, 16 threads along them and 64 along k
-__global__ __launch_bounds__(1024) void split_columns_kernel(const float* __restrict__ W, int64_t sr, int64_t sk,
-                                                             int rows, int K, char* __restrict__ out,
-                                                             int* __restrict__ shift) {
-  __shared__ unsigned top[16];
-  const int l = threadIdx.x % 16, g = threadIdx.x / 16, r = blockIdx.x * 16 + l;
-  const float* const w = W + min(r, rows - 1) * sr;
-  if (threadIdx.x < 16) top[threadIdx.x] = 0;
+// sr is the short stride: a workgroup 16 rows, 16 threads along them and 16 along k
+__device__ __forceinline__ void split_columns(int block, const Weight& a, unsigned* scratch) {
+  const int l = threadIdx.x % 16, g = threadIdx.x / 16, r = block * 16 + l;
+  const float* const w = a.W + min(r, a.rows - 1) * a.sr;
+  if (threadIdx.x < 16) scratch[threadIdx.x] = 0;
   __syncthreads();
-  unsigned a = 0;
-#pragma unroll 4
-  for (int k = g; k < K; k += 64) a = max(a, abs_bits(w[k * sk]));
-  a = max(a, (unsigned)__shfl_xor((int)a, 16));
-  a = max(a, (unsigned)__shfl_xor((int)a, 32));
-  if (threadIdx.x % 64 < 16) atomicMax(&top[l], a);  // a maximum: in any order the same
+  unsigned t = 0;
+#pragma unroll 8
+  for (int k = g; k < a.K; k += 16) t = max(t, abs_bits(w[k * a.sk]));
+  t = max(t, (unsigned)__shfl_xor((int)t, 16));
+  t = max(t, (unsigned)__shfl_xor((int)t, 32));
+  if (threadIdx.x % 64 < 16) atomicMax(&scratch[l], t);  // a maximum: in any order the same
   __syncthreads();
-  if (r >= rows) return;
-  const int e = shift_of(__uint_as_float(top[l]));
-  if (g == 0) shift[r] = e;
-  const int Kp = (K + 31) / 32 * 32;
-  for (int c = g; c < Kp / 8; c += 64) put_pieces(out + (int64_t)r * Kp * 4, w, sk, c, K, e);
+  if (r >= a.rows) return;
+  const int e = shift_of(__uint_as_float(scratch[l]));
+  if (g == 0) a.shift[r] = e;
+  const int Kp = (a.K + 31) / 32 * 32;
+  for (int c = g; c < Kp / 8; c += 16) put_pieces(a.out + (int64_t)r * Kp * 4, w, a.sk, c, a.K, e);
+}
+
+bool along_k(const Weight& w) { return std::abs(w.sk) <= std::abs(w.sr); }
+int split_blocks(const Weight& w) { return along_k(w) ? w.rows : (int)ceil_div(w.rows, 16); }
+
+// One launch before the forward product: the weight's pieces, and the rows of x in 8 bits.
+template <typename T, int LPR, int CH, int R, bool ALONG_K>
+__global__ __launch_bounds__(256) void before_forward_kernel(Weight w, int nw, const T* __restrict__ x, int64_t rows,
+                                                             int k, int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
+                                                             float* __restrict__ scale) {
+  __shared__ unsigned scratch[16];
+  if ((int)blockIdx.x < nw) {
+    if constexpr (ALONG_K) split_row(blockIdx.x, w, scratch);
+    else split_columns(blockIdx.x, w, scratch);
+  } else {
+    quantize_rows_block<T, LPR, CH, R>((int64_t)blockIdx.x - nw, x, rows, k, ldx, q, ldq, scale);
+  }
+}
+
+template <bool ALONG_K>
+__global__ __launch_bounds__(256) void split_kernel(Weight w) {
+  __shared__ unsigned scratch[16];
+  if constexpr (ALONG_K) split_row(blockIdx.x, w, scratch);
+  else split_columns(blockIdx.x, w, scratch);
 }
 
 // ---- dz -------------------------------------------------------------------------------
@@ -126,15 +153,40 @@ __device__ __forceinline__ float dz_at(const Dz& d, int64_t m, int c) {
   return g;
 }
 
-// each row's shift; LPR lanes a row
-template <int ACT, int LPR>
-__global__ __launch_bounds__(256) void dz_shift_kernel(Dz d, int64_t rows, int n, int* __restrict__ shift) {
-  const int64_t m = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+// One launch before the backward products: the pieces of the weight's columns, and each row's
+// shift of dz, LPR lanes a row, four values a turn.
+template <int ACT, int LPR, bool ALONG_K>
+__global__ __launch_bounds__(256) void before_dx_kernel(Weight w, int nw, Dz d, int64_t rows, int n,
+                                                        int* __restrict__ shift) {
+  __shared__ unsigned scratch[16];
+  if ((int)blockIdx.x < nw) {
+    if constexpr (ALONG_K) split_row(blockIdx.x, w, scratch);
+    else split_columns(blockIdx.x, w, scratch);
+    return;
+  }
+  const int64_t m = ((int64_t)blockIdx.x - nw) * (256 / LPR) + threadIdx.x / LPR;
   if (m >= rows) return;
   unsigned a = 0;
-  for (int c = threadIdx.x % LPR; c < n; c += LPR) a = max(a, abs_bits(dz_at<ACT>(d, m, c)));
+#pragma unroll 2
+  for (int c = threadIdx.x % LPR * 4; c < n; c += LPR * 4) {
+    if (c + 4 <= n) {
+      const f32x4u g = *reinterpret_cast<const f32x4u*>(d.dy + m * d.lddy + c);
+      f32x4u y = {};
+      uint32_t bits = 0;
+      if (ACT == DZ_SIGMOID) y = *reinterpret_cast<const f32x4u*>(d.y + m * d.ldy + c);
+      if (ACT == DZ_RELU) bits = d.mask[m * d.words + c / 32] >> (c % 32);
 #pragma unroll
-  for (int h = LPR / 2; h > 0; h >>= 1) a = max(a, (unsigned)__shfl_xor((int)a, h));
+      for (int e = 0; e < 4; ++e) {
+        float v = g[e];
+        if (ACT == DZ_SIGMOID) v *= y[e] * (1.f - y[e]);
+        if (ACT == DZ_RELU) v = (bits >> e) & 1 ? v : 0.f;
+        a = max(a, abs_bits(v));
+      }
+    } else {
+      for (int e = c; e < n; ++e) a = max(a, abs_bits(dz_at<ACT>(d, m, e)));
+    }
+  }
+  a = row_max<LPR>(a);
   if (threadIdx.x % LPR == 0) shift[m] = shift_of(__uint_as_float(a));
 }
 
@@ -415,6 +467,7 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
       }
     }
     if (!direct) {
+      own_lds_order();
       constexpr int AT_ONCE = 64 / P::WCOLS;  // rows of a store
       const int c = lane % P::WCOLS, n = n0 + wc * P::WCOLS + c;
 #pragma unroll
@@ -424,6 +477,7 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
         const float v = *reinterpret_cast<const float*>(mine + row * RS + c * 4);
         if (mr < a.rows && n < a.cols) reinterpret_cast<T*>(a.out)[mr * a.ldo + n] = from_f32<T>(v);
       }
+      own_lds_order();
     }
   }
 }
@@ -620,21 +674,29 @@ __global__ __launch_bounds__(DW_THREADS) void dw_tile_kernel(DwArgs a) {
   }
 }
 
-// dW and db from the splits' sums, in order
+// dW and db from the splits' sums: 32 outputs a workgroup, eight threads each an eighth of the
+// splits in order, then the eight in order.
 __global__ __launch_bounds__(256) void add_slabs_kernel(const float* __restrict__ slabs, int64_t count, int k,
                                                         int splits, float* __restrict__ dW, int64_t lddw,
                                                         const float* __restrict__ dbs, int n, float* __restrict__ db) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < count) {
-    float v = 0.f;
+  __shared__ float part[8][32];
+  const int l = threadIdx.x % 32, g = threadIdx.x / 32;
+  const int64_t i = (int64_t)blockIdx.x * 32 + l;
+  const bool is_w = i < count, is_b = !is_w && i - count < n && db != nullptr;
+  const int s0 = splits * g / 8, s1 = splits * (g + 1) / 8;
+  float v = 0.f;
+  if (is_w)
 #pragma unroll 8
-    for (int s = 0; s < splits; ++s) v += slabs[s * count + i];
-    dW[i / k * lddw + i % k] = v;
-  } else if (i - count < n && db != nullptr) {
-    float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += dbs[(int64_t)s * n + (i - count)];
-    db[i - count] = v;
-  }
+    for (int s = s0; s < s1; ++s) v += slabs[s * count + i];
+  if (is_b)
+    for (int s = s0; s < s1; ++s) v += dbs[(int64_t)s * n + (i - count)];
+  part[g][l] = v;
+  __syncthreads();
+  if (g != 0 || !(is_w || is_b)) return;
+#pragma unroll
+  for (int h = 1; h < 8; ++h) v += part[h][l];
+  if (is_w) dW[i / k * lddw + i % k] = v;
+  else db[i - count] = v;
 }
 
 // db alone (no weight gradient asked for)
@@ -683,19 +745,44 @@ int launch_tiles(const SideArgs& a, hipStream_t stream) {
   return launch_tile<MODE, ACT, X, T, 64, 64, 2, 2>(a, stream);
 }
 
-int launch_split(const float* W, int64_t sr, int64_t sk, int rows, int K, char* out, int* shift, hipStream_t stream) {
-  if (std::abs(sk) <= std::abs(sr))
-    split_rows_kernel<<<(unsigned)rows, 256, 0, stream>>>(W, sr, sk, rows, K, out, shift);
-  else
-    split_columns_kernel<<<(unsigned)ceil_div(rows, 16), 1024, 0, stream>>>(W, sr, sk, rows, K, out, shift);
+int launch_split(const Weight& w, hipStream_t stream) {
+  const auto kernel = along_k(w) ? split_kernel<true> : split_kernel<false>;
+  kernel<<<(unsigned)split_blocks(w), 256, 0, stream>>>(w);
   INF_LAUNCH_CHECK();
   return INF_OK;
 }
 
+template <typename T>
+int launch_before_forward(const Weight& w, const T* x, int64_t rows, int k, int64_t ldx, int8_t* q, int64_t ldq,
+                          float* scale, hipStream_t stream) {
+  const int nw = split_blocks(w);
+  const bool held = with_row_layout<T>(rows, k, [&](auto lpr, auto ch, auto r) {
+    constexpr int LPR = decltype(lpr)::value, CH = decltype(ch)::value, R = decltype(r)::value;
+    const auto kernel = along_k(w) ? before_forward_kernel<T, LPR, CH, R, true>
+                                   : before_forward_kernel<T, LPR, CH, R, false>;
+    kernel<<<(unsigned)(nw + ceil_div(rows, R * 256 / LPR)), 256, 0, stream>>>(w, nw, x, rows, k, ldx, q, ldq, scale);
+  });
+  if (!held) {
+    const int rc = launch_quantize_rows(x, sizeof(T) == 4 ? INF_DTYPE_F32 : INF_DTYPE_BF16, rows, k, ldx, q, ldq, scale,
+                                        stream);
+    return rc != INF_OK ? rc : launch_split(w, stream);
+  }
+  INF_LAUNCH_CHECK();
+  return INF_OK;
+}
+
+template <int ACT, int LPR>
+void launch_before_dx_as(const Weight& w, const Dz& d, int64_t rows, int n, int* shift, hipStream_t stream) {
+  const int nw = split_blocks(w);
+  const auto kernel = along_k(w) ? before_dx_kernel<ACT, LPR, true> : before_dx_kernel<ACT, LPR, false>;
+  kernel<<<(unsigned)(nw + ceil_div(rows, 256 / LPR)), 256, 0, stream>>>(w, nw, d, rows, n, shift);
+}
+
 template <int ACT>
-int launch_dz_shift(const Dz& d, int64_t rows, int n, int* shift, hipStream_t stream) {
-  if (n <= 16) dz_shift_kernel<ACT, 4><<<(unsigned)ceil_div(rows, 64), 256, 0, stream>>>(d, rows, n, shift);
-  else dz_shift_kernel<ACT, 64><<<(unsigned)ceil_div(rows, 4), 256, 0, stream>>>(d, rows, n, shift);
+int launch_before_dx(const Weight& w, const Dz& d, int64_t rows, int n, int* shift, hipStream_t stream) {
+  if (n <= 16) launch_before_dx_as<ACT, 4>(w, d, rows, n, shift, stream);
+  else if (n <= 64) launch_before_dx_as<ACT, 16>(w, d, rows, n, shift, stream);
+  else launch_before_dx_as<ACT, 64>(w, d, rows, n, shift, stream);
   INF_LAUNCH_CHECK();
   return INF_OK;
 }
@@ -767,9 +854,8 @@ int backward(int64_t rows, int n, int k, const Dz& dz, const int8_t* q, int64_t 
   const BackwardSpace o = backward_space(rows, n, k);
   int rc;
   if (dx != nullptr && rows > 0) {
-    rc = launch_dz_shift<ACT>(dz, rows, n, (int*)(ws + o.shift), st);
-    if (rc != INF_OK) return rc;
-    rc = launch_split(W, swk, swn, k, n, ws + o.V, (int*)(ws + o.vshift), st);
+    const Weight w{W, swk, swn, k, n, ws + o.V, (int*)(ws + o.vshift)};
+    rc = launch_before_dx<ACT>(w, dz, rows, n, (int*)(ws + o.shift), st);
     if (rc != INF_OK) return rc;
     SideArgs a{};
     a.rows = rows;
@@ -797,7 +883,7 @@ int backward(int64_t rows, int n, int k, const Dz& dz, const int8_t* q, int64_t 
     if (rc != INF_OK) return rc;
     if (d.splits > 1) {
       const int64_t count = (int64_t)n * k;
-      add_slabs_kernel<<<(unsigned)ceil_div(count + n, 256), 256, 0, st>>>(a.out, count, k, d.splits, dW, lddw, a.db, n,
+      add_slabs_kernel<<<(unsigned)ceil_div(count + n, 32), 256, 0, st>>>(a.out, count, k, d.splits, dW, lddw, a.db, n,
                                                                            db);
       INF_LAUNCH_CHECK();
     }
@@ -837,19 +923,18 @@ int inf_linear_ckpt_forward(int64_t rows, int n, int k, const void* x, int x_dty
   const hipStream_t st = (hipStream_t)stream;
   char* const ws = (char*)workspace;
   const ForwardSpace o = forward_space(rows, n, k);
+  const Weight w{W, stride_wn, stride_wk, n, k, ws + o.V, (int*)(ws + o.vshift)};
   SideArgs a{};
   a.scale = scale;
   int rc;
-  if (q != nullptr) {
-    rc = launch_quantize_rows(x, x_dtype, rows, k, ld_x, q, ld_q, scale, st);
-  } else if (scale == nullptr) {
-    a.scale = (float*)(ws + o.scale);
-    rc = launch_quantize_rows(x, x_dtype, rows, k, ld_x, nullptr, 0, (float*)(ws + o.scale), st);
+  if (q == nullptr && scale != nullptr) {
+    rc = launch_split(w, st);
   } else {
-    rc = INF_OK;
+    if (scale == nullptr) a.scale = (float*)(ws + o.scale);
+    rc = x_dtype == INF_DTYPE_F32
+             ? launch_before_forward(w, (const float*)x, rows, k, ld_x, q, ld_q, (float*)a.scale, st)
+             : launch_before_forward(w, (const bf16*)x, rows, k, ld_x, q, ld_q, (float*)a.scale, st);
   }
-  if (rc != INF_OK) return rc;
-  rc = launch_split(W, stride_wn, stride_wk, n, k, ws + o.V, (int*)(ws + o.vshift), st);
   if (rc != INF_OK) return rc;
   a.rows = rows;
   a.cols = n;

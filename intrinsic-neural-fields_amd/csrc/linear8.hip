@@ -5,9 +5,10 @@
 // The roundings are written out one by one and never contracted: a row that goes into 8
 // bits again has the same numbers whichever kernel made it.
 //
-// Two kernels.  Up to 16 rows: linear8_few_kernel, one launch, bound by its latency and by
-// reading the weights once.  More: x goes into 8 bits in a launch of its own (rows8.hip: a
-// row's maximum is needed before its first product), then linear8_tile_kernel.
+// Three kernels.  Up to 16 rows: linear8_few_kernel, one launch, bound by its latency and by
+// reading the weights once.  Many rows and a weight that fits in LDS: linear8_rows_kernel, one
+// launch.  Otherwise x goes into 8 bits in a launch of its own (rows8.hip: a row's maximum is
+// needed before its first product), then linear8_tile_kernel.
 #include <algorithm>
 
 #include "mtile.hpp"
@@ -36,12 +37,13 @@ struct Linear8Args {
   float* os;  // scales of an int8 result
 };
 
-__device__ __forceinline__ float combine(int acc, float sx, float sw, float bias, float add, int act) {
+__device__ __forceinline__ float combine(int acc, float sx, float sw, float bias) {
 #pragma clang fp contract(off)
-  float z = (float)acc * (sx * sw);
-  z = z + bias;
-  z = z + add;
-  return activate(z, act);
+  const float z = (float)acc * (sx * sw);
+  return z + bias;
+}
+__device__ __forceinline__ float combine(int acc, float sx, float sw, float bias, float add, int act) {
+  return activate(combine(acc, sx, sw, bias) + add, act);
 }
 
 // four neighbouring results of a row, as they are stored
@@ -263,7 +265,7 @@ __global__ __launch_bounds__(256) void linear8_few_kernel(Linear8Args a, const X
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = c + e < a.k ? to_f32(x[m * ldx + c + e]) : 0.f;
-        *reinterpret_cast<uint32_t*>(smem + m * ld + c) = quantize4(v[0], v[1], v[2], v[3], rs);
+        *reinterpret_cast<uint32_t*>(smem + m * ld + c) = quantize4<X>(v[0], v[1], v[2], v[3], rs);
       }
     }
   }
@@ -292,6 +294,246 @@ __global__ __launch_bounds__(256) void linear8_few_kernel(Linear8Args a, const X
                             a.add != nullptr ? a.add[r * a.ldadd + n] : 0.f, a.act);
     reinterpret_cast<T*>(a.out)[r * a.ldo + n] = from_f32<T>(y);
   }
+}
+
+// ---- many rows, the weight in LDS -------------------------------------------------------
+// A workgroup (one a CU) holds the whole weight in LDS and walks over the rows; a wave owns 16 of
+// them at a time with all their outputs, so that nothing is exchanged between waves and no
+// barrier is left in the loop.  x goes from memory into the registers that the instruction reads
+// (v_mfma_i32_16x16x64_i8), the next rows' while these are worked on; fp32 and bf16 rows are put
+// into 8 bits there, and so are the results, whose row maximum is two exchanges between lanes.
+// Bound by the rounding and scaling of the results, about twelve operations each, and by bytes.
+//   k runs over KS blocks of 64.  Within a block, byte p of lane group g's 16 is k = G (4 p / G +
+//   g) + p % G with G = 16 bytes of x (4 fp32, 8 bf16, 16 int8 values): each load of 16 bytes then
+//   lies next to the neighbouring lane groups'.  The weight is laid out the same way on its way to
+//   LDS.  Behind k its bytes are zero.
+template <typename X> constexpr int granule() { return 16 / sizeof(X); }
+constexpr int WALK_WAVES = 8;  // (16 have 128 registers each, and spill)
+
+template <typename X, typename T, int KS, int TJ>
+struct LR {
+  static constexpr int NW = WALK_WAVES;
+  static constexpr int THREADS = 64 * NW, WS = KS * 64 + 16;  // (16 bytes: rows start in other banks)
+  static constexpr int OS = TJ * 16 + 16;                     // a result row in 8 bits
+  static constexpr int WEIGHT = TJ * 16 * WS, SCALES = TJ * 16 * 8, OUT = sizeof(T) == 1 ? NW * 16 * OS : 0;
+  static constexpr int LDS = WEIGHT + SCALES + OUT;
+  static_assert(LDS <= 160 * 1024, "LDS");
+};
+
+__device__ __forceinline__ float positive_nan(float v) { return v != v ? __uint_as_float(0x7fc00000u) : v; }
+
+template <typename X, typename T, int KS, int TJ>
+__global__ __launch_bounds__(64 * WALK_WAVES) void linear8_rows_kernel(Linear8Args a, const X* __restrict__ x,
+                                                                                 int64_t ldx) {
+  using P = LR<X, T, KS, TJ>;
+  constexpr int G = granule<X>(), L = 16 / G;  // values of a load, loads of a block
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float* const sws = reinterpret_cast<float*>(smem + P::WEIGHT);  // scales, then biases
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g4 = lane >> 4;
+
+  // the weight: 64 bytes of a row a thread and turn; dword d of them is k = 4 d on
+  for (int i = tid; i < TJ * 16 * KS; i += P::THREADS) {
+    const int n = i / KS, b = i % KS;
+    i32x4 v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      v[c] = b * 64 < a.ldw ? *reinterpret_cast<const i32x4*>(a.w + min(n, a.n - 1) * a.ldw + b * 64 + c * 16)
+                            : i32x4{0, 0, 0, 0};
+    int* const to = reinterpret_cast<int*>(smem + n * P::WS + b * 64);
+#pragma unroll
+    for (int d = 0; d < 16; ++d) {
+      const int g = d * 4 / G % 4, load = d * 4 / G / 4, at = d * 4 % G;  // whose, in which load, where
+      to[g * 4 + (load * G + at) / 4] = v[d / 4][d % 4];
+    }
+  }
+  for (int i = tid; i < TJ * 16; i += P::THREADS) {
+    sws[i] = i < a.n ? positive_nan(a.ws[i]) : 0.f;  // columns behind the last are zero
+    sws[TJ * 16 + i] = i < a.n && a.bias != nullptr ? positive_nan(a.bias[i]) : 0.f;
+  }
+  __syncthreads();
+
+  const int tiles = (int)((a.rows + 15) / 16), step = (int)gridDim.x * P::NW;
+  typedef X XV __attribute__((ext_vector_type(G), aligned(sizeof(X))));
+  XV raw[KS][L];
+  const bool whole = a.k == KS * 64;
+  auto fetch = [&](int tile) {
+    const X* const row = x + min((int64_t)tile * 16 + r16, a.rows - 1) * ldx + g4 * G;
+    if (whole) {
+#pragma unroll
+      for (int b = 0; b < KS; ++b)
+#pragma unroll
+        for (int i = 0; i < L; ++i) raw[b][i] = *reinterpret_cast<const XV*>(row + b * 64 + i * 4 * G);
+    } else {
+#pragma unroll
+      for (int b = 0; b < KS; ++b)
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+          const int k = b * 64 + i * 4 * G, left = a.k - g4 * G - k;  // of these, values in the row
+          if constexpr (sizeof(X) == 1) {
+            raw[b][i] = *reinterpret_cast<const XV*>(row + (left > 0 ? k : -g4 * G));  // zero weights behind k
+          } else if (left >= G) {
+            raw[b][i] = *reinterpret_cast<const XV*>(row + k);
+          } else {
+#pragma unroll
+            for (int e = 0; e < G; ++e) raw[b][i][e] = e < left ? row[k + e] : (X)0.f;
+          }
+        }
+    }
+  };
+  const bool relu = a.act == 1;
+  int tile = (int)blockIdx.x * P::NW + wave;
+  if (tile < tiles) fetch(tile);
+  for (; tile < tiles; tile += step) {
+    const int64_t m = (int64_t)tile * 16 + r16;
+    i32x4 xf[KS];
+    float sx;
+    if constexpr (sizeof(X) == 1) {
+#pragma unroll
+      for (int b = 0; b < KS; ++b) xf[b] = __builtin_bit_cast(i32x4, raw[b][0]);
+      sx = positive_nan(a.qs[min(m, a.rows - 1)]);
+    } else {
+      unsigned top = 0;
+      if constexpr (sizeof(X) == 2) {  // two values at a time: bf16 is the upper half of its fp32
+        u16x2 two = {0, 0};
+#pragma unroll
+        for (int b = 0; b < KS; ++b)
+#pragma unroll
+          for (int i = 0; i < L; ++i) {
+            const u32x4 v = __builtin_bit_cast(u32x4, raw[b][i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              two = __builtin_elementwise_max(two, __builtin_bit_cast(u16x2, v[e] & 0x7fff7fffu));
+          }
+        top = (unsigned)max(two[0], two[1]) << 16;
+      } else {
+#pragma unroll
+        for (int b = 0; b < KS; ++b)
+#pragma unroll
+          for (int i = 0; i < L; ++i)
+#pragma unroll
+            for (int e = 0; e < G; ++e) top = max(top, abs_bits((float)raw[b][i][e]));
+      }
+      top = max(top, (unsigned)__shfl_xor((int)top, 16));
+      top = max(top, (unsigned)__shfl_xor((int)top, 32));
+      const RowScale rs = row_scale(top);
+      sx = rs.s;
+#pragma unroll
+      for (int b = 0; b < KS; ++b)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const int i = d * 4 / G, e = d * 4 % G;
+          xf[b][d] = (int)quantize4<X>((float)raw[b][i][e], (float)raw[b][i][e + 1], (float)raw[b][i][e + 2],
+                                    (float)raw[b][i][e + 3], rs);
+        }
+    }
+    if (tile + step < tiles) fetch(tile + step);
+    i32x4 acc[TJ];
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) acc[j] = i32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int b = 0; b < KS; ++b)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) {
+        if (j % 8 == 0) __builtin_amdgcn_sched_barrier(0);
+        acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+            *reinterpret_cast<const i32x4*>(smem + (16 * j + r16) * P::WS + b * 64 + g4 * 16), xf[b], acc[j], 0, 0, 0);
+      }
+    // lane: row m, columns 16 j + 4 g4 + (0..3); one j at a time (taken together they need more
+    // registers than there are)
+    unsigned top = 0;
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+      __builtin_amdgcn_sched_barrier(0);
+      const int n = 16 * j + 4 * g4;
+      const f32x4 sw = *reinterpret_cast<const f32x4*>(sws + n), bias = *reinterpret_cast<const f32x4*>(sws + TJ * 16 + n);
+      float z[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        z[e] = combine(acc[j][e], sx, sw[e], bias[e]);
+        // as whole numbers, negative values lie below zero and a NaN (of positive sign: every one here
+        // is) above: one operation
+        if (relu) z[e] = __int_as_float(max(__float_as_int(z[e]), 0));
+      }
+      if constexpr (sizeof(T) == 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          top = max(top, abs_bits(z[e]));
+          acc[j][e] = __float_as_int(z[e]);
+        }
+      } else if (m < a.rows) {
+        T* const to = reinterpret_cast<T*>(a.out) + m * a.ldo + n;
+        if (n + 4 <= a.n) {
+          typename Four<T>::V v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = from_f32<T>(z[e]);
+          *reinterpret_cast<typename Four<T>::V*>(to) = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < a.n) to[e] = from_f32<T>(z[e]);
+        }
+      }
+    }
+    if constexpr (sizeof(T) == 1) {
+      top = max(top, (unsigned)__shfl_xor((int)top, 16));
+      top = max(top, (unsigned)__shfl_xor((int)top, 32));
+      const RowScale rs = row_scale(top);
+      if (g4 == 0 && m < a.rows) a.os[m] = rs.s;
+      char* const mine = smem + P::WEIGHT + P::SCALES + wave * 16 * P::OS;
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+        *reinterpret_cast<uint32_t*>(mine + r16 * P::OS + 16 * j + 4 * g4) =
+            quantize4(__int_as_float(acc[j][0]), __int_as_float(acc[j][1]), __int_as_float(acc[j][2]),
+                      __int_as_float(acc[j][3]), rs);
+      }
+      own_lds_order();
+#pragma unroll
+      for (int i = 0; i < TJ / 4; ++i) {  // 16 rows of TJ chunks of 16 bytes, 64 a turn
+        const int r = (i * 64 + lane) / TJ, c = (i * 64 + lane) % TJ;
+        if ((int64_t)tile * 16 + r < a.rows && c * 16 < a.n)
+          *reinterpret_cast<u32x4*>((int8_t*)a.out + ((int64_t)tile * 16 + r) * a.ldo + c * 16) =
+              *reinterpret_cast<const u32x4*>(mine + r * P::OS + c * 16);
+      }
+      own_lds_order();
+    }
+  }
+}
+
+template <typename X, typename T, int KS, int TJ>
+int launch_rows(const Linear8Args& a, const X* x, int64_t ldx, hipStream_t stream) {
+  using P = LR<X, T, KS, TJ>;
+  const auto kernel = linear8_rows_kernel<X, T, KS, TJ>;
+  static const hipError_t attr =
+      hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
+  INF_HIP_TRY(attr);
+  const int64_t groups = ceil_div(a.rows, 16 * P::NW);
+  kernel<<<(unsigned)std::min<int64_t>(groups, 256), P::THREADS, P::LDS, stream>>>(a, x, ldx);
+  INF_LAUNCH_CHECK();
+  return INF_OK;
+}
+
+// k up to 256 with up to 256 outputs, and rows for a turn of every CU.  (Fewer outputs than 33 are
+// bound by x's bytes whichever kernel reads them; a sigmoid or a sum to add to is a head's or a skip
+// layer's, one a network.)
+bool rows_walk(const Linear8Args& a) {
+  return a.rows >= 16384 && a.k <= 256 && a.n > 32 && a.n <= 256 && a.act != 2 && a.add == nullptr;
+}
+
+template <typename X, typename T>
+int launch_rows_any(const Linear8Args& a, const void* x, int64_t ldx, hipStream_t stream) {
+  if (a.k <= 128)
+    return a.n <= 128 ? launch_rows<X, T, 2, 8>(a, (const X*)x, ldx, stream)
+                      : launch_rows<X, T, 2, 16>(a, (const X*)x, ldx, stream);
+  return a.n <= 128 ? launch_rows<X, T, 4, 8>(a, (const X*)x, ldx, stream)
+                    : launch_rows<X, T, 4, 16>(a, (const X*)x, ldx, stream);
+}
+
+template <typename X>
+int launch_rows_out(const Linear8Args& a, int out_dtype, const void* x, int64_t ldx, hipStream_t stream) {
+  if (out_dtype == INF_DTYPE_I8) return launch_rows_any<X, int8_t>(a, x, ldx, stream);
+  if (out_dtype == INF_DTYPE_BF16) return launch_rows_any<X, bf16>(a, x, ldx, stream);
+  return launch_rows_any<X, float>(a, x, ldx, stream);
 }
 
 template <typename T, int BM, int BN, int WM, int WN>
@@ -419,6 +661,10 @@ int inf_linear_int(int64_t rows, int n, int k, const void* x, int x_dtype, int64
     rc = x8 ? launch_few_out<int8_t>(a, product_dtype, x, ld_x, st)
             : x_dtype == INF_DTYPE_BF16 ? launch_few_out<bf16>(a, product_dtype, x, ld_x, st)
                                         : launch_few_out<float>(a, product_dtype, x, ld_x, st);
+  } else if (rows_walk(a)) {
+    rc = x8 ? launch_rows_out<int8_t>(a, product_dtype, x, ld_x, st)
+            : x_dtype == INF_DTYPE_BF16 ? launch_rows_out<bf16>(a, product_dtype, x, ld_x, st)
+                                        : launch_rows_out<float>(a, product_dtype, x, ld_x, st);
   } else {
     if (!x8) {
       a.q = (int8_t*)(wsp + o.q);

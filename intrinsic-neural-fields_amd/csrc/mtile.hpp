@@ -9,6 +9,7 @@ namespace mt {
 
 typedef __attribute__((address_space(3))) void lds_void;
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -39,6 +40,10 @@ __device__ __forceinline__ void wait_lds_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+
+// Between writes and reads of a piece of LDS that one wave alone uses: its LDS accesses are served
+// in order, the compiler has to leave them so.
+__device__ __forceinline__ void own_lds_order() { asm volatile("" ::: "memory"); }
 
 // Workgroups that one XCD receives (every eighth) take consecutive tiles, so that tiles which
 // share rows find them in that XCD's L2.

@@ -11,78 +11,11 @@ namespace {
 
 using namespace q8;
 
-// A row is held in the registers of LPR lanes (4, 16 or 64), CH chunks of 16 bytes of x a
-// lane, between its maximum and its rounding: x is read once, with 16-byte loads, and the
-// rows of a wave's other lanes keep more loads on their way.  Bound by bytes.
-// Loads and stores of a whole chunk need their element's alignment only (rows of odd
-// lengths: k = 1023).
-template <typename T> struct Chunk;
-template <> struct Chunk<float> {
-  static constexpr int V = 4;
-  typedef float X __attribute__((ext_vector_type(4), aligned(4)));
-};
-template <> struct Chunk<bf16> {
-  static constexpr int V = 8;
-  typedef bf16 X __attribute__((ext_vector_type(8), aligned(2)));
-};
-
-// columns [c, c + V) of a row; those from k on are zero
-template <typename T>
-__device__ __forceinline__ void load_chunk(const T* row, int c, int k, float (&v)[Chunk<T>::V]) {
-  constexpr int V = Chunk<T>::V;
-  if (c + V <= k) {
-    const typename Chunk<T>::X x = *reinterpret_cast<const typename Chunk<T>::X*>(row + c);
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = (float)x[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = c + e < k ? to_f32(row[c + e]) : 0.f;
-  }
-}
-
-template <int LPR>
-__device__ __forceinline__ unsigned row_max(unsigned a) {
-#pragma unroll
-  for (int h = LPR / 2; h > 0; h >>= 1) a = max(a, (unsigned)__shfl_xor((int)a, h));
-  return a;
-}
-
-template <typename T, int LPR, int CH>
+template <typename T, int LPR, int CH, int R>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int k, int64_t ldx,
                                                             int8_t* __restrict__ q, int64_t ldq,
                                                             float* __restrict__ scale) {
-  constexpr int V = Chunk<T>::V;
-  const int64_t m = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  const int l = threadIdx.x % LPR;
-  if (m >= rows) return;  // whole rows of lanes: the exchanges below stay within a row
-  float v[CH][V];
-  unsigned a = 0;
-#pragma unroll
-  for (int i = 0; i < CH; ++i) load_chunk(x + m * ldx, (i * LPR + l) * V, k, v[i]);
-#pragma unroll
-  for (int i = 0; i < CH; ++i)
-#pragma unroll
-    for (int e = 0; e < V; ++e) a = max(a, abs_bits(v[i][e]));
-  const RowScale rs = row_scale(row_max<LPR>(a));
-  if (l == 0) scale[m] = rs.s;
-  if (q == nullptr) return;  // the scales alone
-#pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    const int c = (i * LPR + l) * V;
-    if (c >= k) break;
-    uint32_t w[V / 4];
-#pragma unroll
-    for (int e = 0; e < V; e += 4) w[e / 4] = quantize4(v[i][e], v[i][e + 1], v[i][e + 2], v[i][e + 3], rs);
-    int8_t* const to = q + m * ldq + c;
-    if (c + V <= k) {
-#pragma unroll
-      for (int e = 0; e < V / 4; ++e) reinterpret_cast<uint32_t*>(to)[e] = w[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (c + e < k) to[e] = (int8_t)(w[e / 4] >> (8 * (e % 4)));
-    }
-  }
+  quantize_rows_block<T, LPR, CH, R>(blockIdx.x, x, rows, k, ldx, q, ldq, scale);
 }
 
 // Rows too long for a wave's registers: a workgroup a row, which is read twice.
@@ -111,7 +44,7 @@ __global__ __launch_bounds__(256) void quantize_long_rows_kernel(const T* __rest
       load_chunk(x + m * ldx, c, k, v);
 #pragma unroll
       for (int e = 0; e < V; ++e)
-        if (c + e < k) q[m * ldq + c + e] = (int8_t)quantize(v[e], rs);
+        if (c + e < k) q[m * ldq + c + e] = (int8_t)quantize<T>(v[e], rs);
     }
   }
 }
@@ -160,21 +93,11 @@ unsigned blocks_of(int64_t n) { return (unsigned)std::min<int64_t>(std::max<int6
 template <typename T>
 static void quantize_rows_any(const T* x, int64_t rows, int k, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
                               hipStream_t st) {
-  constexpr int V = Chunk<T>::V;
-  const int chunks = (int)ceil_div(k, V);
-  auto grid = [&](int lpr) { return (unsigned)ceil_div(rows, 256 / lpr); };
-#define INF_Q(LPR, CH) quantize_rows_kernel<T, LPR, CH><<<grid(LPR), 256, 0, st>>>(x, rows, k, ldx, q, ldq, scale)
-  // the fewest lanes that hold a row in one chunk each, then more chunks a lane; 64 values a
-  // lane is the most that still leaves several waves a SIMD
-  if (chunks <= 4) INF_Q(4, 1);
-  else if (chunks <= 16) INF_Q(16, 1);
-  else if (chunks <= 64) INF_Q(64, 1);
-  else if (chunks <= 128) INF_Q(64, 2);
-  else if (chunks <= 256) INF_Q(64, 4);
-  else if (chunks <= 512) INF_Q(64, 8);
-  else if (V == 4 && chunks <= 1024) INF_Q(64, V == 4 ? 16 : 8);
-  else quantize_long_rows_kernel<<<blocks_of(rows), 256, 0, st>>>(x, rows, k, ldx, q, ldq, scale);
-#undef INF_Q
+  const bool held = with_row_layout<T>(rows, k, [&](auto lpr, auto ch, auto r) {
+    constexpr int LPR = decltype(lpr)::value, CH = decltype(ch)::value, R = decltype(r)::value;
+    quantize_rows_kernel<T, LPR, CH, R><<<(unsigned)ceil_div(rows, R * 256 / LPR), 256, 0, st>>>(x, rows, k, ldx, q, ldq, scale);
+  });
+  if (!held) quantize_long_rows_kernel<<<blocks_of(rows), 256, 0, st>>>(x, rows, k, ldx, q, ldq, scale);
 }
 
 template <typename T>

@@ -122,12 +122,19 @@ def linear(segments, weights, biases, act=None, checkpoint=None):
 
 
 # ---- 8 bits -------------------------------------------------------------------------
+# (These calls are short: addresses go to the library as plain numbers, and each allocation
+# counts.)
+
+_ON_CURRENT = contextlib.nullcontext()
+
 
 def _on(device):
     """The device of the tensors as the current one, for launches on its current stream."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _ON_CURRENT if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _round_up(n, m):
@@ -155,12 +162,6 @@ class Rows8:
         self.q = torch.empty(rows * ld + 128, dtype=torch.int8, device=device).as_strided((rows, k), (ld, 1))
         self.scale = torch.empty(rows, dtype=torch.float32, device=device)
 
-    @classmethod
-    def _from(cls, q, scale):
-        r = cls.__new__(cls)
-        r.q, r.scale = q, scale
-        return r
-
     @property
     def shape(self):
         return self.q.shape
@@ -172,14 +173,14 @@ class Rows8:
     def restore(self, dtype=torch.float32):
         """scale * q, rounded once to fp32 / bf16."""
         rt = _rt()
-        from inf_hip import lib
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"8-bit rows are restored to fp32 or bf16, not {dtype}")
-        rows, k = self.q.shape
-        out = torch.empty((rows, k), dtype=dtype, device=self.q.device)
-        with _on(self.q.device):
-            rt.check(lib.inf_restore_rows(rt.ptr(self.q), self.q.stride(0), rt.ptr(self.scale), rows, k, rt.ptr(out),
-                                          rt.dtype_code(out), k, rt.stream_handle()), "restore_rows")
+        q = self.q
+        rows, k = q.shape
+        out = torch.empty((rows, k), dtype=dtype, device=q.device)
+        with _on(q.device):
+            rt.check(rt.lib.inf_restore_rows(q.data_ptr(), q.stride(0), self.scale.data_ptr(), rows, k, out.data_ptr(),
+                                             rt.dtype_code(out), k, rt.stream_handle()), "restore_rows")
         return out
 
 
@@ -188,14 +189,13 @@ def quantize_rows(x):
     nearest to 127 x / max|x| (ties to even).  Rows of zeros have scale 0; a row with an
     infinity or a NaN has scale NaN, and whatever is made of it is NaN.  No gradient."""
     rt = _rt()
-    from inf_hip import lib
     rt.require_hip(x)
     x = _rows_of(x.detach(), "x")
     rows, k = x.shape
     r = Rows8(rows, k, x.device)
     with _on(x.device):
-        rt.check(lib.inf_quantize_rows(rt.ptr(x), rt.dtype_code(x), rows, k, x.stride(0), rt.ptr(r.q), r.q.stride(0),
-                                       rt.ptr(r.scale), rt.stream_handle()), "quantize_rows")
+        rt.check(rt.lib.inf_quantize_rows(x.data_ptr(), rt.dtype_code(x), rows, k, x.stride(0), r.q.data_ptr(),
+                                          r.q.stride(0), r.scale.data_ptr(), rt.stream_handle()), "quantize_rows")
     return r
 
 
@@ -211,18 +211,17 @@ class Weight8:
 def pack_weight8(q, scale):
     """8-bit weights q int8 [n, k] (any strides) with scales fp32 [n], laid out for linear8."""
     rt = _rt()
-    from inf_hip import lib
     rt.require_hip(q, scale)
     if q.dim() != 2 or q.dtype != torch.int8 or min(q.shape) < 1:
         raise ValueError("an 8-bit weight is an int8 matrix [n, k]")
     n, k = q.shape
     if scale.shape != (n,) or scale.dtype != torch.float32 or scale.device != q.device:
         raise ValueError("an 8-bit weight has one fp32 scale a row, on its device")
-    packed = torch.empty(int(lib.inf_packed_weight_bytes(n, k)), dtype=torch.int8, device=q.device)
+    packed = torch.empty(int(rt.lib.inf_packed_weight_bytes(n, k)), dtype=torch.int8, device=q.device)
     with _on(q.device):
-        rt.check(lib.inf_pack_weight(rt.ptr(q), q.stride(0), q.stride(1), n, k, rt.ptr(packed), rt.stream_handle()),
-                 "pack_weight")
-    return Weight8(packed, scale.contiguous().clone(), n, k)
+        rt.check(rt.lib.inf_pack_weight(q.data_ptr(), q.stride(0), q.stride(1), n, k, packed.data_ptr(),
+                                        rt.stream_handle()), "pack_weight")
+    return Weight8(packed, scale.clone(), n, k)
 
 
 def quantize_weight(W, col0=0, cols=None):
@@ -243,26 +242,27 @@ def linear8(xs, weights, biases, act=None, out=torch.float32):
     out: torch.float32, torch.bfloat16, or torch.int8 for a Rows8 of the result.
     For rendering: it has no gradient, and refuses inputs that ask for one."""
     rt = _rt()
-    from inf_hip import DTYPE_I8, lib
-    code = {torch.float32: rt.DTYPE_F32, torch.bfloat16: rt.DTYPE_BF16, torch.int8: DTYPE_I8}.get(out)
+    i8 = rt.DTYPE_I8
+    code = i8 if out is torch.int8 else rt.DTYPE_F32 if out is torch.float32 else \
+        rt.DTYPE_BF16 if out is torch.bfloat16 else None
     if code is None:
         raise ValueError(f"linear8 gives fp32, bf16 or int8 rows, not {out}")
     if len(xs) < 1 or len(xs) != len(weights) or len(biases) > len(xs):
         raise ValueError("linear8 takes one weight and at most one bias for each segment")
     rows, n, device = xs[0].shape[0], weights[0].n, xs[0].device
-    grad = torch.is_grad_enabled()
-    acc, last = None, len(xs) - 1
-    with _on(device) if device.type == "cuda" else contextlib.nullcontext():
+    acc, last, lib, a = None, len(xs) - 1, rt.lib, ACT[act]
+    if device.type != "cuda":
+        rt.require_hip(xs[0].q if isinstance(xs[0], Rows8) else xs[0])
+    with _on(device):
         for s, (x, w) in enumerate(zip(xs, weights)):
             if isinstance(x, Rows8):
-                q, scale, xc = x.q, x.scale, DTYPE_I8
+                q, scale, xc = x.q, x.scale.data_ptr(), i8
             else:
-                rt.require_hip(x)
-                if grad and x.requires_grad:
+                if x.requires_grad and torch.is_grad_enabled():
                     raise RuntimeError("linear8 has no gradient: call it under torch.no_grad(), or train with linear")
                 q, scale = _rows_of(x, "x"), None
                 xc = rt.dtype_code(q)
-            if q.shape != (rows, w.k) or w.n != n:
+            if q.shape[0] != rows or q.shape[1] != w.k or w.n != n:
                 raise ValueError(f"segment {s}: x {list(q.shape)} and weight [{w.n}, {w.k}] do not fit [{rows}, {n}]")
             b = biases[s] if s < len(biases) else None
             if b is not None and (b.shape != (n,) or b.dtype != torch.float32 or not b.is_contiguous()):
@@ -270,17 +270,17 @@ def linear8(xs, weights, biases, act=None, out=torch.float32):
             if q.device != device or w.packed.device != device or (b is not None and b.device != device):
                 raise ValueError("linear8 takes its tensors on one device")
             oc = code if s == last else rt.DTYPE_F32
-            if oc == DTYPE_I8:
+            if oc == i8:
                 y = Rows8(rows, n, device)
-                op, ldo, osc = y.q, y.q.stride(0), y.scale
+                op, ldo, osc = y.q.data_ptr(), y.q.stride(0), y.scale.data_ptr()
             else:
                 y = torch.empty((rows, n), dtype=out if s == last else torch.float32, device=device)
-                op, ldo, osc = y, n, None
-            nws = int(lib.inf_linear_int_workspace_bytes(rows, n, w.k, xc, oc))
+                op, ldo, osc = y.data_ptr(), n, None
+            nws = lib.inf_linear_int_workspace_bytes(rows, n, w.k, xc, oc)
             ws = torch.empty(nws, dtype=torch.uint8, device=device) if nws else None
-            rt.check(lib.inf_linear_int(rows, n, w.k, rt.ptr(q), xc, q.stride(0), rt.ptr(scale), rt.ptr(w.packed),
-                                        rt.ptr(w.scale), rt.ptr(b), rt.ptr(acc), n, ACT[act] if s == last else 0,
-                                        rt.ptr(op), oc, ldo, rt.ptr(osc), rt.ptr(ws), rt.stream_handle()), "linear_int")
+            rt.check(lib.inf_linear_int(rows, n, w.k, q.data_ptr(), xc, q.stride(0), scale, w.packed.data_ptr(),
+                                        w.scale.data_ptr(), _at(b), _at(acc), n, a if s == last else 0, op, oc, ldo,
+                                        osc, _at(ws), rt.stream_handle()), "linear_int")
             acc = y
     return y
 
@@ -290,84 +290,111 @@ class _LinearCkpt(torch.autograd.Function):
     def forward(ctx, spec, act, kept, *tensors):
         # spec and tensors as _Linear; kept: per segment the Rows8 of x, or None to make them
         rt = _rt()
-        from inf_hip import lib
+        lib = rt.lib
         nseg = len(spec)
+        nb = len(tensors) - nseg
         nw = max(w for w, _ in spec) + 1
-        xs, ws, bs = tensors[:nseg], tensors[nseg:nseg + nw], tensors[nseg + nw:]
-        needs = ctx.needs_input_grad[3:]
-        rows, n, device = xs[0].shape[0], ws[0].shape[0], xs[0].device
-        save, y, mask = [], None, None
+        nb -= nw
+        needs = ctx.needs_input_grad
+        W0 = tensors[nseg]
+        rows, n, device = tensors[0].shape[0], W0.shape[0], W0.device
+        # one allocation for what is kept: each segment's q and scale, then the mask
+        at, places = 0, []
+        for s, (wi, _) in enumerate(spec):
+            make = needs[3 + nseg + wi] and kept[s] is None
+            places.append(at if make else None)
+            if make:
+                at += _round_up(rows * _round_up(tensors[s].shape[1], 16) + 128, 256) + _round_up(rows * 4, 256)
+        mask_at = at if act == 1 and any(needs) else None
+        if mask_at is not None:
+            at += rows * ((n + 31) // 32) * 4
         with _on(device):
             st = rt.stream_handle()
             y = torch.empty((rows, n), dtype=torch.float32, device=device)
-            if act == 1 and any(needs):
-                mask = torch.empty((rows, (n + 31) // 32), dtype=torch.int32, device=device)
+            yp = y.data_ptr()
+            held = torch.empty(at, dtype=torch.uint8, device=device) if at else None
+            base = held.data_ptr() if at else 0
             for s, (wi, c0) in enumerate(spec):
-                x, W = xs[s], ws[wi]
-                k, last = x.shape[1], s == nseg - 1
-                rows8 = kept[s]
-                make = needs[nseg + wi] and rows8 is None
-                if make:
-                    rows8 = Rows8(rows, k, device)
+                x, W = tensors[s], tensors[nseg + wi]
+                k, last, own = x.shape[1], s == nseg - 1, kept[s]
+                ldq = _round_up(k, 16)
+                q = scale = None
+                if places[s] is not None:
+                    q = base + places[s]
+                    scale = q + _round_up(rows * ldq + 128, 256)
+                elif own is not None:
+                    scale = own.scale.data_ptr()
                 xc = rt.dtype_code(x)
-                work = torch.empty(int(lib.inf_linear_ckpt_workspace_bytes(rows, n, k, xc, 0)), dtype=torch.uint8,
+                work = torch.empty(lib.inf_linear_ckpt_workspace_bytes(rows, n, k, xc, 0), dtype=torch.uint8,
                                    device=device)
-                b = bs[s] if s < len(bs) else None
                 rt.check(lib.inf_linear_ckpt_forward(
-                    rows, n, k, rt.ptr(x), xc, x.stride(0), W.data_ptr() + 4 * c0 * W.stride(1), W.stride(0),
-                    W.stride(1), rt.ptr(b), rt.ptr(y) if s else None, n, act if last else 0, rt.ptr(y), n,
-                    rt.ptr(mask) if last else None, rt.ptr(rows8.q) if make else None,
-                    rows8.q.stride(0) if make else 0, rt.ptr(rows8.scale) if rows8 is not None else None, rt.ptr(work), st),
-                    "linear_ckpt_forward")
-                save += [rows8.q, rows8.scale] if needs[nseg + wi] else [None, None]
-        ctx.spec, ctx.act, ctx.nw, ctx.nb = spec, act, nw, len(bs)
-        ctx.widths, ctx.dtypes = [x.shape[1] for x in xs], [x.dtype for x in xs]
-        ctx.rows, ctx.n = rows, n
-        ctx.save_for_backward(*save, *ws, mask, y if act == 2 else None)
+                    rows, n, k, x.data_ptr(), xc, x.stride(0), W.data_ptr() + 4 * c0 * W.stride(1), W.stride(0),
+                    W.stride(1), tensors[nseg + nw + s].data_ptr() if s < nb else None, yp if s else None, n,
+                    act if last else 0, yp, n, base + mask_at if last and mask_at is not None else None, q, ldq, scale,
+                    work.data_ptr(), st), "linear_ckpt_forward")
+        ctx.layer = (spec, act, nw, nb, rows, n, places, mask_at, [t.shape[1] for t in tensors[:nseg]],
+                     [t.dtype for t in tensors[:nseg]])
+        save = [held, y if act == 2 else None, *tensors[nseg:nseg + nw]]
+        for own in kept:
+            if own is not None:
+                save += [own.q, own.scale]
+        ctx.kept = [own is not None for own in kept]
+        ctx.save_for_backward(*save)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         rt = _rt()
-        from inf_hip import lib
-        spec, act, nw, nb = ctx.spec, ctx.act, ctx.nw, ctx.nb
-        nseg, rows, n = len(spec), ctx.rows, ctx.n
+        lib = rt.lib
+        spec, act, nw, nb, rows, n, places, mask_at, widths, dtypes = ctx.layer
+        nseg = len(spec)
         saved = ctx.saved_tensors
-        ws, mask, y = saved[2 * nseg:2 * nseg + nw], saved[-2], saved[-1]
-        needs = ctx.needs_input_grad[3:]
-        dy = dy.to(torch.float32)
+        held, y, ws = saved[0], saved[1], saved[2:2 + nw]
+        own = iter(saved[2 + nw:])
+        needs = ctx.needs_input_grad
+        if dy.dtype != torch.float32:
+            dy = dy.to(torch.float32)
         if dy.stride(1) != 1 or dy.stride(0) < n:
             dy = dy.contiguous()
         device = dy.device
-        dxs, dws, dbs = [None] * nseg, [None] * nw, [None] * nb
+        base = held.data_ptr() if held is not None else 0
+        grads = [None] * (3 + nseg + nw + nb)
         with _on(device):
             st = rt.stream_handle()
             for s, (wi, c0) in enumerate(spec):
-                q, scale, W, k = saved[2 * s], saved[2 * s + 1], ws[wi], ctx.widths[s]
-                dx = dwp = None
-                if needs[s]:
-                    dxs[s] = dx = torch.empty((rows, k), dtype=ctx.dtypes[s], device=device)
-                if needs[nseg + wi]:
-                    if dws[wi] is None:
-                        covered = sum(kk for (wj, _), kk in zip(spec, ctx.widths) if wj == wi) == W.shape[1]
-                        dws[wi] = (torch.empty if covered else torch.zeros)(W.shape, dtype=torch.float32,
-                                                                            device=device)
-                    dwp = dws[wi].data_ptr() + 4 * c0
-                if s < nb and needs[nseg + nw + s]:
-                    dbs[s] = torch.empty(n, dtype=torch.float32, device=device)
-                db = dbs[s] if s < nb else None
-                if dx is None and dwp is None and db is None:
+                W, k = ws[wi], widths[s]
+                ldq = _round_up(k, 16)
+                q = scale = None
+                if places[s] is not None:
+                    q = base + places[s]
+                    scale = q + _round_up(rows * ldq + 128, 256)
+                elif ctx.kept[s]:
+                    qt, st_ = next(own), next(own)
+                    q, scale, ldq = qt.data_ptr(), st_.data_ptr(), qt.stride(0)
+                dx = dw = db = None
+                if needs[3 + s]:
+                    grads[3 + s] = dx = torch.empty((rows, k), dtype=dtypes[s], device=device)
+                if needs[3 + nseg + wi]:
+                    g = grads[3 + nseg + wi]
+                    if g is None:
+                        covered = sum(kk for (wj, _), kk in zip(spec, widths) if wj == wi) == W.shape[1]
+                        g = grads[3 + nseg + wi] = (torch.empty if covered else torch.zeros)(
+                            W.shape, dtype=torch.float32, device=device)
+                    dw = g.data_ptr() + 4 * c0
+                if s < nb and needs[3 + nseg + nw + s]:
+                    grads[3 + nseg + nw + s] = db = torch.empty(n, dtype=torch.float32, device=device)
+                if dx is None and dw is None and db is None:
                     continue
                 xc = rt.dtype_code(dx) if dx is not None else rt.DTYPE_F32
-                work = torch.empty(int(lib.inf_linear_ckpt_workspace_bytes(rows, n, k, xc, 1)), dtype=torch.uint8,
+                work = torch.empty(lib.inf_linear_ckpt_workspace_bytes(rows, n, k, xc, 1), dtype=torch.uint8,
                                    device=device)
                 rt.check(lib.inf_linear_ckpt_backward(
-                    rows, n, k, rt.ptr(dy), dy.stride(0), act, rt.ptr(y), n, rt.ptr(mask), rt.ptr(q),
-                    q.stride(0) if q is not None else 0, rt.ptr(scale), W.data_ptr() + 4 * c0 * W.stride(1),
-                    W.stride(0), W.stride(1), rt.ptr(dx), xc, k, dwp, W.shape[1], rt.ptr(db), rt.ptr(work), st),
-                    "linear_ckpt_backward")
-        return (None, None, None, *dxs, *dws, *dbs)
+                    rows, n, k, dy.data_ptr(), dy.stride(0), act, _at(y), n,
+                    base + mask_at if mask_at is not None else None, q, ldq, scale,
+                    W.data_ptr() + 4 * c0 * W.stride(1), W.stride(0), W.stride(1), _at(dx), xc, k, dw, W.shape[1],
+                    _at(db), work.data_ptr(), st), "linear_ckpt_backward")
+        return tuple(grads)
 
 
 def _linear_ckpt(segments, spec, weights, biases, act, checkpoint):
@@ -378,31 +405,30 @@ def _linear_ckpt(segments, spec, weights, biases, act, checkpoint):
         raise ValueError("linear takes at least one segment and at most one bias for each")
     if max(w for w, _ in spec) + 1 != len(weights) or min(w for w, _ in spec) < 0:
         raise ValueError("every weight belongs to a segment")
-    xs = [x if x.dtype in (torch.float32, torch.bfloat16) else x.to(torch.float32) for x, _, _ in segments]
-    xs = [_rows_of(x, "x") for x in xs]
+    xs = [_rows_of(x if x.dtype in (torch.float32, torch.bfloat16) else x.to(torch.float32), "x")
+          for x, _, _ in segments]
     rows, device = xs[0].shape[0], xs[0].device
     n = weights[0].shape[0]
-    for t in (*xs, *weights, *biases):
-        if t.device != device:
-            raise ValueError("linear takes its tensors on one device")
     for W in weights:
         if W.dim() != 2 or W.dtype != torch.float32 or W.shape[0] != n or n < 1:
             raise ValueError("weights are fp32 matrices with the same number of rows")
     for b in biases:
         if b.shape != (n,) or b.dtype != torch.float32 or not b.is_contiguous():
             raise ValueError("a bias is a contiguous fp32 [n] tensor")
-    taken = {}
+    taken = []
     for (wi, c0), x, c in zip(spec, xs, kept):
         k = x.shape[1]
         if x.shape[0] != rows or c0 < 0 or c0 + k > weights[wi].shape[1]:
             raise ValueError(f"x {list(x.shape)} at column {c0} does not fit weight {list(weights[wi].shape)}")
-        if any(c0 < b and a < c0 + k for a, b in taken.setdefault(wi, [])):
+        if any(wi == w and c0 < b and a < c0 + k for w, a, b in taken):
             raise ValueError("segments of one weight take separate columns")
-        taken[wi].append((c0, c0 + k))
-        if isinstance(c, Rows8) and (c.shape != x.shape or c.device != device):
+        taken.append((wi, c0, c0 + k))
+        if c != "int8" and (c.shape != x.shape or c.device != device):
             raise ValueError(f"checkpoint {list(c.shape)} is not of x {list(x.shape)}")
-    return _LinearCkpt.apply(spec, act, tuple(c if isinstance(c, Rows8) else None for c in kept), *xs, *weights,
-                             *biases)
+    for t in (*xs, *weights, *biases):
+        if t.device != device:
+            raise ValueError("linear takes its tensors on one device")
+    return _LinearCkpt.apply(spec, act, tuple(None if isinstance(c, str) else c for c in kept), *xs, *weights, *biases)
 
 
 def view_angles(unit_dirs, face_idxs, face_normals):

@@ -100,6 +100,18 @@ def test_rows8_ties_extremes_and_empty_rows():
     assert (v[8] == 0).all() and torch.isnan(v[9:]).all() and torch.isfinite(v[:8]).all()
 
 
+def test_rows8_every_ratio_of_bf16():
+    """All 128 significands over all, three exponents apart: every exact half of two bf16 values."""
+    sig = (1 + torch.arange(128) / 128).to(torch.bfloat16)
+    for scale in (1.0, 2.0 ** -110, 2.0 ** 120):
+        rows = torch.stack([torch.cat([sig * 2.0 ** -e * scale for e in range(1, 9)] + [s[None] * scale])
+                            for s in sig.to(torch.bfloat16)]).to(torch.bfloat16)
+        rows[:, ::2] *= -1
+        x = rows.cuda()
+        check_rows(x, dense().quantize_rows(x))
+        check_rows(x.float(), dense().quantize_rows(x.float()))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_rows8_strides(dtype):
     """Column ranges at odd offsets, a row repeated with stride 0, columns, no rows."""
@@ -151,7 +163,8 @@ def weight8(n, k, seed):
 
 SIZES = [(1, 1, 1), (1, 3, 1024), (1, 256, 1024), (2, 17, 63), (5, 256, 1023), (15, 128, 64), (16, 100, 129),
          (17, 3, 256), (33, 130, 100), (64, 64, 4096), (65, 257, 300), (127, 96, 127), (128, 128, 128),
-         (300, 256, 256), (257, 511, 193), (1000, 3, 16), (520, 1030, 65), (1, 4096, 2048), (8, 4097, 33)]
+         (300, 256, 256), (257, 511, 193), (1000, 3, 16), (520, 1030, 65), (1, 4096, 2048), (8, 4097, 33),
+         (16390, 256, 256), (16400, 100, 77), (17001, 129, 200), (16384, 255, 3), (16385, 64, 128)]
 
 
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
@@ -173,7 +186,8 @@ def test_linear8(rows, n, k, dtype, out):
 
 
 @pytest.mark.parametrize("rows,n,k", [(1, 1, 5), (1, 256, 1024), (3, 255, 64), (130, 256, 256), (700, 128, 100),
-                                      (70, 64, 1023), (20, 3, 40), (65, 300, 30), (9, 1025, 17)])
+                                      (70, 64, 1023), (20, 3, 40), (65, 300, 30), (9, 1025, 17), (16390, 256, 255),
+                                      (16400, 100, 128), (16411, 37, 64)])
 def test_linear8_rows_out_are_the_rows_of_the_result(rows, n, k):
     """out=int8 is quantize_rows of the fp32 result, bit for bit, whichever kernel makes it."""
     d = dense()
@@ -192,14 +206,14 @@ def test_linear8_rows_out_are_the_rows_of_the_result(rows, n, k):
 def test_linear8_each_form_gives_the_same_numbers():
     """A row's result does not depend on how many rows come with it, nor on who quantised it."""
     d = dense()
-    for n, k in ((256, 1024), (100, 77), (3, 256)):
-        x = make(600, k, torch.float32, 2)
+    for n, k, rows in ((256, 1024, 600), (100, 77, 16500), (3, 256, 600), (256, 200, 20000)):
+        x = make(rows, k, torch.float32, 2)
         qw, sw = weight8(n, k, 1)
         w, b = d.pack_weight8(qw.cuda(), sw.cuda()), torch.randn(n).cuda()
         whole = d.linear8([x], [w], [b], "relu")
         r8 = d.quantize_rows(x)
         assert torch.equal(d.linear8([r8], [w], [b], "relu"), whole)
-        for m in (1, 2, 16, 17, 64, 65, 300):
+        for m in (1, 2, 16, 17, 64, 65, 300, 16390):
             assert torch.equal(d.linear8([x[:m]], [w], [b], "relu"), whole[:m])
 
 
