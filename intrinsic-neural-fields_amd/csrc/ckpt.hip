@@ -16,6 +16,7 @@
 // A value that is not finite makes NaN of the rows (and columns) that it enters.
 #include <algorithm>
 #include <cstdlib>
+#include <type_traits>
 
 #include "mtile.hpp"
 
@@ -45,9 +46,12 @@ __device__ __forceinline__ _Float16 piece_hi(float x) { return (_Float16)x; }
 __device__ __forceinline__ _Float16 piece_lo(float x, _Float16 hi) { return (_Float16)(x - (float)hi); }
 
 // ---- the weight's rows as fp16 pieces ---------------------------------------------------
-// Row r of the product's side: V(r, k) = W[r sr + k sk], k < K, as blocks of 32 k: 64 bytes hi,
-// 64 bytes lo, zero behind K.
-__device__ __forceinline__ void put_pieces(char* row, const float* w, int64_t sk, int c, int K, int e) {
+// Row r of the product's side: V(r, k) = W[r sr + k sk], k < K, as the images that the instruction
+// reads: for 16 rows and 32 k a KiB hi and a KiB lo, lane l's 16 bytes at 16 l (row l % 16, k = 8
+// (l / 16) on).  Zero behind K up to a multiple of 64; rows behind the last hold anything.
+__host__ __device__ __forceinline__ int blocks_of_32(int K) { return (K + 63) / 64 * 2; }
+
+__device__ __forceinline__ void put_pieces(char* image, int r, const float* w, int64_t sk, int c, int K, int e) {
   float v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = c * 8 + i < K ? w[(c * 8 + i) * sk] : 0.f;
@@ -58,9 +62,9 @@ __device__ __forceinline__ void put_pieces(char* row, const float* w, int64_t sk
     hi[i] = piece_hi(x);
     lo[i] = piece_lo(x, hi[i]);
   }
-  char* const to = row + c / 4 * 128 + c % 4 * 16;
+  char* const to = image + ((int64_t)(r / 16) * blocks_of_32(K) + c / 4) * 2048 + (c % 4 * 16 + r % 16) * 16;
   *reinterpret_cast<f16x8*>(to) = hi;
-  *reinterpret_cast<f16x8*>(to + 64) = lo;
+  *reinterpret_cast<f16x8*>(to + 1024) = lo;
 }
 
 struct Weight {
@@ -84,8 +88,7 @@ __device__ __forceinline__ void split_row(int block, const Weight& a, unsigned* 
   __syncthreads();
   const int e = shift_of(__uint_as_float(max(max(scratch[0], scratch[1]), max(scratch[2], scratch[3]))));
   if (tid == 0) a.shift[r] = e;
-  const int Kp = (a.K + 31) / 32 * 32;
-  for (int c = tid; c < Kp / 8; c += 256) put_pieces(a.out + (int64_t)r * Kp * 4, w, a.sk, c, a.K, e);
+  for (int c = tid; c < blocks_of_32(a.K) * 4; c += 256) put_pieces(a.out, r, w, a.sk, c, a.K, e);
 }
 
 // sr is the short stride: a workgroup 16 rows, 16 threads along them and 16 along k
@@ -104,8 +107,7 @@ __device__ __forceinline__ void split_columns(int block, const Weight& a, unsign
   if (r >= a.rows) return;
   const int e = shift_of(__uint_as_float(scratch[l]));
   if (g == 0) a.shift[r] = e;
-  const int Kp = (a.K + 31) / 32 * 32;
-  for (int c = g; c < Kp / 8; c += 16) put_pieces(a.out + (int64_t)r * Kp * 4, w, a.sk, c, a.K, e);
+  for (int c = g; c < blocks_of_32(a.K) * 4; c += 16) put_pieces(a.out, r, w, a.sk, c, a.K, e);
 }
 
 bool along_k(const Weight& w) { return std::abs(w.sk) <= std::abs(w.sr); }
@@ -215,13 +217,79 @@ struct SideArgs {
   uint32_t* mask;
 };
 
+// add, activation of a forward result's four columns
+__device__ __forceinline__ void finish_forward(const SideArgs& a, int64_t m, int n, f32x4& z) {
+  if (a.add != nullptr && m < a.rows) {
+    const float* const from = a.add + m * a.ldadd + n;
+    if (n + 4 <= a.cols) {
+      const f32x4u v = *reinterpret_cast<const f32x4u*>(from);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] += v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < a.cols) z[e] += from[e];
+    }
+  }
+  if (a.act == DZ_RELU) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = activate(z[e], DZ_RELU);
+  } else if (a.act == DZ_SIGMOID) {
+    // one copy of its code for the four: with 16 of these a thread, 64 took the 65,536 x 256 x 256
+    // product from 49 to 58 us, ReLU or not
+#pragma unroll 1
+    for (int e = 0; e < 4; ++e) z = f32x4{z[1], z[2], z[3], activate(z[0], DZ_SIGMOID)};
+  }
+}
+
+// 16 bits of a row's mask: this lane's four, joined with those of the other lane groups
+__device__ __forceinline__ uint32_t mask_bits(const f32x4& z, int n, int cols, int g4) {
+  uint32_t b = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) b |= (uint32_t)(z[e] > 0.f && n + e < cols) << (4 * g4 + e);
+  b |= (uint32_t)__shfl_xor((int)b, 16);
+  return b | (uint32_t)__shfl_xor((int)b, 32);
+}
+
+// Rows that all start on 16 bytes (`direct`) are stored from the registers.  Others (k = 1023) go
+// through the wave's own piece of LDS, so that a store is one run of a row: 16-byte stores across
+// lines took 224 us where these took 164 (65,536 x 1023 x 256, dx, in 256 x 256 tiles).
+template <typename T>
+__device__ __forceinline__ void store_four(const SideArgs& a, int64_t m, int n, const f32x4& z) {
+  if (m >= a.rows) return;
+  T* const to = reinterpret_cast<T*>(a.out) + m * a.ldo + n;
+  if (n + 4 <= a.cols) {
+    typedef T V4 __attribute__((ext_vector_type(4)));
+    V4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(z[e]);
+    *reinterpret_cast<V4*>(to) = o;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < a.cols) to[e] = from_f32<T>(z[e]);
+  }
+}
+template <typename T, int ROWS, int COLS>
+__device__ __forceinline__ void store_runs(const SideArgs& a, const char* mine, int stride, int64_t m0, int n0, int lane) {
+  own_lds_order();
+  const int c = lane % COLS, n = n0 + c;
+#pragma unroll
+  for (int r = 0; r < ROWS; r += 64 / COLS) {
+    const int row = r + lane / COLS;
+    const float v = *reinterpret_cast<const float*>(mine + row * stride + c * 4);
+    if (m0 + row < a.rows && n < a.cols) reinterpret_cast<T*>(a.out)[(m0 + row) * a.ldo + n] = from_f32<T>(v);
+  }
+  own_lds_order();
+}
+
 template <int BM, int BN, int WM, int WN>
 struct ST {
   static constexpr int THREADS = 64 * WM * WN;
   static constexpr int WROWS = BM / WM, WCOLS = BN / WN, TI = WROWS / 16, TJ = WCOLS / 16;
-  static constexpr int STAGE = (BM + BN) * 128, LDS = 2 * STAGE;
-  static constexpr int LOADS = BN * 128 / (THREADS * 16);
-  static_assert(BN * 128 % (THREADS * 16) == 0 && LDS <= 160 * 1024, "tile");
+  static constexpr int V_STAGE = BN * 128, STAGE = V_STAGE + BM * 128, LDS = 2 * STAGE;
+  static constexpr int LOADS = V_STAGE / (THREADS * 16);
+  static_assert(V_STAGE % (THREADS * 16) == 0 && LDS <= 160 * 1024, "tile");
   static_assert(WCOLS % 32 == 0, "a wave holds whole words of the mask");
 };
 
@@ -246,16 +314,16 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
   const int turns = (a.K + 31) / 32;
 
   // (offsets of 32 bits from uniform bases: with 128 registers a lane each address counts)
-  // rows of V behind the last are in the workspace, whatever they hold: their columns are not stored
-  const unsigned src = (unsigned)(n0 + (tid >> 3)) * (unsigned)turns * 128u + (unsigned)(((tid & 7) ^ swz(tid >> 3)) << 4);
-  static_assert(P::THREADS / 8 % 16 == 0, "the swizzle of a thread's rows is the same");
+  // (rows of V behind the last are in the workspace, whatever they hold: their columns are not stored)
+  const int blocks = blocks_of_32(a.K);
   auto issue = [&](int t, int stage) {
     char* st = smem + (stage & 1) * P::STAGE;
 #pragma unroll
     for (int i = 0; i < P::LOADS; ++i) {
-      const char* const V = a.V + (int64_t)t * 128 + (int64_t)i * (P::THREADS / 8) * turns * 128;
-      const char* from = V + pinned(src);
-      __builtin_amdgcn_global_load_lds(from, (lds_void*)(st + (wave + (P::THREADS / 64) * i) * 1024), 16, 0, 0);
+      const int kib = wave + WM * WN * i;  // 16 rows of V, hi or lo
+      const char* const V = a.V + ((int64_t)(n0 / 16 + kib / 2) * blocks + t) * 2048 + kib % 2 * 1024;
+      const char* from = V + pinned(lane * 16u);
+      __builtin_amdgcn_global_load_lds(from, (lds_void*)(st + kib * 1024), 16, 0, 0);
     }
   };
   // this thread's rows (PASS of them) and its values of each turn: k = V (tid % LANES) + (0..V)
@@ -312,7 +380,7 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
     }
   };
   auto put = [&](const Raw& r, int t) {
-    char* st = smem + (t & 1) * P::STAGE;
+    char* st = smem + (t & 1) * P::STAGE + P::V_STAGE;
 #pragma unroll
     for (int p = 0; p < PASS; ++p) {
       typedef _Float16 Piece __attribute__((ext_vector_type(V)));
@@ -326,7 +394,7 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
         hi[e] = piece_hi(x);
         if (LO) lo[e] = piece_lo(x, hi[e]);
       }
-      const int row = BN + row_of(p);
+      const int row = row_of(p);
       *reinterpret_cast<Piece*>(st + chunk_at(row, kc / 8) + (kc % 8) * 2) = hi;
       if (LO) *reinterpret_cast<Piece*>(st + chunk_at(row, 4 + kc / 8) + (kc % 8) * 2) = lo;
     }
@@ -340,35 +408,37 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
   // Two passes over the products, so that one of V's pieces at a time is held: hi of V by both
   // pieces of the rows, then lo of V by hi of the rows.
   auto turn_products = [&](int t) {
-    const char* st = smem + (t & 1) * P::STAGE;
+    const char* const vs = smem + (t & 1) * P::STAGE;
+    const char* const xs = vs + P::V_STAGE;
     f16x8 w[TJ];
 #pragma unroll
-    for (int j = 0; j < TJ; ++j) w[j] = *reinterpret_cast<const f16x8*>(st + chunk_at(wc * P::WCOLS + 16 * j + r16, g4));
+    for (int j = 0; j < TJ; ++j) w[j] = *reinterpret_cast<const f16x8*>(vs + (wc * TJ + j) * 2048 + lane * 16);
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
-      const int r = BN + wr * P::WROWS + 16 * i + r16;
+      const int r = wr * P::WROWS + 16 * i + r16;
       if (LO) {
-        const f16x8 xl = *reinterpret_cast<const f16x8*>(st + chunk_at(r, 4 + g4));
+        const f16x8 xl = *reinterpret_cast<const f16x8*>(xs + chunk_at(r, 4 + g4));
 #pragma unroll
         for (int j = 0; j < TJ; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], xl, acc[j][i], 0, 0, 0);
       }
-      const f16x8 xh = *reinterpret_cast<const f16x8*>(st + chunk_at(r, g4));
+      const f16x8 xh = *reinterpret_cast<const f16x8*>(xs + chunk_at(r, g4));
 #pragma unroll
       for (int j = 0; j < TJ; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], xh, acc[j][i], 0, 0, 0);
     }
 #pragma unroll
     for (int j = 0; j < TJ; ++j)
-      w[j] = *reinterpret_cast<const f16x8*>(st + chunk_at(wc * P::WCOLS + 16 * j + r16, 4 + g4));
+      w[j] = *reinterpret_cast<const f16x8*>(vs + (wc * TJ + j) * 2048 + 1024 + lane * 16);
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
-      const f16x8 xh = *reinterpret_cast<const f16x8*>(st + chunk_at(BN + wr * P::WROWS + 16 * i + r16, g4));
+      const f16x8 xh = *reinterpret_cast<const f16x8*>(xs + chunk_at(wr * P::WROWS + 16 * i + r16, g4));
 #pragma unroll
       for (int j = 0; j < TJ; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], xh, acc[j][i], 0, 0, 0);
     }
   };
   Raw raw;
   issue(block_of(0), 0);
-  fetch_last(raw);
+  if (a.K % 32 == 0) fetch(raw, turns - 1);
+  else fetch_last(raw);
   put(raw, 0);
   if (turns > 1) fetch(raw, block_of(1));
   wait_barrier<0>();
@@ -404,9 +474,6 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
       sn[j][e] = a.vshift[n];
       bias[j][e] = MODE == 0 && a.bias != nullptr ? a.bias[n] : 0.f;
     }
-  // Rows that all start on 16 bytes are stored from the registers.  Others (k = 1023) go through
-  // this wave's own piece of LDS, so that a store is one run of a row: 16-byte stores across
-  // lines took 224 us where these take 163 (65,536 x 1023 x 256, dx).
   const bool direct = ((uintptr_t)a.out | (uintptr_t)(a.ldo * sizeof(T))) % 16 == 0;
   constexpr int RS = P::WCOLS * 4 + 16;
   static_assert(WM * WN * 16 * RS <= P::LDS, "the waves' pieces fit the stages");
@@ -418,68 +485,199 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
 #pragma unroll
     for (int j = 0; j < TJ; ++j) {
       const int n = n0 + wc * P::WCOLS + 16 * j + 4 * g4;
-      float z[4];
+      f32x4 z;
 #pragma unroll
       for (int e = 0; e < 4; ++e) z[e] = by_power(acc[j][i][e], -(sm[i] + sn[j][e])) + bias[j][e];
-      if (MODE == 0) {
-        if (a.add != nullptr && m < a.rows) {
-          const float* const from = a.add + m * a.ldadd + n;
-          if (n + 4 <= a.cols) {
-            const f32x4u v = *reinterpret_cast<const f32x4u*>(from);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z[e] += v[e];
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (n + e < a.cols) z[e] += from[e];
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) z[e] = activate(z[e], a.act);
-      }
-      if (!direct) {
-        *reinterpret_cast<f32x4*>(mine + r16 * RS + (16 * j + 4 * g4) * 4) = f32x4{z[0], z[1], z[2], z[3]};
-      } else if (m < a.rows) {
-        T* const to = reinterpret_cast<T*>(a.out) + m * a.ldo + n;
-        if (n + 4 <= a.cols) {
-          typedef T V4 __attribute__((ext_vector_type(4)));
-          V4 o;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(z[e]);
-          *reinterpret_cast<V4*>(to) = o;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < a.cols) to[e] = from_f32<T>(z[e]);
-        }
-      }
+      if (MODE == 0) finish_forward(a, m, n, z);
+      if (direct) store_four<T>(a, m, n, z);
+      else *reinterpret_cast<f32x4*>(mine + r16 * RS + (16 * j + 4 * g4) * 4) = z;
       if (MODE == 0 && a.mask != nullptr) {
-        uint32_t b = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) b |= (uint32_t)(z[e] > 0.f && n + e < a.cols) << (4 * g4 + e);
-        b |= (uint32_t)__shfl_xor((int)b, 16);
-        b |= (uint32_t)__shfl_xor((int)b, 32);
-        if (j % 2 == 0) {
-          bits = b;
-        } else if (g4 == 0 && m < a.rows && n - 16 < a.cols) {
+        const uint32_t b = mask_bits(z, n, a.cols, g4);
+        if (j % 2 == 0) bits = b;
+        else if (g4 == 0 && m < a.rows && n - 16 < a.cols)
           a.mask[m * ((a.cols + 31) / 32) + (n - 16) / 32] = bits | b << 16;
-        }
       }
     }
-    if (!direct) {
-      own_lds_order();
-      constexpr int AT_ONCE = 64 / P::WCOLS;  // rows of a store
-      const int c = lane % P::WCOLS, n = n0 + wc * P::WCOLS + c;
+    if (!direct)
+      store_runs<T, 16, P::WCOLS>(a, mine, RS, m0 + wr * P::WROWS + 16 * i, n0 + wc * P::WCOLS, lane);
+  }
+}
+
+// ---- dx of short sums, many rows and columns -------------------------------------------------
+// Sums of up to 256.  A workgroup takes 64 whole rows of dz: their largest values and their pieces
+// come from registers that hold them once, and the pieces stay in LDS.  Then each of its 4 waves
+// makes 64 columns of all 64 rows at a time, with V's images straight from L2 into its registers a
+// step ahead: no barrier, nothing split twice, no launch before it that reads dy as well.  Two
+// workgroups a CU: one's rows come in beside the other's products (one of 128 rows and 8 waves,
+// which reads V half as often, 142 us where these take 138: 65,536 x 1024 x 256).
+constexpr int PB = 64, PW = 4, PJ = 4, PC = 16 * PJ, P_BLOCKS = 8;
+constexpr int P_ROW = PC * 4 + 16;  // a row of a wave's piece for results: 8 rows
+constexpr int panel_lds(int blocks) { return blocks * PB * 128 + PB * 4 + PW * 8 * P_ROW; }
+static_assert(panel_lds(P_BLOCKS) <= 160 * 1024, "LDS");
+
+template <int ACT, typename T>
+__global__ __launch_bounds__(64 * PW, 2) void panel_kernel(SideArgs a) {
+  constexpr int LANES = 8, ROWS = 64 * PW / LANES, PASS = PB / ROWS;
+  constexpr bool MASK = ACT == DZ_RELU, WITH_Y = ACT == DZ_SIGMOID;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, g4 = lane >> 4;
+  const int64_t m0 = (int64_t)blockIdx.x * PB;
+  const int blocks = blocks_of_32(a.K);
+  int* const shifts = reinterpret_cast<int*>(smem + blocks * PB * 128);
+  char* const mine = smem + blocks * PB * 128 + PB * 4 + wave * 8 * P_ROW;
+
+  // the rows: LANES lanes each, four values of each block of 32
+  const int kc = tid % LANES * 4;
 #pragma unroll
-      for (int r = 0; r < 16; r += AT_ONCE) {
-        const int row = r + lane / P::WCOLS;
-        const int64_t mr = m0 + wr * P::WROWS + 16 * i + row;
-        const float v = *reinterpret_cast<const float*>(mine + row * RS + c * 4);
-        if (mr < a.rows && n < a.cols) reinterpret_cast<T*>(a.out)[mr * a.ldo + n] = from_f32<T>(v);
+  for (int p = 0; p < PASS; ++p) {
+    const int r = tid / LANES + p * ROWS;
+    const int64_t m = min(m0 + r, a.rows - 1);
+    const float* const row = a.dz.dy + m * a.dz.lddy;
+    f32x4 v[P_BLOCKS], y[WITH_Y ? P_BLOCKS : 1];
+    uint32_t w[MASK ? P_BLOCKS : 1];
+    auto load = [&](f32x4& to, const float* from, int k) {
+      if (k + 4 <= a.K) {
+        to = *reinterpret_cast<const f32x4u*>(from + k);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = k + e < a.K ? from[k + e] : 0.f;
       }
-      own_lds_order();
+    };
+#pragma unroll
+    for (int b = 0; b < P_BLOCKS; ++b)
+      if (b < blocks) {
+        load(v[b], row, b * 32 + kc);
+        if constexpr (WITH_Y) load(y[b], a.dz.y + m * a.dz.ldy, b * 32 + kc);
+        if constexpr (MASK) w[b] = a.dz.mask[m * a.dz.words + min(b, a.dz.words - 1)];
+      }
+    unsigned top = 0;
+#pragma unroll
+    for (int b = 0; b < P_BLOCKS; ++b)
+      if (b < blocks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (WITH_Y) v[b][e] *= y[b][e] * (1.f - y[b][e]);
+          if constexpr (MASK) v[b][e] = (w[b] >> (kc + e)) & 1 ? v[b][e] : 0.f;
+          top = max(top, abs_bits(v[b][e]));
+        }
+    top = row_max<LANES>(top);
+    const int e2 = shift_of(__uint_as_float(top));
+    if (tid % LANES == 0) shifts[r] = e2;
+#pragma unroll
+    for (int b = 0; b < P_BLOCKS; ++b)
+      if (b < blocks) {
+        typedef _Float16 Piece __attribute__((ext_vector_type(4)));
+        Piece hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = by_power(v[b][e], e2);
+          hi[e] = piece_hi(x);
+          lo[e] = piece_lo(x, hi[e]);
+        }
+        char* const st = smem + b * PB * 128;
+        *reinterpret_cast<Piece*>(st + chunk_at(r, kc / 8) + (kc % 8) * 2) = hi;
+        *reinterpret_cast<Piece*>(st + chunk_at(r, 4 + kc / 8) + (kc % 8) * 2) = lo;
+      }
+  }
+  __syncthreads();
+
+  const int tiles = (a.cols + PC - 1) / PC;
+  struct Images {
+    f16x8 hi[PJ], lo[PJ];
+  } va, vb;
+  auto load_v = [&](Images& f, int tile, int b) {
+    const char* const from = a.V + ((int64_t)tile * PJ * blocks + b) * 2048;
+#pragma unroll
+    for (int j = 0; j < PJ; ++j) {
+      f.hi[j] = *reinterpret_cast<const f16x8*>(from + j * blocks * 2048 + pinned(lane * 16u));
+      f.lo[j] = *reinterpret_cast<const f16x8*>(from + j * blocks * 2048 + 1024 + pinned(lane * 16u));
+    }
+  };
+  const bool direct = ((uintptr_t)a.out | (uintptr_t)(a.ldo * sizeof(T))) % 16 == 0;
+  int tile = wave;
+  if (tile < tiles) load_v(va, tile, 0);
+  for (; tile < tiles; tile += PW) {
+    f32x4 acc[PJ][PB / 16];
+#pragma unroll
+    for (int j = 0; j < PJ; ++j)
+#pragma unroll
+      for (int i = 0; i < PB / 16; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto products = [&](const Images& f, int b) {
+      const char* const st = smem + b * PB * 128;
+#pragma unroll
+      for (int i = 0; i < PB / 16; ++i) {
+        const f16x8 xh = *reinterpret_cast<const f16x8*>(st + chunk_at(16 * i + r16, g4));
+        const f16x8 xl = *reinterpret_cast<const f16x8*>(st + chunk_at(16 * i + r16, 4 + g4));
+#pragma unroll
+        for (int j = 0; j < PJ; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.lo[j], xh, acc[j][i], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < PJ; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.hi[j], xl, acc[j][i], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < PJ; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.hi[j], xh, acc[j][i], 0, 0, 0);
+      }
+    };
+#pragma unroll 1
+    for (int b = 0; b < blocks; b += 2) {
+      load_v(vb, tile, b + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      products(va, b);
+      __builtin_amdgcn_sched_barrier(0);
+      const bool last = b + 2 == blocks;
+      load_v(va, last ? min(tile + PW, tiles - 1) : tile, last ? 0 : b + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      products(vb, b + 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // lane: row 16 i + r16, columns 16 j + 4 g4 + (0..3) of the tile's
+    const int n0 = tile * PC;
+    int sn[PJ][4];
+#pragma unroll
+    for (int j = 0; j < PJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sn[j][e] = a.vshift[min(n0 + 16 * j + 4 * g4 + e, a.cols - 1)];
+#pragma unroll
+    for (int i = 0; i < PB / 16; ++i) {
+      const int sm = shifts[16 * i + r16];
+      f32x4 z[PJ];
+#pragma unroll
+      for (int j = 0; j < PJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[j][e] = by_power(acc[j][i][e], -(sm + sn[j][e]));
+      if (direct) {
+#pragma unroll
+        for (int j = 0; j < PJ; ++j) store_four<T>(a, m0 + 16 * i + r16, n0 + 16 * j + 4 * g4, z[j]);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (r16 / 8 == h)
+#pragma unroll
+            for (int j = 0; j < PJ; ++j)
+              *reinterpret_cast<f32x4*>(mine + r16 % 8 * P_ROW + (16 * j + 4 * g4) * 4) = z[j];
+          store_runs<T, 8, PC>(a, mine, P_ROW, m0 + 16 * i + 8 * h, n0, lane);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
+}
+
+template <int ACT, typename T>
+int launch_panel(const SideArgs& a, hipStream_t stream) {
+  const auto kernel = panel_kernel<ACT, T>;
+  static const hipError_t attr =
+      hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, panel_lds(P_BLOCKS));
+  INF_HIP_TRY(attr);
+  kernel<<<(unsigned)ceil_div(a.rows, PB), 64 * PW, panel_lds(blocks_of_32(a.K)), stream>>>(a);
+  INF_LAUNCH_CHECK();
+  return INF_OK;
+}
+
+// Rows for two workgroups a CU, columns for each wave, and sums that the fill is worth.  With the
+// launch before it, here and in tiles, us: 65,536 x 1024 x 256 133 and 169 (x 128 95 and 112, x 32 66
+// and 62), 65,536 x 256 x 256 56 and 56; 32,768 x 1024 x 256 68 and 77, 16,384 45 and 45.
+bool takes_panel(int64_t rows, int K, int cols) {
+  return rows >= 32768 && K > 64 && K <= 32 * P_BLOCKS && cols >= PW * PC;
 }
 
 // ---- dW and db ------------------------------------------------------------------------
@@ -731,9 +929,8 @@ int launch_tile(const SideArgs& a, hipStream_t stream) {
 }
 
 // The widest tile that still fills the CUs.  65,536 x 1024 x 256: forward 108 us with 256 x 256
-// (one of 16 waves a CU), 128 with 128 x 128 (two of 8); dx, whose sums are short and whose
-// results are many, 163 with 128 x 128, where one's stores run beside the other's products, 172
-// with 256 x 128.
+// (one of 16 waves a CU), 128 with 128 x 128 (two of 8); dx, whose results are many, 163 with 128 x
+// 128, where one's stores run beside the other's products, 172 with 256 x 128.
 template <int MODE, int ACT, typename X, typename T>
 int launch_tiles(const SideArgs& a, hipStream_t stream) {
   const int64_t wide = ceil_div(a.rows, 256);
@@ -816,7 +1013,7 @@ DwShape dw_shape(int64_t rows, int n, int k) {
 
 // what the products' 32-bit offsets reach: a weight's pieces, and 256 rows
 bool fits(int n, int k, int64_t ld) {
-  return round_up(n, 256) * round_up(k, 32) < (int64_t)1 << 29 && round_up(k, 256) * round_up(n, 32) < (int64_t)1 << 29 &&
+  return round_up(n, 256) * round_up(k, 64) < (int64_t)1 << 29 && round_up(k, 256) * round_up(n, 64) < (int64_t)1 << 29 &&
          ld < (int64_t)1 << 21;
 }
 
@@ -828,7 +1025,7 @@ ForwardSpace forward_space(int64_t rows, int n, int k) {
   ForwardSpace w;
   w.scale = 0;
   w.V = w.scale + round_up(rows * 4, 256);
-  w.vshift = w.V + round_up(n, 256) * round_up(k, 32) * 4;
+  w.vshift = w.V + round_up(n, 256) * round_up(k, 64) * 4;
   w.bytes = w.vshift + round_up((int64_t)n * 4, 256);
   return w;
 }
@@ -840,7 +1037,7 @@ BackwardSpace backward_space(int64_t rows, int n, int k) {
   BackwardSpace w;
   w.shift = 0;
   w.V = w.shift + round_up(rows * 4, 256);
-  w.vshift = w.V + round_up(k, 256) * round_up(n, 32) * 4;
+  w.vshift = w.V + round_up(k, 256) * round_up(n, 64) * 4;
   w.slabs = w.vshift + round_up((int64_t)k * 4, 256);
   w.db = w.slabs + round_up((int64_t)d.splits * n * k * 4, 256);
   w.bytes = w.db + round_up((int64_t)d.splits * n * 4, 256);
@@ -855,7 +1052,8 @@ int backward(int64_t rows, int n, int k, const Dz& dz, const int8_t* q, int64_t 
   int rc;
   if (dx != nullptr && rows > 0) {
     const Weight w{W, swk, swn, k, n, ws + o.V, (int*)(ws + o.vshift)};
-    rc = launch_before_dx<ACT>(w, dz, rows, n, (int*)(ws + o.shift), st);
+    const bool panel = takes_panel(rows, n, k);
+    rc = panel ? launch_split(w, st) : launch_before_dx<ACT>(w, dz, rows, n, (int*)(ws + o.shift), st);
     if (rc != INF_OK) return rc;
     SideArgs a{};
     a.rows = rows;
@@ -867,7 +1065,9 @@ int backward(int64_t rows, int n, int k, const Dz& dz, const int8_t* q, int64_t 
     a.vshift = (int*)(ws + o.vshift);
     a.out = dx;
     a.ldo = lddx;
-    rc = dx_dtype == INF_DTYPE_F32 ? launch_tiles<1, ACT, float, float>(a, st) : launch_tiles<1, ACT, float, bf16>(a, st);
+    rc = panel ? (dx_dtype == INF_DTYPE_F32 ? launch_panel<ACT, float>(a, st) : launch_panel<ACT, bf16>(a, st))
+               : (dx_dtype == INF_DTYPE_F32 ? launch_tiles<1, ACT, float, float>(a, st)
+                                            : launch_tiles<1, ACT, float, bf16>(a, st));
     if (rc != INF_OK) return rc;
   }
   if (dW != nullptr) {
@@ -926,13 +1126,13 @@ int inf_linear_ckpt_forward(int64_t rows, int n, int k, const void* x, int x_dty
   const Weight w{W, stride_wn, stride_wk, n, k, ws + o.V, (int*)(ws + o.vshift)};
   SideArgs a{};
   a.scale = scale;
+  const bool f32 = x_dtype == INF_DTYPE_F32;
   int rc;
   if (q == nullptr && scale != nullptr) {
     rc = launch_split(w, st);
   } else {
     if (scale == nullptr) a.scale = (float*)(ws + o.scale);
-    rc = x_dtype == INF_DTYPE_F32
-             ? launch_before_forward(w, (const float*)x, rows, k, ld_x, q, ld_q, (float*)a.scale, st)
+    rc = f32 ? launch_before_forward(w, (const float*)x, rows, k, ld_x, q, ld_q, (float*)a.scale, st)
              : launch_before_forward(w, (const bf16*)x, rows, k, ld_x, q, ld_q, (float*)a.scale, st);
   }
   if (rc != INF_OK) return rc;
@@ -950,7 +1150,7 @@ int inf_linear_ckpt_forward(int64_t rows, int n, int k, const void* x, int x_dty
   a.out = y;
   a.ldo = ld_y;
   a.mask = mask;
-  return x_dtype == INF_DTYPE_F32 ? launch_tiles<0, 0, float, float>(a, st) : launch_tiles<0, 0, bf16, float>(a, st);
+  return f32 ? launch_tiles<0, 0, float, float>(a, st) : launch_tiles<0, 0, bf16, float>(a, st);
 }
 
 int inf_linear_ckpt_backward(int64_t rows, int n, int k, const float* dy, int64_t ld_dy, int act, const float* y,

@@ -341,7 +341,8 @@ def leaves(rows, n, widths, dtype, seed=0):
 
 LAYERS = [(1, 1, (1,)), (1, 3, (5,)), (2, 33, (31,)), (64, 64, (64,)), (100, 3, (256,)), (65, 130, (63,)),
           (300, 256, (1023,)), (512, 256, (256,)), (129, 257, (255,)), (1000, 128, (3,)), (257, 64, (100, 40)),
-          (600, 256, (256, 1024)), (3000, 96, (64,)), (77, 512, (512,))]
+          (600, 256, (256, 1024)), (3000, 96, (64,)), (77, 512, (512,)),
+          (32769, 256, (256,)), (32800, 66, (257, 300)), (33000, 130, (1,)), (32768, 200, (511,))]
 
 
 @pytest.mark.parametrize("act", [None, "relu", "sigmoid"])
