@@ -30,13 +30,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 enum { DZ_NONE = 0, DZ_RELU = 1, DZ_SIGMOID = 2 };  // act
 
-// An offset that the compiler adds to its uniform base in the load itself: left to it, it adds
-// them before the loop, into two registers each, and spills.
-__device__ __forceinline__ unsigned pinned(unsigned o) {
-  asm volatile("" : "+v"(o));
-  return o;
-}
-
 // the power of two that takes a row of largest value a below 2^15
 __device__ __forceinline__ int shift_of(float a) { return 15 - __builtin_amdgcn_frexp_expf(a); }
 __device__ __forceinline__ float by_power(float v, int e) { return __builtin_amdgcn_ldexpf(v, e); }

@@ -5,10 +5,11 @@
 // The roundings are written out one by one and never contracted: a row that goes into 8
 // bits again has the same numbers whichever kernel made it.
 //
-// Three kernels.  Up to 16 rows: linear8_few_kernel, one launch, bound by its latency and by
-// reading the weights once.  Many rows and a weight that fits in LDS: linear8_rows_kernel, one
-// launch.  Otherwise x goes into 8 bits in a launch of its own (rows8.hip: a row's maximum is
-// needed before its first product), then linear8_tile_kernel.
+// Four kernels.  Up to 16 rows: linear8_few_kernel, one launch, bound by its latency and by
+// reading the weights once.  Up to 256 outputs: one launch that holds the weight and walks over
+// the rows, linear8_rows_kernel (in LDS; many rows of up to 256 values) or linear8_long_kernel (in
+// registers; up to 1024).  Otherwise x goes into 8 bits in a launch of its own (rows8.hip: a row's
+// maximum is needed before its first product), then linear8_tile_kernel.
 #include <algorithm>
 
 #include "mtile.hpp"
@@ -536,6 +537,235 @@ int launch_rows_out(const Linear8Args& a, int out_dtype, const void* x, int64_t 
   return launch_rows_any<X, float>(a, x, ldx, stream);
 }
 
+// ---- many long rows, up to 256 outputs -----------------------------------------------------
+// A workgroup of 16 waves (one a CU) holds the whole weight in registers, 16 outputs a wave, as the
+// instruction reads them, and walks over the rows, 32 at a time: each row of x, fp32 or bf16, is held in
+// one wave's registers between its maximum and its rounding and goes to LDS in 8 bits, where every wave
+// reads it; the next rows are on their way meanwhile.  Two stages, so one barrier a turn.
+// 262,144 x 1024 x 256, us: fp32 260, its bytes at a copy's rate (in 8 bits through memory, then
+// tiles: 414); bf16 186, where they would take 156 (264).  32 rows a turn where the registers hold them
+// (16: 262,144 x 512 x 256, bf16 166 where these take 142), fp32 rows of more than 512 values 16 (32 spill:
+// 394 where these take 260).
+constexpr int LONG_WAVES = 16, LONG_K = 1024;
+
+template <typename X, typename T, int CH, int ROWS>
+struct LL {
+  static constexpr int V = Chunk<X>::V, K = CH * 64 * V, BLOCKS = K / 128;  // the longest row
+  static constexpr int THREADS = 64 * LONG_WAVES, R = ROWS / LONG_WAVES;
+  static constexpr int STAGE = BLOCKS * ROWS * 128, SCALES = 2 * STAGE;
+  static constexpr int TOPS = SCALES + 2 * ROWS * 4, IMAGE = TOPS + 2 * ROWS * 4;
+  static constexpr int WS = IMAGE + (sizeof(T) == 1 ? ROWS * 256 : 0), LDS = WS + 16 * LONG_WAVES * 8;
+  static_assert(LDS <= 160 * 1024, "LDS");
+};
+
+template <typename X, typename T, int CH, int ROWS>
+__global__ __launch_bounds__(64 * LONG_WAVES) void linear8_long_kernel(Linear8Args a, const X* __restrict__ x,
+                                                                        int64_t ldx) {
+  using P = LL<X, T, CH, ROWS>;
+  constexpr int V = P::V, R = P::R, TI = ROWS / 16;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tiles = (int)((a.rows + ROWS - 1) / ROWS), blocks = (int)(a.ldw / 128);
+  const bool busy = wave * 16 < a.n;
+
+  i32x4 w[P::BLOCKS][2];
+  float* const sws = reinterpret_cast<float*>(smem + P::WS);  // scales, then biases
+  if (tid < 16 * LONG_WAVES) {
+    sws[tid] = a.ws[min(tid, a.n - 1)];
+    sws[16 * LONG_WAVES + tid] = a.bias != nullptr ? a.bias[min(tid, a.n - 1)] : 0.f;
+  }
+  {
+    const char* const from = reinterpret_cast<const char*>(a.w + min(wave * 16 + lane % 16, a.n - 1) * a.ldw) + lane / 16 * 16;
+#pragma unroll
+    for (int b = 0; b < P::BLOCKS; ++b)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w[b][h] = b < blocks ? *reinterpret_cast<const i32x4*>(from + b * 128 + h * 64) : i32x4{0, 0, 0, 0};
+  }
+
+  // A chunk across the end of a row is loaded from its last V values and moved down when it is used
+  // (no branch around a load: the loads stay on their way).
+  typename Chunk<X>::X raw[R][CH];
+  // Of rows that fill the registers, each turn works its addresses out again from the lane's number:
+  // kept, they do not fit (284 us where these take 260).  Of shorter ones they do, and cost less: 262,144 x
+  // 512 x 256 into bf16 169 and 142.
+  auto this_lane = [&]() { return P::BLOCKS == LONG_K / 128 ? (int)pinned(tid & 63) : tid & 63; };
+  auto fetch = [&](int tile) {
+    const int lane = this_lane();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const X* const row = x + min((int64_t)tile * ROWS + wave * R + r, a.rows - 1) * ldx;
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+        raw[r][i] = *reinterpret_cast<const typename Chunk<X>::X*>(
+            reinterpret_cast<const char*>(row) + (unsigned)min((i * 64 + lane) * V, a.k - V) * sizeof(X));
+    }
+  };
+  if (sizeof(T) == 1 && tid < 2 * ROWS) reinterpret_cast<unsigned*>(smem + P::TOPS)[tid] = 0;
+  int tile = (int)blockIdx.x;
+  if (tile < tiles) fetch(tile);
+#pragma unroll 1
+  for (int t = 0; tile < tiles; ++t) {
+    const int lane = this_lane();
+    char* const st = smem + (t & 1) * P::STAGE;
+    float* const sxs = reinterpret_cast<float*>(smem + P::SCALES) + (t & 1) * ROWS;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      __builtin_amdgcn_sched_barrier(0);
+      const int row = wave * R + r;
+      float v[CH][V];
+      unsigned top = 0;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[i][e] = to_f32(raw[r][i][e]);
+        if ((i + 1) * 64 * V > a.k) {
+          const int past = (i * 64 + lane + 1) * V - a.k;  // values of the chunk behind the row's end
+#pragma unroll
+          for (int h = 1; h < V; h *= 2)
+            if (past > 0 && (past & h))
+#pragma unroll
+              for (int e = 0; e < V; ++e) v[i][e] = e + h < V ? v[i][e + h] : 0.f;
+          if (past >= V)
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[i][e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) top = max(top, abs_bits(v[i][e]));
+      }
+      const RowScale rs = row_scale(row_max<64>(top));
+      if (lane == 0) sxs[row] = rs.s;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int c = (i * 64 + lane) * V;
+        uint32_t q[V / 4];
+#pragma unroll
+        for (int e = 0; e < V; e += 4) q[e / 4] = quantize4<X>(v[i][e], v[i][e + 1], v[i][e + 2], v[i][e + 3], rs);
+        char* const to = st + c / 128 * ROWS * 128 + chunk_at(row, c % 128 / 16) + c % 16;
+        if constexpr (V == 4) *reinterpret_cast<uint32_t*>(to) = q[0];
+        else *reinterpret_cast<u32x2*>(to) = u32x2{q[0], q[V / 4 - 1]};
+      }
+    }
+    const int64_t m0 = (int64_t)tile * ROWS;
+    tile += (int)gridDim.x;
+    __builtin_amdgcn_sched_barrier(0);
+    if (tile < tiles) fetch(tile);
+    wait_lds_barrier();
+
+    const int again = this_lane(), r16 = again & 15, g4 = again >> 4, n = wave * 16 + 4 * g4;  // n: this lane's outputs
+    i32x4 acc[TI];
+#pragma unroll
+    for (int i = 0; i < TI; ++i) acc[i] = i32x4{0, 0, 0, 0};
+    if (busy) {
+#pragma unroll
+      for (int b = 0; b < P::BLOCKS; ++b) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (b < blocks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < TI; ++i) {
+              const i32x4 xf =
+                  *reinterpret_cast<const i32x4*>(st + b * ROWS * 128 + chunk_at(16 * i + r16, 4 * h + g4));
+              acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[b][h], xf, acc[i], 0, 0, 0);
+            }
+      }
+    }
+    // lane: row 16 i + r16, outputs n + (0..3)
+    __builtin_amdgcn_sched_barrier(0);
+    const f32x4 sw = *reinterpret_cast<const f32x4*>(sws + n), bias = *reinterpret_cast<const f32x4*>(sws + 16 * LONG_WAVES + n);
+    f32x4 z[TI];
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      const int64_t m = m0 + 16 * i + r16;
+      const float sx = sxs[16 * i + r16];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[i][e] = combine(acc[i][e], sx, sw[e], bias[e]);
+      if (a.add != nullptr)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[i][e] += a.add[min(m, a.rows - 1) * a.ldadd + min(n + e, a.n - 1)];
+      if (a.act == 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[i][e] = activate(z[i][e], 1);
+      if (a.act == 2)  // one copy of its code for the four
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) z[i] = f32x4{z[i][1], z[i][2], z[i][3], activate(z[i][0], 2)};
+      if constexpr (sizeof(T) != 1) {
+        if (m >= a.rows) continue;
+        T* const to = reinterpret_cast<T*>(a.out) + m * a.ldo + n;
+        if (n + 4 <= a.n) {
+          typename Four<T>::V o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(z[i][e]);
+          *reinterpret_cast<typename Four<T>::V*>(to) = o;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < a.n) to[e] = from_f32<T>(z[i][e]);
+        }
+      }
+    }
+    if constexpr (sizeof(T) == 1) {
+      unsigned* const tops = reinterpret_cast<unsigned*>(smem + P::TOPS) + (t & 1) * ROWS;
+      char* const image = smem + P::IMAGE;
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        unsigned b = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < a.n) b = max(b, abs_bits(z[i][e]));
+        b = max(b, (unsigned)__shfl_xor((int)b, 16));
+        b = max(b, (unsigned)__shfl_xor((int)b, 32));
+        if (g4 == 0 && busy) atomicMax(&tops[16 * i + r16], b);  // a maximum: in any order the same
+      }
+      // the other turn's maxima: last read before this turn's first barrier, next used after its last
+      if (tid < ROWS) reinterpret_cast<unsigned*>(smem + P::TOPS)[((t + 1) & 1) * ROWS + tid] = 0;
+      wait_lds_barrier();
+      if (tid < ROWS && m0 + tid < a.rows) a.os[m0 + tid] = row_scale(tops[tid]).s;
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        const int row = 16 * i + r16;
+        if (busy)
+          *reinterpret_cast<uint32_t*>(image + row * 256 + ((wave ^ r16) << 4) + 4 * g4) =
+              quantize4(z[i][0], z[i][1], z[i][2], z[i][3], row_scale(tops[row]));
+      }
+      wait_lds_barrier();
+      // whole 16-byte pieces: q rows are multiples of 16, so a piece that begins before n fits
+      if (tid < ROWS * 16) {
+        const int row = tid / 16, c = tid % 16;
+        if (m0 + row < a.rows && c * 16 < a.n)
+          *reinterpret_cast<u32x4*>((int8_t*)a.out + (m0 + row) * a.ldo + c * 16) =
+              *reinterpret_cast<const u32x4*>(image + row * 256 + ((c ^ (row & 15)) << 4));
+      }
+    }
+  }
+}
+
+template <typename X, typename T, int CH, int ROWS>
+int launch_long_as(const Linear8Args& a, const X* x, int64_t ldx, hipStream_t stream) {
+  using P = LL<X, T, CH, ROWS>;
+  const auto kernel = linear8_long_kernel<X, T, CH, ROWS>;
+  static const hipError_t attr =
+      hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
+  INF_HIP_TRY(attr);
+  kernel<<<(unsigned)std::min<int64_t>(ceil_div(a.rows, ROWS), 256), P::THREADS, P::LDS, stream>>>(a, x, ldx);
+  INF_LAUNCH_CHECK();
+  return INF_OK;
+}
+
+template <typename X>
+int launch_long(const Linear8Args& a, int out_dtype, const void* x, int64_t ldx, hipStream_t stream) {
+  constexpr int CH = LONG_K / 64 / Chunk<X>::V;
+  const auto go = [&](auto t) {
+    using T = decltype(t);
+    return a.k <= LONG_K / 2 ? launch_long_as<X, T, CH / 2, 32>(a, (const X*)x, ldx, stream)
+                             : launch_long_as<X, T, CH, sizeof(X) == 4 ? 16 : 32>(a, (const X*)x, ldx, stream);
+  };
+  if (out_dtype == INF_DTYPE_I8) return go(int8_t{});
+  if (out_dtype == INF_DTYPE_BF16) return go(bf16{});
+  return go(float{});
+}
+
 template <typename T, int BM, int BN, int WM, int WN>
 int launch_tile(const Linear8Args& a, hipStream_t stream) {
   using P = L8<BM, BN, WM, WN>;
@@ -589,6 +819,11 @@ int launch_few_out(const Linear8Args& a, int out_dtype, const void* x, int64_t l
 }
 
 bool is_few(int64_t rows, int k) { return rows <= FEW && rows * (round_up(k, W_ALIGN) + 16) <= FEW_LDS; }
+// Rows of any number that are longer than linear8_rows_kernel's.  4096 x 1024, us: 64 outputs 9 (in two
+// launches 5 + 8), 256 outputs 13 (5 + 8); 128 rows 8 (4 + 7) and 12 (4 + 8).
+bool takes_long(int64_t rows, int n, int k, int x_dtype) {
+  return x_dtype != INF_DTYPE_I8 && !is_few(rows, k) && k > 256 && k <= LONG_K && n <= 16 * LONG_WAVES;
+}
 // whether a result in 8 bits is made by the product's own kernel
 bool rows_whole(int64_t rows, int n, int k) { return n <= 256 && !is_few(rows, k); }
 
@@ -598,7 +833,7 @@ struct Workspace {
 
 Workspace workspace_of(int64_t rows, int n, int k, int x_dtype, int out_dtype) {
   Workspace w{0, 0, 0, 0};
-  if (x_dtype != INF_DTYPE_I8 && !is_few(rows, k)) {
+  if (x_dtype != INF_DTYPE_I8 && !is_few(rows, k) && !takes_long(rows, n, k, x_dtype)) {
     w.q = w.bytes;
     w.bytes += round_up(rows * round_up(k, Q_ALIGN) + Q_SLACK, 256);
     w.qs = w.bytes;
@@ -665,6 +900,9 @@ int inf_linear_int(int64_t rows, int n, int k, const void* x, int x_dtype, int64
     rc = x8 ? launch_rows_out<int8_t>(a, product_dtype, x, ld_x, st)
             : x_dtype == INF_DTYPE_BF16 ? launch_rows_out<bf16>(a, product_dtype, x, ld_x, st)
                                         : launch_rows_out<float>(a, product_dtype, x, ld_x, st);
+  } else if (takes_long(rows, n, k, x_dtype)) {
+    rc = x_dtype == INF_DTYPE_BF16 ? launch_long<bf16>(a, product_dtype, x, ld_x, st)
+                                   : launch_long<float>(a, product_dtype, x, ld_x, st);
   } else {
     if (!x8) {
       a.q = (int8_t*)(wsp + o.q);

@@ -14,6 +14,13 @@ typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
+// An offset that the compiler adds to its uniform base in the load itself: left to it, it adds
+// them before the loop, into two registers each, and spills.
+__device__ __forceinline__ unsigned pinned(unsigned o) {
+  asm volatile("" : "+v"(o));
+  return o;
+}
+
 // Chunk c (16 bytes) of a stage row lies at c ^ ((row >> 1) & 7): the 16 rows that a
 // fragment read touches at one c fall into all 64 banks evenly.
 __device__ __forceinline__ int swz(int row) { return (row >> 1) & 7; }

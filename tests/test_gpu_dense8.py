@@ -164,7 +164,8 @@ def weight8(n, k, seed):
 SIZES = [(1, 1, 1), (1, 3, 1024), (1, 256, 1024), (2, 17, 63), (5, 256, 1023), (15, 128, 64), (16, 100, 129),
          (17, 3, 256), (33, 130, 100), (64, 64, 4096), (65, 257, 300), (127, 96, 127), (128, 128, 128),
          (300, 256, 256), (257, 511, 193), (1000, 3, 16), (520, 1030, 65), (1, 4096, 2048), (8, 4097, 33),
-         (16390, 256, 256), (16400, 100, 77), (17001, 129, 200), (16384, 255, 3), (16385, 64, 128)]
+         (16390, 256, 256), (16400, 100, 77), (17001, 129, 200), (16384, 255, 3), (16385, 64, 128),
+         (32769, 256, 1023), (32790, 40, 300), (32770, 3, 513), (32831, 129, 512), (32768, 253, 769)]
 
 
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
@@ -187,7 +188,8 @@ def test_linear8(rows, n, k, dtype, out):
 
 @pytest.mark.parametrize("rows,n,k", [(1, 1, 5), (1, 256, 1024), (3, 255, 64), (130, 256, 256), (700, 128, 100),
                                       (70, 64, 1023), (20, 3, 40), (65, 300, 30), (9, 1025, 17), (16390, 256, 255),
-                                      (16400, 100, 128), (16411, 37, 64)])
+                                      (16400, 100, 128), (16411, 37, 64), (32769, 256, 1024),
+                                      (32800, 70, 290), (33000, 3, 1000)])
 def test_linear8_rows_out_are_the_rows_of_the_result(rows, n, k):
     """out=int8 is quantize_rows of the fp32 result, bit for bit, whichever kernel makes it."""
     d = dense()
@@ -206,7 +208,8 @@ def test_linear8_rows_out_are_the_rows_of_the_result(rows, n, k):
 def test_linear8_each_form_gives_the_same_numbers():
     """A row's result does not depend on how many rows come with it, nor on who quantised it."""
     d = dense()
-    for n, k, rows in ((256, 1024, 600), (100, 77, 16500), (3, 256, 600), (256, 200, 20000)):
+    for n, k, rows in ((256, 1024, 600), (100, 77, 16500), (3, 256, 600), (256, 200, 20000),
+                       (200, 1023, 32900)):
         x = make(rows, k, torch.float32, 2)
         qw, sw = weight8(n, k, 1)
         w, b = d.pack_weight8(qw.cuda(), sw.cuda()), torch.randn(n).cuda()
@@ -238,6 +241,25 @@ def test_linear8_segments_and_bad_rows():
         assert bad[[7, 9, 11]].all() and bad.sum() == 3 * n
     r = d.linear8([x0, x1], w, b, None, out=torch.int8)
     assert torch.isnan(r.scale.cpu()[[7, 9, 11]]).all() and int(torch.isnan(r.scale).sum()) == 3
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.int8])
+def test_linear8_long_rows_add_and_bad_rows(out):
+    """Many long rows on top of another segment's result; a bad row and a zero row stay by themselves."""
+    d = dense()
+    rows, n = 32770, 90
+    x0, x1 = make(rows, 31, torch.float32, 1), make(rows, 700, torch.bfloat16, 2)
+    x0[3], x1[3] = 0, 0
+    ws = [weight8(n, 31, 5), weight8(n, 700, 6)]
+    w = [d.pack_weight8(q.cuda(), s.cuda()) for q, s in ws]
+    b = [torch.randn(n).cuda()]
+    y = d.linear8([x0, x1], w, b, "sigmoid")
+    want, err = oracle_linear8([x0, x1], ws, b, "sigmoid")
+    assert ((y.cpu().double() - want).abs() <= err).all()
+    x1[9, 0], x1[rows - 1, 699] = float("nan"), -float("inf")
+    r = d.linear8([x0, x1], w, b, "relu", out=out)
+    bad = torch.isnan(r.scale if out == torch.int8 else r.sum(1)).cpu()
+    assert bad[[9, rows - 1]].all() and int(bad.sum()) == 2
 
 
 def test_linear8_largest_sum_and_strided_weight():
