@@ -29,9 +29,15 @@ from torch.autograd.function import once_differentiable
 ACT = {None: 0, "relu": 1, "sigmoid": 2}
 
 
+_runtime = None
+
+
 def _rt():
-    from inf_hip import runtime  # raises if the HIP library is missing: no fallback
-    return runtime
+    global _runtime
+    if _runtime is None:
+        from inf_hip import runtime  # raises if the HIP library is missing: no fallback
+        _runtime = runtime
+    return _runtime
 
 
 def _gemm(M, N, K, A, sam, sak, B, sbn, sbk, bias, act, beta, C, ldc):
@@ -130,7 +136,11 @@ _ON_CURRENT = contextlib.nullcontext()
 
 def _on(device):
     """The device of the tensors as the current one, for launches on its current stream."""
-    return _ON_CURRENT if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _ON_CURRENT if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def _stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _at(t):
@@ -180,7 +190,7 @@ class Rows8:
         out = torch.empty((rows, k), dtype=dtype, device=q.device)
         with _on(q.device):
             rt.check(rt.lib.inf_restore_rows(q.data_ptr(), q.stride(0), self.scale.data_ptr(), rows, k, out.data_ptr(),
-                                             rt.dtype_code(out), k, rt.stream_handle()), "restore_rows")
+                                             rt.dtype_code(out), k, _stream(q.device)), "restore_rows")
         return out
 
 
@@ -195,7 +205,7 @@ def quantize_rows(x):
     r = Rows8(rows, k, x.device)
     with _on(x.device):
         rt.check(rt.lib.inf_quantize_rows(x.data_ptr(), rt.dtype_code(x), rows, k, x.stride(0), r.q.data_ptr(),
-                                          r.q.stride(0), r.scale.data_ptr(), rt.stream_handle()), "quantize_rows")
+                                          r.q.stride(0), r.scale.data_ptr(), _stream(x.device)), "quantize_rows")
     return r
 
 
@@ -220,7 +230,7 @@ def pack_weight8(q, scale):
     packed = torch.empty(int(rt.lib.inf_packed_weight_bytes(n, k)), dtype=torch.int8, device=q.device)
     with _on(q.device):
         rt.check(rt.lib.inf_pack_weight(q.data_ptr(), q.stride(0), q.stride(1), n, k, packed.data_ptr(),
-                                        rt.stream_handle()), "pack_weight")
+                                        _stream(q.device)), "pack_weight")
     return Weight8(packed, scale.clone(), n, k)
 
 
@@ -280,7 +290,7 @@ def linear8(xs, weights, biases, act=None, out=torch.float32):
             ws = torch.empty(nws, dtype=torch.uint8, device=device) if nws else None
             rt.check(lib.inf_linear_int(rows, n, w.k, q.data_ptr(), xc, q.stride(0), scale, w.packed.data_ptr(),
                                         w.scale.data_ptr(), _at(b), _at(acc), n, a if s == last else 0, op, oc, ldo,
-                                        osc, _at(ws), rt.stream_handle()), "linear_int")
+                                        osc, _at(ws), _stream(device)), "linear_int")
             acc = y
     return y
 
@@ -309,7 +319,7 @@ class _LinearCkpt(torch.autograd.Function):
         if mask_at is not None:
             at += rows * ((n + 31) // 32) * 4
         with _on(device):
-            st = rt.stream_handle()
+            st = _stream(device)
             y = torch.empty((rows, n), dtype=torch.float32, device=device)
             yp = y.data_ptr()
             held = torch.empty(at, dtype=torch.uint8, device=device) if at else None
@@ -361,7 +371,7 @@ class _LinearCkpt(torch.autograd.Function):
         base = held.data_ptr() if held is not None else 0
         grads = [None] * (3 + nseg + nw + nb)
         with _on(device):
-            st = rt.stream_handle()
+            st = _stream(device)
             for s, (wi, c0) in enumerate(spec):
                 W, k = ws[wi], widths[s]
                 ldq = _round_up(k, 16)
