@@ -658,9 +658,9 @@ __global__ __launch_bounds__(64 * PW, 2) void panel_kernel(SideArgs a) {
 template <int ACT, typename T>
 int launch_panel(const SideArgs& a, hipStream_t stream) {
   const auto kernel = panel_kernel<ACT, T>;
-  static const hipError_t attr =
-      hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, panel_lds(P_BLOCKS));
-  INF_HIP_TRY(attr);
+  static LdsLimit lds;
+  const int allowed = lds.raise((const void*)kernel, panel_lds(P_BLOCKS));
+  if (allowed != INF_OK) return allowed;
   kernel<<<(unsigned)ceil_div(a.rows, PB), 64 * PW, panel_lds(blocks_of_32(a.K)), stream>>>(a);
   INF_LAUNCH_CHECK();
   return INF_OK;
@@ -913,9 +913,9 @@ int launch_tile(const SideArgs& a, hipStream_t stream) {
   const int64_t nblocks = ceil_div(a.rows, BM) * tiles_n;
   INF_CHECK_ARG(nblocks < (int64_t)1 << 31, "linear_ckpt: too many tiles");
   const auto kernel = split_tile_kernel<MODE, ACT, X, T, BM, BN, WM, WN>;
-  static const hipError_t attr =
-      hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
-  INF_HIP_TRY(attr);
+  static LdsLimit lds;
+  const int allowed = lds.raise((const void*)kernel, P::LDS);
+  if (allowed != INF_OK) return allowed;
   kernel<<<(unsigned)nblocks, P::THREADS, P::LDS, stream>>>(a, tiles_n, (int)nblocks);
   INF_LAUNCH_CHECK();
   return INF_OK;
@@ -979,9 +979,9 @@ int launch_before_dx(const Weight& w, const Dz& d, int64_t rows, int n, int* shi
 
 template <int ACT>
 int launch_dw(const DwArgs& a, hipStream_t stream) {
-  static const hipError_t attr =
-      hipFuncSetAttribute((const void*)dw_tile_kernel<ACT>, hipFuncAttributeMaxDynamicSharedMemorySize, DW_LDS);
-  INF_HIP_TRY(attr);
+  static LdsLimit lds;
+  const int allowed = lds.raise((const void*)dw_tile_kernel<ACT>, DW_LDS);
+  if (allowed != INF_OK) return allowed;
   dw_tile_kernel<ACT><<<(unsigned)(a.tiles * a.splits), DW_THREADS, DW_LDS, stream>>>(a);
   INF_LAUNCH_CHECK();
   return INF_OK;

@@ -519,9 +519,9 @@ template <typename X, typename T, int KS, int TJ>
 int launch_rows(const Linear8Args& a, const X* x, int64_t ldx, hipStream_t stream) {
   using P = LR<X, T, KS, TJ>;
   const auto kernel = linear8_rows_kernel<X, T, KS, TJ>;
-  static const hipError_t attr =
-      hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
-  INF_HIP_TRY(attr);
+  static LdsLimit lds;
+  const int allowed = lds.raise((const void*)kernel, P::LDS);
+  if (allowed != INF_OK) return allowed;
   const int64_t groups = ceil_div(a.rows, 16 * P::NW);
   kernel<<<(unsigned)std::min<int64_t>(groups, 256), P::THREADS, P::LDS, stream>>>(a, x, ldx);
   INF_LAUNCH_CHECK();
@@ -759,9 +759,9 @@ template <typename X, typename T, int CH, int ROWS>
 int launch_long_as(const Linear8Args& a, const X* x, int64_t ldx, hipStream_t stream) {
   using P = LL<X, T, CH, ROWS>;
   const auto kernel = linear8_long_kernel<X, T, CH, ROWS>;
-  static const hipError_t attr =
-      hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
-  INF_HIP_TRY(attr);
+  static LdsLimit lds;
+  const int allowed = lds.raise((const void*)kernel, P::LDS);
+  if (allowed != INF_OK) return allowed;
   kernel<<<(unsigned)std::min<int64_t>(ceil_div(a.rows, ROWS), 256), P::THREADS, P::LDS, stream>>>(a, x, ldx);
   INF_LAUNCH_CHECK();
   return INF_OK;
@@ -786,9 +786,9 @@ int launch_tile(const Linear8Args& a, hipStream_t stream) {
   const int tiles_n = (int)ceil_div(a.n, BN);
   const int64_t nblocks = ceil_div(a.rows, BM) * tiles_n;
   INF_CHECK_ARG(nblocks < (int64_t)1 << 31, "linear_int: too many tiles");
-  static const hipError_t attr = hipFuncSetAttribute((const void*)linear8_tile_kernel<T, BM, BN, WM, WN>,
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
-  INF_HIP_TRY(attr);
+  static LdsLimit lds;
+  const int allowed = lds.raise((const void*)linear8_tile_kernel<T, BM, BN, WM, WN>, P::LDS);
+  if (allowed != INF_OK) return allowed;
   linear8_tile_kernel<T, BM, BN, WM, WN>
       <<<(unsigned)nblocks, P::THREADS, P::LDS, stream>>>(a, tiles_n, (int)nblocks);
   INF_LAUNCH_CHECK();
@@ -815,9 +815,9 @@ int launch_linear8(const Linear8Args& a, int out_dtype, hipStream_t stream) {
 
 template <typename X, typename T>
 int launch_few(const Linear8Args& a, const X* x, int64_t ldx, hipStream_t stream) {
-  static const hipError_t attr = hipFuncSetAttribute((const void*)linear8_few_kernel<X, T>,
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, FEW_LDS);
-  INF_HIP_TRY(attr);
+  static LdsLimit lds;
+  const int allowed = lds.raise((const void*)linear8_few_kernel<X, T>, FEW_LDS);
+  if (allowed != INF_OK) return allowed;
   int log_rows = 0;
   while ((1 << log_rows) < a.rows) ++log_rows;
   linear8_few_kernel<X, T><<<(unsigned)ceil_div(a.n, 16), 256, (size_t)(a.rows * (a.ldw + 16)), stream>>>(a, x, ldx,

@@ -2,6 +2,8 @@
 // rows, filled straight from memory, and their fragments.
 #pragma once
 
+#include <atomic>
+
 #include "quant.hpp"
 
 namespace inf {
@@ -58,6 +60,22 @@ __device__ __forceinline__ int xcd_order(int orig, int nblocks) {
   const int q = nblocks / 8, r = nblocks % 8, xcd = orig % 8;
   return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + orig / 8;
 }
+
+// Leave for a kernel to take more LDS than a launch may by default: asked for once a device, by
+// whichever call comes first.
+struct LdsLimit {
+  std::atomic<uint64_t> devices{0};
+  int raise(const void* kernel, int bytes) {
+    int device = 0;
+    INF_HIP_TRY(hipGetDevice(&device));
+    const uint64_t bit = (uint64_t)1 << (device & 63);
+    if (!(devices.load(std::memory_order_relaxed) & bit)) {
+      INF_HIP_TRY(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+      devices.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return INF_OK;
+  }
+};
 
 }  // namespace mt
 }  // namespace inf

@@ -160,6 +160,11 @@ def _rows_of(x, what):
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
+def _near(x):
+    """x with rows less than 2^21 values apart, as the checkpointed layer's products take them."""
+    return x if x.stride(0) < 1 << 21 else x.contiguous()
+
+
 class Rows8:
     """The rows of a matrix in 8 bits: `q` int8 [rows, k] (rows start on 16 bytes) and
     `scale` fp32 [rows], standing for scale[:, None] * q.  Made by quantize_rows and linear8."""
@@ -367,6 +372,7 @@ class _LinearCkpt(torch.autograd.Function):
             dy = dy.to(torch.float32)
         if dy.stride(1) != 1 or dy.stride(0) < n:
             dy = dy.contiguous()
+        dy = _near(dy)
         device = dy.device
         base = held.data_ptr() if held is not None else 0
         grads = [None] * (3 + nseg + nw + nb)
@@ -415,7 +421,7 @@ def _linear_ckpt(segments, spec, weights, biases, act, checkpoint):
         raise ValueError("linear takes at least one segment and at most one bias for each")
     if max(w for w, _ in spec) + 1 != len(weights) or min(w for w, _ in spec) < 0:
         raise ValueError("every weight belongs to a segment")
-    xs = [_rows_of(x if x.dtype in (torch.float32, torch.bfloat16) else x.to(torch.float32), "x")
+    xs = [_near(_rows_of(x if x.dtype in (torch.float32, torch.bfloat16) else x.to(torch.float32), "x"))
           for x, _, _ in segments]
     rows, device = xs[0].shape[0], xs[0].device
     n = weights[0].shape[0]

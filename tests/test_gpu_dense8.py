@@ -483,6 +483,24 @@ def test_checkpointed_layer_layouts():
     assert xg.grad is not None
 
 
+def test_rows_far_apart():
+    """Rows that are millions of values apart, of x and of the gradient."""
+    d = dense()
+    wide = torch.zeros((5, (1 << 21) + 9), device="cuda")
+    wide[:, 7:57] = make(5, 50, torch.float32, 1)
+    x, w = wide[:, 7:57], torch.randn((20, 50), generator=torch.Generator().manual_seed(2)).cuda().requires_grad_()
+    near_x = x.contiguous()
+    r, want = d.quantize_rows(x), d.quantize_rows(near_x)
+    assert torch.equal(r.q, want.q) and torch.equal(r.scale, want.scale)
+    w8 = d.quantize_weight(w)
+    assert torch.equal(d.linear8([x], [w8], []), d.linear8([near_x], [w8], []))
+    dy = torch.zeros((5, 1 << 21), device="cuda")[:, 3:23]
+    dy.copy_(make(5, 20, torch.float32, 3))
+    got = [d.linear([(v, 0, 0)], [w], [], None, checkpoint="int8") for v in (x, near_x)]
+    assert torch.equal(*got)
+    assert torch.equal(*[torch.autograd.grad(y, w, dy)[0] for y in got])
+
+
 def test_checkpointed_layer_no_rows_and_bad_rows():
     d = dense()
     xs, ws, bs, dy = leaves(0, 40, (30,), torch.float32)
@@ -614,13 +632,44 @@ def test_streams_and_graph_replay():
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_graph_replay_of_many_rows():
+    """The forms for many rows, captured and replayed with the program's own calls in between."""
+    d = dense()
+    rows, n, k = 33000, 130, 300
+    xs, ws, bs, dy = leaves(rows, n, (k,), torch.bfloat16, 4)
+    w8, v8 = d.quantize_weight(ws[0]), d.quantize_weight(torch.randn((n, n), device="cuda"))
+
+    def step(x):
+        x = x.detach().requires_grad_()
+        y = d.linear([(x, 0, 0)], ws, bs, "sigmoid", checkpoint="int8")
+        g = torch.autograd.grad(y, [x, *ws, *bs], dy)
+        with torch.no_grad():
+            h = d.linear8([x], [w8], [], "relu", out=torch.int8)
+            return [y.detach(), *g, h.q, h.scale, d.linear8([h], [v8], [], out=torch.bfloat16)]
+
+    sx = xs[0].detach().clone()
+    step(sx)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(sx)
+    for i in range(3):
+        sx.copy_(make(rows, k, torch.bfloat16, 60 + i))
+        graph.replay()
+        want = step(sx)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
 def test_repeats_are_equal():
     """No result depends on the order in which the device finishes."""
     d = dense()
-    xs, ws, bs, dy = leaves(5000, 200, (300,), torch.float32, 2)
+    xs, ws, bs, dy = leaves(40000, 200, (300,), torch.float32, 2)
     first = None
+    w8 = d.quantize_weight(ws[0])
     for _ in range(3):
         y = d.linear([(xs[0], 0, 0)], ws, bs, "relu", checkpoint="int8")
         got = [y.detach(), *torch.autograd.grad(y, [*xs, *ws, *bs], dy)]
+        r = d.linear8([xs[0].detach()], [w8], [], out=torch.int8)
+        got += [r.q, r.scale]
         first = first or got
         assert all(torch.equal(a, b) for a, b in zip(got, first))
