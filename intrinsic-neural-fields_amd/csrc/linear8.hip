@@ -307,16 +307,16 @@ __global__ __launch_bounds__(256) void linear8_few_kernel(Linear8Args a, const X
 //   k runs over KS blocks of 64.  Within a block, byte p of lane group g's 16 is k = G (4 p / G +
 //   g) + p % G with G = 16 bytes of x (4 fp32, 8 bf16, 16 int8 values): each load of 16 bytes then
 //   lies next to the neighbouring lane groups'.  The weight is laid out the same way on its way to
-//   LDS.  Behind k its bytes are zero.
+//   LDS, in the order of the lanes that read it: a KiB for 16 outputs and 64 k.  Behind k its bytes are zero.
 template <typename X> constexpr int granule() { return 16 / sizeof(X); }
 constexpr int WALK_WAVES = 8;  // (16 have 128 registers each, and spill)
 
 template <typename X, typename T, int KS, int TJ>
 struct LR {
   static constexpr int NW = WALK_WAVES;
-  static constexpr int THREADS = 64 * NW, WS = KS * 64 + 16;  // (16 bytes: rows start in other banks)
+  static constexpr int THREADS = 64 * NW;
   static constexpr int OS = TJ * 16 + 16;                     // a result row in 8 bits
-  static constexpr int WEIGHT = TJ * 16 * WS, SCALES = TJ * 16 * 8, OUT = sizeof(T) == 1 ? NW * 16 * OS : 0;
+  static constexpr int WEIGHT = TJ * KS * 1024, SCALES = TJ * 16 * 8, OUT = sizeof(T) == 1 ? NW * 16 * OS : 0;
   static constexpr int LDS = WEIGHT + SCALES + OUT;
   static_assert(LDS <= 160 * 1024, "LDS");
 };
@@ -340,11 +340,11 @@ __global__ __launch_bounds__(64 * WALK_WAVES) void linear8_rows_kernel(Linear8Ar
     for (int c = 0; c < 4; ++c)
       v[c] = b * 64 < a.ldw ? *reinterpret_cast<const i32x4*>(a.w + min(n, a.n - 1) * a.ldw + b * 64 + c * 16)
                             : i32x4{0, 0, 0, 0};
-    int* const to = reinterpret_cast<int*>(smem + n * P::WS + b * 64);
+    int* const to = reinterpret_cast<int*>(smem + (n / 16 * KS + b) * 1024 + n % 16 * 16);
 #pragma unroll
     for (int d = 0; d < 16; ++d) {
       const int g = d * 4 / G % 4, load = d * 4 / G / 4, at = d * 4 % G;  // whose, in which load, where
-      to[g * 4 + (load * G + at) / 4] = v[d / 4][d % 4];
+      to[g * 64 + (load * G + at) / 4] = v[d / 4][d % 4];
     }
   }
   for (int i = tid; i < TJ * 16; i += P::THREADS) {
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(64 * WALK_WAVES) void linear8_rows_kernel(Linear8Ar
 #pragma unroll
       for (int u = 0; u < GROUP; ++u) {
         const int j = g * GROUP % TJ + u, b = g * GROUP / TJ;
-        wf[g & 1][u] = *reinterpret_cast<const i32x4*>(smem + (16 * j + r16) * P::WS + b * 64 + g4 * 16);
+        wf[g & 1][u] = *reinterpret_cast<const i32x4*>(smem + (j * KS + b) * 1024 + lane * 16);
       }
     };
     load_group(0);
