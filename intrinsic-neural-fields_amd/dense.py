@@ -116,7 +116,8 @@ def linear(segments, weights, biases, act=None, checkpoint=None):
     where dW_s = dz^T (s q)_s; the output, dx_s and the bias gradients do not depend on it.
     A list names it for each segment: "int8", or the `Rows8` of that x_s where several layers
     read the same tensor.  Products are exact to fp32, as without it, in another order of
-    summation; a row with an infinity or a NaN gives NaN."""
+    summation; a row with an infinity or a NaN gives NaN.  (As with every layer here: a backward
+    is captured into a graph only while no eager graph of the same leaves is alive.)"""
     for t in [x for x, _, _ in segments] + list(weights) + list(biases):
         if not t.is_cuda:
             raise RuntimeError("the dense layers run on the HIP device only; there is no CPU fallback")
@@ -282,6 +283,8 @@ def linear8(xs, weights, biases, act=None, out=torch.float32):
             b = biases[s] if s < len(biases) else None
             if b is not None and (b.shape != (n,) or b.dtype != torch.float32 or not b.is_contiguous()):
                 raise ValueError("a bias is a contiguous fp32 [n] tensor")
+            if b is not None and b.requires_grad and torch.is_grad_enabled():
+                raise RuntimeError("linear8 has no gradient: call it under torch.no_grad(), or train with linear")
             if q.device != device or w.packed.device != device or (b is not None and b.device != device):
                 raise ValueError("linear8 takes its tensors on one device")
             oc = code if s == last else rt.DTYPE_F32

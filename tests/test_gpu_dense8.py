@@ -434,6 +434,52 @@ def test_checkpointed_layer_against_differences():
         assert abs((f(x, b + e) - f(x, b - e)) / (2 * h) - float(gb[j])) <= lim
 
 
+@pytest.mark.parametrize("rows", [70, 16400, 32771])
+@pytest.mark.parametrize("k", [90, 300])
+def test_wider_rows_of_results_stay(rows, k):
+    """Results as columns of wider buffers, through the C entries: what is around them stays."""
+    d = dense()
+    from inf_hip import DTYPE_F32, DTYPE_I8, lib, check
+    from inf_hip import runtime as rt
+    n = 100
+    x, qw_sw = make(rows, k, torch.float32, rows), weight8(n, k, 1)
+    w = d.pack_weight8(qw_sw[0].cuda(), qw_sw[1].cuda())
+    wf = (torch.randn((n, k), generator=torch.Generator().manual_seed(3)) * 0.1).cuda()
+
+    def work(size):
+        return torch.empty(max(int(size), 16), dtype=torch.uint8, device="cuda")
+
+    buf = torch.full((rows + 3, 128), 7.0, device="cuda")
+    ws = work(lib.inf_linear_int_workspace_bytes(rows, n, k, 0, 0))
+    check(lib.inf_linear_int(rows, n, k, rt.ptr(x), DTYPE_F32, k, None, rt.ptr(w.packed), rt.ptr(w.scale), None, None,
+                             0, 0, rt.ptr(buf), DTYPE_F32, 128, None, rt.ptr(ws), rt.stream_handle()))
+    assert torch.equal(buf[:rows, :n], d.linear8([x], [w], []))
+    assert (buf[rows:] == 7).all() and (buf[:, n:] == 7).all()
+    q8, s8 = torch.full((rows + 3, 128), 9, dtype=torch.int8, device="cuda"), torch.full((rows + 3,), 7.0, device="cuda")
+    ws = work(lib.inf_linear_int_workspace_bytes(rows, n, k, 0, 4))
+    check(lib.inf_linear_int(rows, n, k, rt.ptr(x), DTYPE_F32, k, None, rt.ptr(w.packed), rt.ptr(w.scale), None, None,
+                             0, 0, rt.ptr(q8), DTYPE_I8, 128, rt.ptr(s8), rt.ptr(ws), rt.stream_handle()))
+    want = d.linear8([x], [w], [], out=torch.int8)
+    assert torch.equal(q8[:rows, :n], want.q) and torch.equal(s8[:rows], want.scale)
+    assert (q8[rows:] == 9).all() and (s8[rows:] == 7).all() and (q8[:, 112:] == 9).all()
+    # the checkpointed layer: y, and dx into columns of a buffer of rows that do not start on 16 bytes
+    buf.fill_(7)
+    ws = work(lib.inf_linear_ckpt_workspace_bytes(rows, n, k, 0, 0))
+    check(lib.inf_linear_ckpt_forward(rows, n, k, rt.ptr(x), DTYPE_F32, k, rt.ptr(wf), k, 1, None, None, 0, 0,
+                                      rt.ptr(buf), 128, None, None, 0, None, rt.ptr(ws), rt.stream_handle()))
+    assert torch.equal(buf[:rows, :n], d.linear([(x, 0, 0)], [wf], [], None, checkpoint="int8"))
+    assert (buf[rows:] == 7).all() and (buf[:, n:] == 7).all()
+    dy = make(rows, n, torch.float32, 5)
+    wide = torch.full((rows + 3, k + 33), 7.0, device="cuda")
+    ws = work(lib.inf_linear_ckpt_workspace_bytes(rows, n, k, 0, 1))
+    check(lib.inf_linear_ckpt_backward(rows, n, k, rt.ptr(dy), n, 0, None, 0, None, None, 0, None, rt.ptr(wf), k, 1,
+                                       rt.ptr(wide), DTYPE_F32, k + 33, None, 0, None, rt.ptr(ws), rt.stream_handle()))
+    xg = x.clone().requires_grad_()
+    y = d.linear([(xg, 0, 0)], [wf], [], None, checkpoint="int8")
+    assert torch.equal(wide[:rows, :k], torch.autograd.grad(y, xg, dy)[0])
+    assert (wide[rows:] == 7).all() and (wide[:, k:] == 7).all()
+
+
 def test_checkpointed_layer_layouts():
     """One weight split by column ranges, columns no segment takes (gradient zero), strided and
     repeated inputs, a transposed weight, gradients of some inputs only, shared rows."""
@@ -568,6 +614,8 @@ def test_refusals():
         d.linear8([x], [w8], [], "tanh")
     with pytest.raises(RuntimeError, match="gradient"):
         d.linear8([x.clone().requires_grad_()], [w8], [])
+    with pytest.raises(RuntimeError, match="gradient"):
+        d.linear8([x], [w8], [b.clone().requires_grad_()])
     with pytest.raises(RuntimeError, match="HIP"):
         d.linear8([x.cpu()], [w8], [])
     for q, s in ((w, b), (w8.packed.view(-1)[:16], b), (torch.zeros((4, 16), dtype=torch.int8).cuda(), b[:3])):
