@@ -381,7 +381,11 @@ __global__ __launch_bounds__(64 * WALK_WAVES) void linear8_rows_kernel(Linear8Ar
         }
     }
   };
-  const bool relu = a.act == 1;
+  // ReLU in one operation: as whole numbers, negative values lie below zero and a NaN (of positive sign:
+  // every one here is) above.  Without it the bound is below everything (and unknown to the compiler,
+  // which else selects: an operation more, 47.5 and 45.8 us from 8 bits into 8 bits).
+  int least = a.act == 1 ? 0 : (int)0x80000000;
+  asm volatile("" : "+s"(least));
   int tile = (int)blockIdx.x * P::NW + wave;
   if (tile < tiles) fetch(tile);
   for (; tile < tiles; tile += step) {
@@ -465,9 +469,7 @@ __global__ __launch_bounds__(64 * WALK_WAVES) void linear8_rows_kernel(Linear8Ar
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         z[e] = combine(acc[j][e], sx, sw[e], bias[e]);
-        // as whole numbers, negative values lie below zero and a NaN (of positive sign: every one here
-        // is) above: one operation
-        if (relu) z[e] = __int_as_float(max(__float_as_int(z[e]), 0));
+        z[e] = __int_as_float(max(__float_as_int(z[e]), least));
       }
       if constexpr (sizeof(T) == 1) {
 #pragma unroll
