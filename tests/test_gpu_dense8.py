@@ -12,6 +12,8 @@ Tolerances.  u = 2^-24 is half a step of fp32, relative; U that of the output's 
     and divide cost 4 u more.
   checkpointed layer: a sum of K products in fp32, whatever its order: |error| <= (K + 8) u
     sum |a b|, the worst case of its additions; 8 covers operands rounded to 24 bits."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -706,6 +708,44 @@ def test_graph_replay_of_many_rows():
         want = step(sx)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_more_values_than_32_bits_count():
+    """Inputs of more than 2^31 values: the last rows are as they are alone (the checkpointed layer's, whose
+    forms for few and many rows sum in other orders, as in 64 bits), and the weight's gradient is exact.  x holds whole numbers up to 127 of 1 / 128, the largest in every row, so that q is they and s
+    is 1 / 128; one row in 257 has a gradient, of whole numbers up to 2: no sum passes 2^24."""
+    d = dense()
+    rows, k, n = (1 << 21) + 4099, 1031, 40
+    tail = slice(rows - 300, rows)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty((rows, k), dtype=torch.bfloat16, device="cuda")
+    for part in x.split(1 << 18):
+        part.copy_(torch.randint(-127, 128, part.shape, generator=g, device="cuda", dtype=torch.int8)).div_(128)
+    x[:, 0] = 127 / 128
+    assert x.numel() > 1 << 31
+    r, want = d.quantize_rows(x), d.quantize_rows(x[tail])
+    assert (r.scale == 1 / 128).all()
+    assert torch.equal(r.q[tail], want.q) and torch.equal(r.restore(torch.bfloat16)[tail], x[tail])
+    qw, sw = weight8(n, k, 1)
+    w8 = d.pack_weight8(qw.cuda(), sw.cuda())
+    for xin, x_tail in ((x, x[tail]), (r, want)):
+        assert torch.equal(d.linear8([xin], [w8], [], "relu")[tail], d.linear8([x_tail], [w8], [], "relu"))
+    c8 = d.pack_weight8(qw[:, :1000].contiguous().cuda(), sw.cuda())  # the form for up to 1024 values
+    assert torch.equal(d.linear8([x[:, :1000]], [c8], [])[tail], d.linear8([x[tail, :1000]], [c8], []))
+    del r, xin
+    some = torch.arange(rows - 1, -1, -257, device="cuda")
+    for cols in (n, 66):  # (66: the form that holds whole rows of dz)
+        w = (torch.randn((cols, k), generator=torch.Generator().manual_seed(cols)) * 0.1).cuda().requires_grad_()
+        dy = torch.zeros((rows, cols), device="cuda")
+        dy[some] = torch.randint(-2, 3, (len(some), cols), generator=g, device="cuda").float()
+        xg = x.detach().requires_grad_()
+        y = d.linear([(xg, 0, 0)], [w], [], None, checkpoint="int8")
+        dx, dw = torch.autograd.grad(y, [xg, w], dy)
+        want = layer64([x[tail]], [w], [], None, dy[tail])
+        near(y[tail], want["y"])
+        near(dx[tail], want["dx"][0], torch.bfloat16)
+        assert torch.equal(dw.cpu().double(), dy[some].cpu().double().t() @ x[some].cpu().double())
+        del y, dx, xg, dy
 
 
 def test_repeats_are_equal():
