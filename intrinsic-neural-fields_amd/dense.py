@@ -303,6 +303,12 @@ def linear8(xs, weights, biases, act=None, out=torch.float32):
     return y
 
 
+def _workspace(lib, rows, n, widths, backward, device):
+    """One for all segments of a layer: their launches follow each other."""
+    need = max([lib.inf_linear_ckpt_workspace_bytes(rows, n, k, 0, backward) for k in widths])
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
 class _LinearCkpt(torch.autograd.Function):
     @staticmethod
     def forward(ctx, spec, act, kept, *tensors):
@@ -332,6 +338,7 @@ class _LinearCkpt(torch.autograd.Function):
             yp = y.data_ptr()
             held = torch.empty(at, dtype=torch.uint8, device=device) if at else None
             base = held.data_ptr() if at else 0
+            work = _workspace(lib, rows, n, [x.shape[1] for x in tensors[:nseg]], 0, device)
             for s, (wi, c0) in enumerate(spec):
                 x, W = tensors[s], tensors[nseg + wi]
                 k, last, own = x.shape[1], s == nseg - 1, kept[s]
@@ -343,8 +350,6 @@ class _LinearCkpt(torch.autograd.Function):
                 elif own is not None:
                     scale = own.scale.data_ptr()
                 xc = rt.dtype_code(x)
-                work = torch.empty(lib.inf_linear_ckpt_workspace_bytes(rows, n, k, xc, 0), dtype=torch.uint8,
-                                   device=device)
                 rt.check(lib.inf_linear_ckpt_forward(
                     rows, n, k, x.data_ptr(), xc, x.stride(0), W.data_ptr() + 4 * c0 * W.stride(1), W.stride(0),
                     W.stride(1), tensors[nseg + nw + s].data_ptr() if s < nb else None, yp if s else None, n,
@@ -381,6 +386,7 @@ class _LinearCkpt(torch.autograd.Function):
         grads = [None] * (3 + nseg + nw + nb)
         with _on(device):
             st = _stream(device)
+            work = _workspace(lib, rows, n, widths, 1, device)
             for s, (wi, c0) in enumerate(spec):
                 W, k = ws[wi], widths[s]
                 ldq = _round_up(k, 16)
@@ -406,8 +412,6 @@ class _LinearCkpt(torch.autograd.Function):
                 if dx is None and dw is None and db is None:
                     continue
                 xc = rt.dtype_code(dx) if dx is not None else rt.DTYPE_F32
-                work = torch.empty(lib.inf_linear_ckpt_workspace_bytes(rows, n, k, xc, 1), dtype=torch.uint8,
-                                   device=device)
                 rt.check(lib.inf_linear_ckpt_backward(
                     rows, n, k, dy.data_ptr(), dy.stride(0), act, _at(y), n,
                     base + mask_at if mask_at is not None else None, q, ldq, scale,
