@@ -992,13 +992,14 @@ struct DwShape {
   int64_t rows_a_split;
 };
 
-// as many splits as give each CU a workgroup, of eight turns at least
+// As many splits as give each CU a workgroup, of two turns at least: with add_slabs_kernel 14 us for
+// 512 x 256 x 256 and 12 for 4096 x 64 x 64 (of eight turns: 21 and 19).
 DwShape dw_shape(int64_t rows, int n, int k) {
   DwShape d;
   d.tiles_k = (int)ceil_div(k, DW_K);
   d.tiles = d.tiles_k * (int)ceil_div(n, DW_N);
   const int64_t turns = std::max<int64_t>(ceil_div(rows, 32), 1);
-  const int64_t splits = std::min<int64_t>(std::max<int64_t>(256 / d.tiles, 1), ceil_div(turns, 8));
+  const int64_t splits = std::min<int64_t>(std::max<int64_t>(256 / d.tiles, 1), ceil_div(turns, 2));
   d.rows_a_split = ceil_div(turns, splits) * 32;
   d.splits = (int)std::max<int64_t>(ceil_div(rows, d.rows_a_split), 1);
   return d;
