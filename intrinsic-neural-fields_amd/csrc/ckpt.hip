@@ -921,9 +921,10 @@ int launch_tile(const SideArgs& a, hipStream_t stream) {
   return INF_OK;
 }
 
-// The widest tile that still fills the CUs.  65,536 x 1024 x 256: forward 108 us with 256 x 256
-// (one of 16 waves a CU), 128 with 128 x 128 (two of 8); dx, whose results are many, 163 with 128 x
-// 128, where one's stores run beside the other's products, 172 with 256 x 128.
+// The widest tile that still gives each CU a workgroup.  65,536 x 1024 x 256: forward 108 us with 256 x
+// 256 (one of 16 waves a CU), 128 with 128 x 128 (two of 8); dx, whose results are many, 163 with 128 x
+// 128, where one's stores run beside the other's products, 172 with 256 x 128.  16,384 x 1024 x 256
+// forward: 34 with 128 x 128, 42 with 64 x 64; 8192 rows, half as many tiles as CUs, 31 and 26.
 template <int MODE, int ACT, typename X, typename T>
 int launch_tiles(const SideArgs& a, hipStream_t stream) {
   const int64_t wide = ceil_div(a.rows, 256);
@@ -931,7 +932,7 @@ int launch_tiles(const SideArgs& a, hipStream_t stream) {
   if constexpr (MODE == 0)
     if (a.cols > 128 && wide * ceil_div(a.cols, 256) >= 256)
       return launch_tile<MODE, ACT, X, T, 256, 256, 4, 4>(a, stream);
-  if (ceil_div(a.rows, 128) * ceil_div(a.cols, 128) >= 512) return launch_tile<MODE, ACT, X, T, 128, 128, 4, 2>(a, stream);
+  if (ceil_div(a.rows, 128) * ceil_div(a.cols, 128) >= 256) return launch_tile<MODE, ACT, X, T, 128, 128, 4, 2>(a, stream);
   return launch_tile<MODE, ACT, X, T, 64, 64, 2, 2>(a, stream);
 }
 

@@ -798,13 +798,16 @@ int launch_tile(const Linear8Args& a, hipStream_t stream) {
 }
 
 // The widest tile that still gives every CU a workgroup (256 of them); a result in 8 bits
-// needs whole rows (n <= 256).
+// needs whole rows (n <= 256).  4096 x 4096 x 2048, us: 128 x 128 43, 64 x 64 60, 256 x 256 (half the
+// CUs) 59; 2048 x 4096 x 1024: 128 x 128 (half the CUs) 27, 64 x 64 21.
 template <typename T>
 int launch_tiles(const Linear8Args& a, hipStream_t stream) {
   const int64_t wide = ceil_div(a.rows, 256);
   if (a.n <= 32) return launch_tile<T, 256, 32, 4, 1>(a, stream);
   if (a.n <= 128 && wide >= 256) return launch_tile<T, 256, 128, 8, 2>(a, stream);
   if (a.n > 128 && wide * ceil_div(a.n, 256) >= 256) return launch_tile<T, 256, 256, 4, 4>(a, stream);
+  if constexpr (sizeof(T) != 1)
+    if (a.n > 64 && ceil_div(a.rows, 128) * ceil_div(a.n, 128) >= 256) return launch_tile<T, 128, 128, 4, 2>(a, stream);
   if (sizeof(T) == 1 && a.n > 64) return launch_tile<T, 64, 256, 1, 4>(a, stream);
   return launch_tile<T, 64, 64, 2, 2>(a, stream);
 }

@@ -167,7 +167,8 @@ SIZES = [(1, 1, 1), (1, 3, 1024), (1, 256, 1024), (2, 17, 63), (5, 256, 1023), (
          (17, 3, 256), (33, 130, 100), (64, 64, 4096), (65, 257, 300), (127, 96, 127), (128, 128, 128),
          (300, 256, 256), (257, 511, 193), (1000, 3, 16), (520, 1030, 65), (1, 4096, 2048), (8, 4097, 33),
          (16390, 256, 256), (16400, 100, 77), (17001, 129, 200), (16384, 255, 3), (16385, 64, 128),
-         (32769, 256, 1023), (32790, 40, 300), (32770, 3, 513), (32831, 129, 512), (32768, 253, 769)]
+         (32769, 256, 1023), (32790, 40, 300), (32770, 3, 513), (32831, 129, 512), (32768, 253, 769),
+         (2049, 2040, 100), (4095, 1025, 260)]
 
 
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
@@ -366,7 +367,8 @@ def leaves(rows, n, widths, dtype, seed=0):
 LAYERS = [(1, 1, (1,)), (1, 3, (5,)), (2, 33, (31,)), (64, 64, (64,)), (100, 3, (256,)), (65, 130, (63,)),
           (300, 256, (1023,)), (512, 256, (256,)), (129, 257, (255,)), (1000, 128, (3,)), (257, 64, (100, 40)),
           (600, 256, (256, 1024)), (3000, 96, (64,)), (77, 512, (512,)),
-          (32769, 256, (256,)), (32800, 66, (257, 300)), (33000, 130, (1,)), (32768, 200, (511,))]
+          (32769, 256, (256,)), (32800, 66, (257, 300)), (33000, 130, (1,)), (32768, 200, (511,)),
+          (16001, 257, (255,)), (8200, 300, (400,))]
 
 
 @pytest.mark.parametrize("act", [None, "relu", "sigmoid"])
