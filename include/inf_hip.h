@@ -213,7 +213,7 @@ int inf_pack_weight(const int8_t* q, int64_t stride_n, int64_t stride_k, int n, 
                     inf_stream_t stream);
 /* out = act(fl(fl(acc) fl(x_scale[m] w_scale[n])) + bias[n] + add[m][n]), acc the exact sum
  * of the 8-bit products (k <= 2^17), each operation rounded once to fp32; bias and add may
- * be NULL.  x: fp32 / bf16 (put into 8 bits first, in the workspace), or INF_DTYPE_I8 rows
+ * be NULL.  x: fp32 / bf16 (put into 8 bits on the way), or INF_DTYPE_I8 rows
  * with x_scale, behind whose last row 128 bytes may be read (their values do not matter).
  * out: fp32 / bf16, or INF_DTYPE_I8 rows with out_scale (inf_quantize_rows of the result).
  * act 0 none, 1 ReLU, 2 sigmoid.  workspace: inf_linear_int_workspace_bytes bytes.        */

@@ -188,9 +188,9 @@ __global__ __launch_bounds__(256) void before_dx_kernel(Weight w, int nw, Dz d, 
 // ---- x W^T and dz W -----------------------------------------------------------------------
 // out(m, c) = sum_k side(m, k) V(c, k): BM rows by BN columns a workgroup, WM x WN waves,
 // v_mfma_f32_16x16x32_f16 with V as its first operand (a lane holds four neighbouring
-// columns of one row).  Per turn 32 k.  LDS: two stages of 128-byte rows (64 hi, 64 lo), V's
-// filled straight from memory one turn ahead.  The rows of x or dz are read in whole lines
-// into registers two turns ahead and split on their way to LDS, each value once.
+// columns of one row).  Per turn 32 k.  LDS: two stages, V's images as they are, filled straight from
+// memory one turn ahead, and 128-byte rows of the side (64 hi, 64 lo).  The rows of x or dz are
+// read in whole lines into registers a turn ahead and split on their way to LDS, each value once.
 struct SideArgs {
   int64_t rows;
   int cols, K;          // output columns; length of the sums
@@ -306,8 +306,8 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
   const int wr = wave / WN, wc = wave % WN, r16 = lane & 15, g4 = lane >> 4;
   const int turns = (a.K + 31) / 32;
 
-  // (offsets of 32 bits from uniform bases: with 128 registers a lane each address counts)
-  // (rows of V behind the last are in the workspace, whatever they hold: their columns are not stored)
+  // Offsets of 32 bits from uniform bases: with 128 registers a lane each address counts.  Rows of V
+  // behind the last are in the workspace, whatever they hold: their columns are not stored.
   const int blocks = blocks_of_32(a.K);
   auto issue = [&](int t, int stage) {
     char* st = smem + (stage & 1) * P::STAGE;
