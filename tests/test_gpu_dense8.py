@@ -10,8 +10,12 @@ Tolerances.  u = 2^-24 is half a step of fp32, relative; U that of the output's 
     sx and sw have one rounding each, which the oracle takes over (it reads the scales).
     A ReLU does not enlarge an error; a sigmoid's slope is at most 1/4, and its exp, add
     and divide cost 4 u more.
-  checkpointed layer: a sum of K products in fp32, whatever its order: |error| <= (K + 8) u
-    sum |a b|, the worst case of its additions; 8 covers operands rounded to 24 bits."""
+  checkpointed layer: fp32 values enter the products as two fp16 pieces.  hi is off by half a step, 2^-11 of
+    the value, lo by 2^-11 of that and at most half of it again (a value just above a power of two has the
+    largest hi error, whose lo then lies in the upper half of its own power of two): 2^-23 a value.  lo lo, at
+    most 2^-22, is left out.  A product is off by 2^-23 + 2^-23 + 2^-22 = 8 u, and its three parts are three
+    additions of u each of the partial sums, whatever their order: |error| <= (3 K + 8) u sum |a b|.  dW: one
+    operand is exact, the other has one rounding (u) and three exact pieces: the same bound covers it."""
 import math
 
 import numpy as np
@@ -315,7 +319,7 @@ def layer64(xs, ws, bs, act, dy, c0s=None):
         k_all += x.shape[1]
     dy = dy.cpu().double()
     y = act64(z, act)
-    ey = (k_all + 8) * U32 * zm
+    ey = (3 * k_all + 8) * U32 * zm
     if act == "relu":
         dz, edz = dy * (z > 0), 0.0
     elif act == "sigmoid":
@@ -328,11 +332,11 @@ def layer64(xs, ws, bs, act, dy, c0s=None):
     out = {"y": (y, ey), "dx": [], "dw": [], "db": (dz.sum(0), (rows + 8) * U32 * dz.abs().sum(0)
                                                      + (edz.sum(0) if act == "sigmoid" else 0))}
     for x, w in zip(xs, w64):
-        e = (n + 8) * U32 * (dz.abs() @ w.abs()) + (edz @ w.abs() if act == "sigmoid" else 0)
+        e = (3 * n + 8) * U32 * (dz.abs() @ w.abs()) + (edz @ w.abs() if act == "sigmoid" else 0)
         out["dx"].append((dz @ w, e))
         q, s = rows64(x.detach())
         v = q * s[:, None]
-        e = (rows + 8) * U32 * (dz.abs().t() @ v.abs()) + (edz.t() @ v.abs() if act == "sigmoid" else 0)
+        e = (3 * rows + 8) * U32 * (dz.abs().t() @ v.abs()) + (edz.t() @ v.abs() if act == "sigmoid" else 0)
         out["dw"].append((dz.t() @ v, e))
     return out
 
@@ -352,7 +356,7 @@ def relu_safe(xs, ws, bs, dy):
         b = bs[i].detach().cpu().double() if i < len(bs) else torch.zeros(w.shape[0]).double()
         z, zm = z + x @ w.t() + b, zm + x.abs() @ w.abs().t() + b.abs()
     k = sum(x.shape[1] for x in xs)
-    return torch.where((z.abs() <= (k + 8) * U32 * zm).cuda(), torch.zeros_like(dy), dy)
+    return torch.where((z.abs() <= (3 * k + 8) * U32 * zm).cuda(), torch.zeros_like(dy), dy)
 
 
 def leaves(rows, n, widths, dtype, seed=0):
@@ -390,6 +394,26 @@ def test_checkpointed_layer(rows, n, widths, dtype, act):
     for b in bs:
         near(b.grad, want["db"])
     assert len({b.grad.data_ptr() for b in bs}) == len(bs)
+
+
+def test_checkpointed_layer_single_products():
+    """Sums of one product, whose bound is the pieces' own: values with the largest low pieces."""
+    d = dense()
+    g = torch.Generator().manual_seed(4)
+
+    def worst(n):  # 2^e (1 + m 2^-10 + 2^-11 +- a little): in the middle between two fp16 values
+        m = torch.randint(0, 16, (n,), generator=g).double()
+        off = torch.randint(-3, 4, (n,), generator=g).double() * 2.0 ** -22
+        e = torch.randint(-20, 20, (n,), generator=g).double()
+        return ((1 + m * 2.0 ** -10 + 2.0 ** -11 + off) * 2.0 ** e).float()
+
+    x, w = worst(500)[:, None].cuda(), worst(300)[:, None].cuda()
+    y = d.linear([(x, 0, 0)], [w], [], None, checkpoint="int8")
+    near(y, layer64([x], [w], [], None, torch.zeros((500, 300)))["y"])
+    w, dy = worst(700)[None, :].cuda(), worst(400)[:, None].cuda()  # dx of one output
+    xs = torch.zeros((400, 700), device="cuda").requires_grad_()
+    y = d.linear([(xs, 0, 0)], [w], [], None, checkpoint="int8")
+    near(torch.autograd.grad(y, xs, dy)[0], layer64([xs], [w], [], None, dy)["dx"][0])
 
 
 def test_checkpointed_layer_matches_the_exact_one():
