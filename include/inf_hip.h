@@ -221,9 +221,9 @@ int64_t inf_linear_int_workspace_bytes(int64_t rows, int n, int k, int x_dtype, 
 int inf_linear_int(int64_t rows, int n, int k, const void* x, int x_dtype, int64_t ld_x, const float* x_scale,
                    const int8_t* w, const float* w_scale, const float* bias, const float* add, int64_t ld_add, int act,
                    void* out, int out_dtype, int64_t ld_out, float* out_scale, void* workspace, inf_stream_t stream);
-/* Linear layer that keeps its input in 8 bits: y = act(x W^T + bias + add) in fp32 (each product
- * within 2^-21) from x (fp32 / bf16) as it is, W(n, k) = W[n stride_wn + k stride_wk]; bias and add may be NULL,
- * add may be y.  q and scale: the rows of x in 8 bits, written; scale alone: x's own scales,
+/* Linear layer that keeps its input in 8 bits: y = act(x W^T + bias + add) from x (fp32 / bf16) as
+ * it is, W(n, k) = W[n stride_wn + k stride_wk]; a value counts to 2^-23 of itself or 2^-39 of its
+ * row's largest, a product to 2^-21, sums are fp32.  bias and add may be NULL, add may be y.  q and scale: the rows of x in 8 bits, written; scale alone: x's own scales,
  * read (q made before); both NULL: nothing is kept.  mask (not NULL): bit j of
  * word w of row m (ceil(n / 32) words a row) = y[m][32 w + j] > 0.  workspace:
  * inf_linear_ckpt_workspace_bytes(.., 0) bytes.  n k below 2^29 (n and k padded to 256), rows

@@ -7,11 +7,11 @@
 // Products of fp32 on the 16-bit matrix instructions.
 //   x W^T and dz W: each row of either side is scaled by a power of two so that its largest
 //   value lies in [2^14, 2^15), and a value is two fp16 pieces, hi = fp16(v), lo = fp16(v - hi), which
-//   leave 2^-23 of it at most (2^-40 of the row's largest for the smallest ones, whose lo is
-//   subnormal).  hi hi + hi lo + lo hi, summed in fp32; lo lo, at most 2^-22 of the product, is left
-//   out: a product is within 2^-21, where fp32 has 2^-24.  (Its matrix instruction would be a
-//   fourth beside three.)  A bf16 x is one piece: two products.  The powers of two leave the result
-//   exactly.
+//   leave at most 2^-23 of it, or 2^-39 of the row's largest where that is more (a subnormal lo).
+//   hi hi + hi lo + lo hi, summed in fp32; lo lo, at most 2^-22 of the product, is left out: a product
+//   is within 2^-21, where fp32 has 2^-24, of values that are not 2^-16 of their row's largest.
+//   (lo lo would be a fourth matrix instruction beside three.)  A bf16 x is one piece, exact down to
+//   2^-31 of the row's largest: two products.  The powers of two leave the result exactly.
 //   dW: q is exact in bf16 and dz s is three bf16 pieces, all 24 bits of it: three products, no
 //   scale (a column of dz has no scale that a sum over its rows could be divided by).
 // A value that is not finite makes NaN of the rows (and columns) that it enters.

@@ -115,8 +115,9 @@ def linear(segments, weights, biases, act=None, checkpoint=None):
     checkpoint="int8": x_s (fp32, or bf16 taken as it is) is kept in 8 bits for the backward,
     where dW_s = dz^T (s q)_s; the output, dx_s and the bias gradients do not depend on it.
     A list names it for each segment: "int8", or the `Rows8` of that x_s where several layers
-    read the same tensor.  A product of two values is within 2^-21 (fp32: 2^-24), their sums are
-    fp32 in another order than without it; a row with an infinity or a NaN gives NaN.  (As with every layer here: a backward
+    read the same tensor.  Its products are not quite fp32's: a value counts to 2^-23 of itself, or
+    to 2^-39 of the largest of its row (of x and dz; of W, its row forward, its column for dx) where
+    that is more, a product to 2^-21; their sums are fp32, in another order; a row with an infinity or a NaN gives NaN.  (As with every layer here: a backward
     is captured into a graph only while no eager graph of the same leaves is alive.)"""
     for t in [x for x, _, _ in segments] + list(weights) + list(biases):
         if not t.is_cuda:

@@ -14,8 +14,10 @@ Tolerances.  u = 2^-24 is half a step of fp32, relative; U that of the output's 
     the value, lo by 2^-11 of that and at most half of it again (a value just above a power of two has the
     largest hi error, whose lo then lies in the upper half of its own power of two): 2^-23 a value.  lo lo, at
     most 2^-22, is left out.  A product is off by 2^-23 + 2^-23 + 2^-22 = 8 u, and its three parts are three
-    additions of u each of the partial sums, whatever their order: |error| <= (3 K + 8) u sum |a b|.  dW: one
-    operand is exact, the other has one rounding (u) and three exact pieces: the same bound covers it."""
+    additions of u each of the partial sums, whatever their order: |error| <= (3 K + 8) u sum |a b|.  Of a
+    value far below its row's largest, which is scaled to 2^14 at least, lo is a multiple of 2^-24: off by
+    2^-25, 2^-39 of the largest: another 2^-39 (max |a| sum |b| + sum |a| max |b|).  dW: one operand is exact,
+    the other has one rounding (u) and three exact pieces: the first bound covers it."""
 import math
 
 import numpy as np
@@ -307,19 +309,26 @@ def test_linear8_leaves_what_is_not_its_own():
 
 # ---- the layer with 8-bit checkpoints -------------------------------------------------
 
+def far_below(a, b):
+    """2^-39 (max |a| sum |b| + sum |a| max |b|) for each row of a with each column of b."""
+    a, b = a.abs(), b.abs()
+    return 2.0 ** -39 * (a.amax(1)[:, None] * b.sum(0)[None] + a.sum(1)[:, None] * b.amax(0)[None])
+
+
 def layer64(xs, ws, bs, act, dy, c0s=None):
     """Output, gradients and their worst-case fp32 bounds."""
-    z, zm, k_all = 0.0, 0.0, 0
+    z, zm, ez, k_all = 0.0, 0.0, 0.0, 0
     x64 = [x.detach().cpu().double() for x in xs]
     w64 = [w.detach().cpu().double() for w in ws]
     for i, (x, w) in enumerate(zip(x64, w64)):
         b = bs[i].detach().cpu().double() if i < len(bs) else torch.zeros(w.shape[0]).double()
         z = z + x @ w.t() + b
         zm = zm + x.abs() @ w.abs().t() + b.abs()
+        ez = ez + far_below(x, w.t())
         k_all += x.shape[1]
     dy = dy.cpu().double()
     y = act64(z, act)
-    ey = (3 * k_all + 8) * U32 * zm
+    ey = (3 * k_all + 8) * U32 * zm + ez
     if act == "relu":
         dz, edz = dy * (z > 0), 0.0
     elif act == "sigmoid":
@@ -332,7 +341,7 @@ def layer64(xs, ws, bs, act, dy, c0s=None):
     out = {"y": (y, ey), "dx": [], "dw": [], "db": (dz.sum(0), (rows + 8) * U32 * dz.abs().sum(0)
                                                      + (edz.sum(0) if act == "sigmoid" else 0))}
     for x, w in zip(xs, w64):
-        e = (3 * n + 8) * U32 * (dz.abs() @ w.abs()) + (edz @ w.abs() if act == "sigmoid" else 0)
+        e = (3 * n + 8) * U32 * (dz.abs() @ w.abs()) + far_below(dz, w) + (edz @ w.abs() if act == "sigmoid" else 0)
         out["dx"].append((dz @ w, e))
         q, s = rows64(x.detach())
         v = q * s[:, None]
@@ -414,6 +423,11 @@ def test_checkpointed_layer_single_products():
     xs = torch.zeros((400, 700), device="cuda").requires_grad_()
     y = d.linear([(xs, 0, 0)], [w], [], None, checkpoint="int8")
     near(torch.autograd.grad(y, xs, dy)[0], layer64([xs], [w], [], None, dy)["dx"][0])
+    # a small value next to a large one that meets a zero
+    x = torch.stack([torch.full((60,), 1e3), torch.logspace(-8, 3, 60)], 1).cuda()
+    w = torch.tensor([[0.0, 1.0], [0.0, 0.37], [1e-9, 1e-3]], device="cuda")
+    y = d.linear([(x, 0, 0)], [w], [], None, checkpoint="int8")
+    near(y, layer64([x], [w], [], None, torch.zeros((60, 3)))["y"])
 
 
 def test_checkpointed_layer_matches_the_exact_one():
