@@ -598,7 +598,7 @@ __global__ __launch_bounds__(64 * LONG_WAVES) void linear8_long_kernel(Linear8Ar
     for (int b = 0; b < P::BLOCKS; ++b)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        w[b][h] = b < blocks ? *reinterpret_cast<const i32x4*>(from + b * 128 + h * 64) : i32x4{0, 0, 0, 0};
+        w[b][h] = busy && b < blocks ? *reinterpret_cast<const i32x4*>(from + b * 128 + h * 64) : i32x4{0, 0, 0, 0};
   }
 
   // A chunk across the end of a row is loaded from its last V values and moved down when it is used
