@@ -722,6 +722,36 @@ def test_streams_and_graph_replay():
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_two_streams_at_once():
+    """Calls of every form on two streams, neither waiting for the other, as one after the other."""
+    d = dense()
+    sets = []
+    for i, (rows, n, k) in enumerate(((33000, 200, 300), (20000, 256, 256), (5, 64, 700), (9000, 300, 400))):
+        xs, ws, bs, dy = leaves(rows, n, (k,), torch.float32, i)
+        sets.append((xs[0], ws[0], bs[0], dy, d.quantize_weight(ws[0])))
+
+    def calls(s):
+        x, w, b, dy, w8 = s
+        y = d.linear([(x, 0, 0)], [w], [b], "sigmoid", checkpoint="int8")
+        g = torch.autograd.grad(y, [x, w, b], dy)
+        with torch.no_grad():
+            r = d.linear8([x], [w8], [b], "relu", out=torch.int8)
+            return [y.detach(), *g, r.q, r.scale, d.linear8([r], [d.quantize_weight(w.t())], [])]
+
+    want = [calls(s) for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    got = {}
+    for i in range(len(sets)):
+        for j, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i, j] = calls(sets[(i + j) % len(sets)])
+    torch.cuda.synchronize()
+    for (i, j), out in got.items():
+        assert all(torch.equal(a, b) for a, b in zip(out, want[(i + j) % len(sets)]))
+
+
 def test_graph_replay_of_many_rows():
     """The forms for many rows, captured and replayed with the program's own calls in between."""
     d = dense()
