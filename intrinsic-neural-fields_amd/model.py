@@ -20,6 +20,7 @@ default, or "bf16" MFMA with fp32 accumulation), overridable by INF_MODE.
 from __future__ import annotations
 
 import contextlib
+import contextvars
 import os
 import weakref
 
@@ -355,6 +356,17 @@ class _TextureFieldFn(torch.autograd.Function):
         return (None, None, None, None, None, *out)
 
 
+class _LaidOut:
+    __slots__ = ("model", "launches_to", "weights")
+
+    def __init__(self, model, launches_to, weights):
+        self.model, self.launches_to, self.weights = model, launches_to, weights
+
+
+# the weights_laid_out contexts that this thread is in, the last entered first
+_LAID_OUT = contextvars.ContextVar("weights_laid_out", default=())
+
+
 class TextureFieldWithViewDependency(nn.Module):
     """Reference model.py:115-191: a TextureField with a ReLU bottleneck output, the
     viewing direction (its angle to the hit face's normal, "intrinsic", or the direction
@@ -383,7 +395,6 @@ class TextureFieldWithViewDependency(nn.Module):
                                              activation(), nn.Linear(directional_hidden_dim, RGB_COLOR_DIM),
                                              nn.Sigmoid())
         self.dense_inference = None   # None or "int8": the layers where no gradient is recorded
-        self._weights8 = None
 
     def set_dense_options(self, checkpoints=None, inference=None):
         """checkpoints="int8": inputs kept in 8 bits until the backward (dense.linear);
@@ -397,14 +408,34 @@ class TextureFieldWithViewDependency(nn.Module):
     @contextlib.contextmanager
     def weights_laid_out(self):
         """With dense_inference="int8", the weights put into 8 bits once for the calls inside (a
-        frame's chunks) instead of once a call.  They must not change meanwhile."""
-        before = self._weights8
+        frame's chunks) instead of once a call.  They must not change meanwhile.  They are this
+        caller's alone: calls from another thread, on another stream or into another graph than
+        those that it was entered in put the weights into 8 bits for themselves."""
+        mine = None
+        if self.dense_inference == "int8":
+            mine = _LaidOut(self, self._launches_to(), self._make_weights8())
+            _LAID_OUT.set((mine, *_LAID_OUT.get()))
         try:
-            if self.dense_inference == "int8":
-                self._weights8 = self._make_weights8()
             yield self
         finally:
-            self._weights8 = before
+            if mine is not None:
+                mine.weights = None  # wherever this is left, nobody finds them again
+                _LAID_OUT.set(tuple(e for e in _LAID_OUT.get() if e is not mine))
+
+    def _launches_to(self):
+        """Device, stream and capture of the launches that a call makes now."""
+        device = next(self.parameters()).device
+        if device.type != "cuda":
+            return device
+        return device, torch.cuda.current_stream(device).cuda_stream, torch.cuda.is_current_stream_capturing()
+
+    @property
+    def _weights8(self):
+        """What this caller's weights_laid_out holds for a call made now, or None."""
+        for e in _LAID_OUT.get():
+            if e.model is self and e.weights is not None and e.launches_to == self._launches_to():
+                return e.weights
+        return None
 
     def _make_weights8(self):
         import dense
