@@ -164,7 +164,8 @@ def _rows_of(x, what):
 
 def _near(x):
     """x with rows less than 2^21 values apart, as the checkpointed layer's products take them."""
-    return x if x.stride(0) < 1 << 21 else x.contiguous()
+    # (of one row or none contiguous() is x itself, whatever the distance)
+    return x if x.stride(0) < 1 << 21 else x.clone(memory_format=torch.contiguous_format)
 
 
 class Rows8:
