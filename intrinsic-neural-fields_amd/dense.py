@@ -24,6 +24,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 ACT = {None: 0, "relu": 1, "sigmoid": 2}
@@ -168,6 +169,11 @@ def _near(x):
     return x if x.stride(0) < 1 << 21 else x.clone(memory_format=torch.contiguous_format)
 
 
+def _has_tangent(x):
+    """x is a dual tensor: forward-mode differentiation (also under no_grad) asks for its derivative."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None
+
+
 class Rows8:
     """The rows of a matrix in 8 bits: `q` int8 [rows, k] (rows start on 16 bytes) and
     `scale` fp32 [rows], standing for scale[:, None] * q.  Made by quantize_rows and linear8."""
@@ -205,9 +211,12 @@ class Rows8:
 def quantize_rows(x):
     """x [rows, k] fp32 / bf16 in 8 bits: scale = max|x| / 127 of each row, q the whole number
     nearest to 127 x / max|x| (ties to even).  Rows of zeros have scale 0; a row with an
-    infinity or a NaN has scale NaN, and whatever is made of it is NaN.  No gradient."""
+    infinity or a NaN has scale NaN, and whatever is made of it is NaN.  No gradient: x counts
+    as detached, and a dual tensor of forward-mode differentiation is refused."""
     rt = _rt()
     rt.require_hip(x)
+    if _has_tangent(x):
+        raise RuntimeError("8-bit rows have no derivative: quantize_rows takes no dual tensor")
     x = _rows_of(x.detach(), "x")
     rows, k = x.shape
     r = Rows8(rows, k, x.device)
@@ -247,7 +256,7 @@ def quantize_weight(W, col0=0, cols=None):
     cols = W.shape[1] - col0 if cols is None else cols
     if col0 < 0 or cols < 1 or col0 + cols > W.shape[1]:
         raise ValueError(f"columns {col0}..{col0 + cols} of a weight with {W.shape[1]}")
-    r = quantize_rows(W.detach()[:, col0:col0 + cols])
+    r = quantize_rows(W[:, col0:col0 + cols])
     return pack_weight8(r.q, r.scale)
 
 
@@ -258,7 +267,7 @@ def linear8(xs, weights, biases, act=None, out=torch.float32):
     xs: for each segment a matrix fp32 / bf16 (put into 8 bits on the way) or a Rows8;
     weights: a Weight8 each; biases: fp32 [n], one for each of the first segments.
     out: torch.float32, torch.bfloat16, or torch.int8 for a Rows8 of the result.
-    For rendering: it has no gradient, and refuses inputs that ask for one."""
+    For rendering: it has no gradient, and refuses inputs that ask for one, in forward mode too."""
     rt = _rt()
     i8 = rt.DTYPE_I8
     code = i8 if out is torch.int8 else rt.DTYPE_F32 if out is torch.float32 else \
@@ -276,7 +285,7 @@ def linear8(xs, weights, biases, act=None, out=torch.float32):
             if isinstance(x, Rows8):
                 q, scale, xc = x.q, x.scale.data_ptr(), i8
             else:
-                if x.requires_grad and torch.is_grad_enabled():
+                if (x.requires_grad and torch.is_grad_enabled()) or _has_tangent(x):
                     raise RuntimeError("linear8 has no gradient: call it under torch.no_grad(), or train with linear")
                 q, scale = _rows_of(x, "x"), None
                 xc = rt.dtype_code(q)
@@ -285,7 +294,7 @@ def linear8(xs, weights, biases, act=None, out=torch.float32):
             b = biases[s] if s < len(biases) else None
             if b is not None and (b.shape != (n,) or b.dtype != torch.float32 or not b.is_contiguous()):
                 raise ValueError("a bias is a contiguous fp32 [n] tensor")
-            if b is not None and b.requires_grad and torch.is_grad_enabled():
+            if b is not None and ((b.requires_grad and torch.is_grad_enabled()) or _has_tangent(b)):
                 raise RuntimeError("linear8 has no gradient: call it under torch.no_grad(), or train with linear")
             if q.device != device or w.packed.device != device or (b is not None and b.device != device):
                 raise ValueError("linear8 takes its tensors on one device")

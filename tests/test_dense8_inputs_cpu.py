@@ -16,3 +16,16 @@ def test_rows_far_apart_are_copied_whatever_their_number(rows):
     x.requires_grad_()
     near = dense._near(x)
     assert torch.equal(torch.autograd.grad(near, x, torch.ones_like(near))[0], torch.ones(rows, 8))
+
+
+def test_dual_tensors_are_told_apart():
+    import dense
+    from torch.autograd import forward_ad
+    x = torch.ones(2, 3)
+    assert not dense._has_tangent(x)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        assert not dense._has_tangent(x) and dense._has_tangent(dual)
+        with torch.no_grad():
+            assert dense._has_tangent(dual) and dense._has_tangent(dual[:, 1:].t())
+        assert not dense._has_tangent(forward_ad.unpack_dual(dual).primal)
