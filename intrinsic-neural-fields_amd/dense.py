@@ -322,21 +322,23 @@ def _workspace(lib, rows, n, widths, backward, device):
 
 class _LinearCkpt(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, spec, act, kept, *tensors):
-        # spec and tensors as _Linear; kept: per segment the Rows8 of x, or None to make them
+    def forward(ctx, spec, act, kept, recorded, *tensors):
+        # spec and tensors as _Linear; kept: per segment the Rows8 of x, or None to make them;
+        # recorded: whether gradients are (needs_input_grad says what the tensors ask for, also
+        # under no_grad; in here nothing is ever recorded)
         rt = _rt()
         lib = rt.lib
         nseg = len(spec)
         nb = len(tensors) - nseg
         nw = max(w for w, _ in spec) + 1
         nb -= nw
-        needs = ctx.needs_input_grad
+        needs = ctx.needs_input_grad if recorded else (False,) * (4 + len(tensors))
         W0 = tensors[nseg]
         rows, n, device = tensors[0].shape[0], W0.shape[0], W0.device
         # one allocation for what is kept: each segment's q and scale, then the mask
         at, places = 0, []
         for s, (wi, _) in enumerate(spec):
-            make = needs[3 + nseg + wi] and kept[s] is None
+            make = needs[4 + nseg + wi] and kept[s] is None
             places.append(at if make else None)
             if make:
                 at += _round_up(rows * _round_up(tensors[s].shape[1], 16) + 128, 256) + _round_up(rows * 4, 256)
@@ -366,6 +368,8 @@ class _LinearCkpt(torch.autograd.Function):
                     W.stride(1), tensors[nseg + nw + s].data_ptr() if s < nb else None, yp if s else None, n,
                     act if last else 0, yp, n, base + mask_at if last and mask_at is not None else None, q, ldq, scale,
                     work.data_ptr(), st), "linear_ckpt_forward")
+        if not recorded:
+            return y
         ctx.layer = (spec, act, nw, nb, rows, n, places, mask_at, [t.shape[1] for t in tensors[:nseg]],
                      [t.dtype for t in tensors[:nseg]])
         save = [held, y if act == 2 else None, *tensors[nseg:nseg + nw]]
@@ -394,7 +398,7 @@ class _LinearCkpt(torch.autograd.Function):
         dy = _near(dy)
         device = dy.device
         base = held.data_ptr() if held is not None else 0
-        grads = [None] * (3 + nseg + nw + nb)
+        grads = [None] * (4 + nseg + nw + nb)
         with _on(device):
             st = _stream(device)
             work = _workspace(lib, rows, n, widths, 1, device)
@@ -409,17 +413,17 @@ class _LinearCkpt(torch.autograd.Function):
                     qt, st_ = next(own), next(own)
                     q, scale, ldq = qt.data_ptr(), st_.data_ptr(), qt.stride(0)
                 dx = dw = db = None
-                if needs[3 + s]:
-                    grads[3 + s] = dx = torch.empty((rows, k), dtype=dtypes[s], device=device)
-                if needs[3 + nseg + wi]:
-                    g = grads[3 + nseg + wi]
+                if needs[4 + s]:
+                    grads[4 + s] = dx = torch.empty((rows, k), dtype=dtypes[s], device=device)
+                if needs[4 + nseg + wi]:
+                    g = grads[4 + nseg + wi]
                     if g is None:
                         covered = sum(kk for (wj, _), kk in zip(spec, widths) if wj == wi) == W.shape[1]
-                        g = grads[3 + nseg + wi] = (torch.empty if covered else torch.zeros)(
+                        g = grads[4 + nseg + wi] = (torch.empty if covered else torch.zeros)(
                             W.shape, dtype=torch.float32, device=device)
                     dw = g.data_ptr() + 4 * c0
-                if s < nb and needs[3 + nseg + nw + s]:
-                    grads[3 + nseg + nw + s] = db = torch.empty(n, dtype=torch.float32, device=device)
+                if s < nb and needs[4 + nseg + nw + s]:
+                    grads[4 + nseg + nw + s] = db = torch.empty(n, dtype=torch.float32, device=device)
                 if dx is None and dw is None and db is None:
                     continue
                 xc = rt.dtype_code(dx) if dx is not None else rt.DTYPE_F32
@@ -462,7 +466,8 @@ def _linear_ckpt(segments, spec, weights, biases, act, checkpoint):
     for t in (*xs, *weights, *biases):
         if t.device != device:
             raise ValueError("linear takes its tensors on one device")
-    return _LinearCkpt.apply(spec, act, tuple(None if isinstance(c, str) else c for c in kept), *xs, *weights, *biases)
+    return _LinearCkpt.apply(spec, act, tuple(None if isinstance(c, str) else c for c in kept), torch.is_grad_enabled(),
+                             *xs, *weights, *biases)
 
 
 def view_angles(unit_dirs, face_idxs, face_normals):
