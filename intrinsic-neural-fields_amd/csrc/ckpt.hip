@@ -453,10 +453,14 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
 
   // lane: row wr WROWS + 16 i + r16, columns wc WCOLS + 16 j + 4 g4 + (0..3)
   int sm[TI];
+  // NaN for a bf16 row that is not finite, else 0: such a value has no low piece whose inf - inf would make NaN
+  // of all that it meets, and an infinity of its own sign, or after a ReLU a zero, would come out
+  float bad[LO ? 1 : TI];
 #pragma unroll
   for (int i = 0; i < TI; ++i) {
     const int64_t m = min(m0 + wr * P::WROWS + 16 * i + r16, a.rows - 1);
     sm[i] = MODE == 0 ? shift_of(a.scale[m] * 127.f) : a.shift[m];
+    if constexpr (!LO) bad[i] = a.scale[m] * 0.f;
   }
   int sn[TJ][4];
   float bias[TJ][4];
@@ -481,7 +485,10 @@ __global__ __launch_bounds__(64 * WM * WN) void split_tile_kernel(SideArgs a, in
       const int n = n0 + wc * P::WCOLS + 16 * j + 4 * g4;
       f32x4 z;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[e] = by_power(acc[j][i][e], -(sm[i] + sn[j][e])) + bias[j][e];
+      for (int e = 0; e < 4; ++e) {
+        z[e] = by_power(acc[j][i][e], -(sm[i] + sn[j][e])) + bias[j][e];
+        if constexpr (!LO) z[e] += bad[i];
+      }
       if (MODE == 0) finish_forward(a, m, n, z);
       if (direct) store_four<T>(a, m, n, z);
       else *reinterpret_cast<f32x4*>(mine + r16 * RS + (16 * j + 4 * g4) * 4) = z;
