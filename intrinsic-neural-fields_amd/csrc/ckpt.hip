@@ -919,7 +919,7 @@ int launch_tile(const SideArgs& a, hipStream_t stream) {
   using P = ST<BM, BN, WM, WN>;
   const int tiles_n = (int)ceil_div(a.cols, BN);
   const int64_t nblocks = ceil_div(a.rows, BM) * tiles_n;
-  INF_CHECK_ARG(nblocks < (int64_t)1 << 31, "linear_ckpt: too many tiles");
+  INF_CHECK_ARG(nblocks * P::THREADS < (int64_t)1 << 32, "linear_ckpt: too many tiles");
   const auto kernel = split_tile_kernel<MODE, ACT, X, T, BM, BN, WM, WN>;
   static LdsLimit lds;
   const int allowed = lds.raise((const void*)kernel, P::LDS);
@@ -1048,31 +1048,42 @@ BackwardSpace backward_space(int64_t rows, int n, int k) {
 }
 
 template <int ACT>
+int backward_dx(int64_t rows, int n, int k, const Dz& dz, const float* W, int64_t swn, int64_t swk, void* dx, int dx_dtype,
+                int64_t lddx, char* ws, const BackwardSpace& o, hipStream_t st) {
+  const Weight w{W, swk, swn, k, n, ws + o.V, (int*)(ws + o.vshift)};
+  const bool panel = takes_panel(rows, n, k);
+  const int rc = panel ? launch_split(w, st) : launch_before_dx<ACT>(w, dz, rows, n, (int*)(ws + o.shift), st);
+  if (rc != INF_OK) return rc;
+  SideArgs a{};
+  a.rows = rows;
+  a.cols = k;
+  a.K = n;
+  a.shift = (int*)(ws + o.shift);
+  a.dz = dz;
+  a.V = ws + o.V;
+  a.vshift = (int*)(ws + o.vshift);
+  a.out = dx;
+  a.ldo = lddx;
+  if (panel) return dx_dtype == INF_DTYPE_F32 ? launch_panel<ACT, float>(a, st) : launch_panel<ACT, bf16>(a, st);
+  return dx_dtype == INF_DTYPE_F32 ? launch_tiles<1, ACT, float, float>(a, st) : launch_tiles<1, ACT, float, bf16>(a, st);
+}
+
+template <int ACT>
 int backward(int64_t rows, int n, int k, const Dz& dz, const int8_t* q, int64_t ldq, const float* scale, const float* W,
              int64_t swn, int64_t swk, void* dx, int dx_dtype, int64_t lddx, float* dW, int64_t lddw, float* db,
              char* ws, hipStream_t st) {
   const BackwardSpace o = backward_space(rows, n, k);
-  int rc;
-  if (dx != nullptr && rows > 0) {
-    const Weight w{W, swk, swn, k, n, ws + o.V, (int*)(ws + o.vshift)};
-    const bool panel = takes_panel(rows, n, k);
-    rc = panel ? launch_split(w, st) : launch_before_dx<ACT>(w, dz, rows, n, (int*)(ws + o.shift), st);
-    if (rc != INF_OK) return rc;
-    SideArgs a{};
-    a.rows = rows;
-    a.cols = k;
-    a.K = n;
-    a.shift = (int*)(ws + o.shift);
-    a.dz = dz;
-    a.V = ws + o.V;
-    a.vshift = (int*)(ws + o.vshift);
-    a.out = dx;
-    a.ldo = lddx;
-    rc = panel ? (dx_dtype == INF_DTYPE_F32 ? launch_panel<ACT, float>(a, st) : launch_panel<ACT, bf16>(a, st))
-               : (dx_dtype == INF_DTYPE_F32 ? launch_tiles<1, ACT, float, float>(a, st)
-                                            : launch_tiles<1, ACT, float, bf16>(a, st));
-    if (rc != INF_OK) return rc;
-  }
+  int rc = INF_OK;
+  if (dx != nullptr)
+    rc = in_turns(rows, k, [&](int64_t r, int64_t count) {
+      Dz part = dz;
+      part.dy += r * dz.lddy;
+      if (ACT == DZ_SIGMOID) part.y += r * dz.ldy;
+      if (ACT == DZ_RELU) part.mask += r * dz.words;
+      char* const out = (char*)dx + r * lddx * (dx_dtype == INF_DTYPE_F32 ? 4 : 2);
+      return backward_dx<ACT>(count, n, k, part, W, swn, swk, out, dx_dtype, lddx, ws, o, st);
+    });
+  if (rc != INF_OK) return rc;
   if (dW != nullptr) {
     const DwShape d = dw_shape(rows, n, k);
     DwArgs a{rows, n, k, dz, q, ldq, scale, d.tiles_k, d.tiles, d.splits, d.rows_a_split, (float*)(ws + o.slabs), k,
@@ -1127,33 +1138,32 @@ int inf_linear_ckpt_forward(int64_t rows, int n, int k, const void* x, int x_dty
   char* const ws = (char*)workspace;
   const ForwardSpace o = forward_space(rows, n, k);
   const Weight w{W, stride_wn, stride_wk, n, k, ws + o.V, (int*)(ws + o.vshift)};
-  SideArgs a{};
-  a.scale = scale;
   const bool f32 = x_dtype == INF_DTYPE_F32;
-  int rc;
-  if (q == nullptr && scale != nullptr) {
-    rc = launch_split(w, st);
-  } else {
-    if (scale == nullptr) a.scale = (float*)(ws + o.scale);
-    rc = f32 ? launch_before_forward(w, (const float*)x, rows, k, ld_x, q, ld_q, (float*)a.scale, st)
-             : launch_before_forward(w, (const bf16*)x, rows, k, ld_x, q, ld_q, (float*)a.scale, st);
-  }
-  if (rc != INF_OK) return rc;
-  a.rows = rows;
-  a.cols = n;
-  a.K = k;
-  a.x = x;
-  a.ldx = ld_x;
-  a.V = ws + o.V;
-  a.vshift = (int*)(ws + o.vshift);
-  a.bias = bias;
-  a.add = add;
-  a.ldadd = ld_add;
-  a.act = act;
-  a.out = y;
-  a.ldo = ld_y;
-  a.mask = mask;
-  return f32 ? launch_tiles<0, 0, float, float>(a, st) : launch_tiles<0, 0, bf16, float>(a, st);
+  return q8::in_turns(rows, n, [&](int64_t r, int64_t count) {
+    SideArgs a{};
+    a.rows = count;
+    a.cols = n;
+    a.K = k;
+    a.x = (const char*)x + r * ld_x * (f32 ? 4 : 2);
+    a.ldx = ld_x;
+    a.V = ws + o.V;
+    a.vshift = (int*)(ws + o.vshift);
+    a.bias = bias;
+    a.add = add != nullptr ? add + r * ld_add : nullptr;
+    a.ldadd = ld_add;
+    a.act = act;
+    a.out = y + r * ld_y;
+    a.ldo = ld_y;
+    a.mask = mask != nullptr ? mask + r * ((n + 31) / 32) : nullptr;
+    float* const s = scale != nullptr ? scale + r : (float*)(ws + o.scale);
+    a.scale = s;
+    int8_t* const to = q != nullptr ? q + r * ld_q : nullptr;
+    const int rc = to == nullptr && scale != nullptr ? launch_split(w, st)
+                   : f32 ? launch_before_forward(w, (const float*)a.x, count, k, ld_x, to, ld_q, s, st)
+                         : launch_before_forward(w, (const bf16*)a.x, count, k, ld_x, to, ld_q, s, st);
+    if (rc != INF_OK) return rc;
+    return f32 ? launch_tiles<0, 0, float, float>(a, st) : launch_tiles<0, 0, bf16, float>(a, st);
+  });
 }
 
 int inf_linear_ckpt_backward(int64_t rows, int n, int k, const float* dy, int64_t ld_dy, int act, const float* y,

@@ -789,7 +789,7 @@ int launch_tile(const Linear8Args& a, hipStream_t stream) {
   using P = L8<BM, BN, WM, WN>;
   const int tiles_n = (int)ceil_div(a.n, BN);
   const int64_t nblocks = ceil_div(a.rows, BM) * tiles_n;
-  INF_CHECK_ARG(nblocks < (int64_t)1 << 31, "linear_int: too many tiles");
+  INF_CHECK_ARG(nblocks * P::THREADS < (int64_t)1 << 32, "linear_int: too many tiles");
   static LdsLimit lds;
   const int allowed = lds.raise((const void*)linear8_tile_kernel<T, BM, BN, WM, WN>, P::LDS);
   if (allowed != INF_OK) return allowed;
@@ -867,6 +867,45 @@ Workspace workspace_of(int64_t rows, int n, int k, int x_dtype, int out_dtype) {
   return w;
 }
 
+// Rows of one turn (in_turns): their product, and their way into and out of 8 bits.
+int linear_rows(const Linear8Args& call, const void* x, int x_dtype, int out_dtype, char* wsp, hipStream_t st) {
+  Linear8Args a = call;
+  const int64_t rows = a.rows, ld_x = a.ldq;
+  const int n = a.n, k = a.k;
+  const bool x8 = x_dtype == INF_DTYPE_I8;
+  const Workspace o = workspace_of(rows, n, k, x_dtype, out_dtype);
+  const bool put_after = out_dtype == INF_DTYPE_I8 && !rows_whole(rows, n, k);
+  if (put_after) {
+    a.out = wsp + o.y;
+    a.ldo = n;
+  }
+  const int product_dtype = put_after ? INF_DTYPE_F32 : out_dtype;
+  int rc;
+  if (is_few(rows, k)) {
+    rc = x8 ? launch_few_out<int8_t>(a, product_dtype, x, ld_x, st)
+            : x_dtype == INF_DTYPE_BF16 ? launch_few_out<bf16>(a, product_dtype, x, ld_x, st)
+                                        : launch_few_out<float>(a, product_dtype, x, ld_x, st);
+  } else if (rows_walk(a)) {
+    rc = x8 ? launch_rows_out<int8_t>(a, product_dtype, x, ld_x, st)
+            : x_dtype == INF_DTYPE_BF16 ? launch_rows_out<bf16>(a, product_dtype, x, ld_x, st)
+                                        : launch_rows_out<float>(a, product_dtype, x, ld_x, st);
+  } else if (takes_long(rows, n, k, x_dtype)) {
+    rc = x_dtype == INF_DTYPE_BF16 ? launch_long<bf16>(a, product_dtype, x, ld_x, st)
+                                   : launch_long<float>(a, product_dtype, x, ld_x, st);
+  } else {
+    if (!x8) {
+      a.q = (int8_t*)(wsp + o.q);
+      a.ldq = round_up(k, q8::Q_ALIGN);
+      a.qs = (float*)(wsp + o.qs);
+      rc = launch_quantize_rows(x, x_dtype, rows, k, ld_x, (int8_t*)a.q, a.ldq, (float*)a.qs, st);
+      if (rc != INF_OK) return rc;
+    }
+    rc = launch_linear8(a, product_dtype, st);
+  }
+  if (rc != INF_OK || !put_after) return rc;
+  return launch_quantize_rows(a.out, INF_DTYPE_F32, rows, n, n, (int8_t*)call.out, call.ldo, call.os, st);
+}
+
 }  // namespace
 }  // namespace inf
 
@@ -902,40 +941,14 @@ int inf_linear_int(int64_t rows, int n, int k, const void* x, int x_dtype, int64
   const Workspace o = workspace_of(rows, n, k, x_dtype, out_dtype);
   INF_CHECK_ARG(o.bytes == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0),
                 "linear_int: null or unaligned workspace");
-  char* const wsp = (char*)workspace;
-  const hipStream_t st = (hipStream_t)stream;
-  Linear8Args a{rows, n, k, (const int8_t*)x, ld_x, x_scale, w, round_up(k, q8::W_ALIGN), w_scale, bias, add, ld_add,
-                act, out, ld_out, out_scale};
-  const bool put_after = y8 && !rows_whole(rows, n, k);
-  if (put_after) {
-    a.out = wsp + o.y;
-    a.ldo = n;
-  }
-  const int product_dtype = put_after ? INF_DTYPE_F32 : out_dtype;
-  int rc;
-  if (is_few(rows, k)) {
-    rc = x8 ? launch_few_out<int8_t>(a, product_dtype, x, ld_x, st)
-            : x_dtype == INF_DTYPE_BF16 ? launch_few_out<bf16>(a, product_dtype, x, ld_x, st)
-                                        : launch_few_out<float>(a, product_dtype, x, ld_x, st);
-  } else if (rows_walk(a)) {
-    rc = x8 ? launch_rows_out<int8_t>(a, product_dtype, x, ld_x, st)
-            : x_dtype == INF_DTYPE_BF16 ? launch_rows_out<bf16>(a, product_dtype, x, ld_x, st)
-                                        : launch_rows_out<float>(a, product_dtype, x, ld_x, st);
-  } else if (takes_long(rows, n, k, x_dtype)) {
-    rc = x_dtype == INF_DTYPE_BF16 ? launch_long<bf16>(a, product_dtype, x, ld_x, st)
-                                   : launch_long<float>(a, product_dtype, x, ld_x, st);
-  } else {
-    if (!x8) {
-      a.q = (int8_t*)(wsp + o.q);
-      a.ldq = round_up(k, q8::Q_ALIGN);
-      a.qs = (float*)(wsp + o.qs);
-      rc = launch_quantize_rows(x, x_dtype, rows, k, ld_x, (int8_t*)a.q, a.ldq, (float*)a.qs, st);
-      if (rc != INF_OK) return rc;
-    }
-    rc = launch_linear8(a, product_dtype, st);
-  }
-  if (rc != INF_OK || !put_after) return rc;
-  return launch_quantize_rows(a.out, INF_DTYPE_F32, rows, n, n, (int8_t*)out, ld_out, out_scale, st);
+  const int64_t x_size = x8 ? 1 : x_dtype == INF_DTYPE_BF16 ? 2 : 4, out_size = y8 ? 1 : out_dtype == INF_DTYPE_BF16 ? 2 : 4;
+  return q8::in_turns(rows, n, [&](int64_t r, int64_t count) {
+    const char* const from = (const char*)x + r * ld_x * x_size;
+    const Linear8Args a{count, n, k, (const int8_t*)from, ld_x, x8 ? x_scale + r : nullptr, w, round_up(k, q8::W_ALIGN),
+                        w_scale, bias, add != nullptr ? add + r * ld_add : nullptr, ld_add, act,
+                        (char*)out + r * ld_out * out_size, ld_out, y8 ? out_scale + r : nullptr};
+    return linear_rows(a, from, x_dtype, out_dtype, (char*)workspace, (hipStream_t)stream);
+  });
 }
 
 }  // extern "C"

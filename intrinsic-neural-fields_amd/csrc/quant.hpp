@@ -8,6 +8,7 @@
 // or a NaN has s = NaN and q = 0, so that whatever is made of it is NaN.
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "common.hpp"
@@ -25,6 +26,19 @@ constexpr int64_t Q_ALIGN = 16;
 constexpr int64_t W_ALIGN = 128;
 // bytes behind the last q row that a product may read
 constexpr int64_t Q_SLACK = 128;
+
+// A launch holds fewer than 2^32 threads.  These kernels take up to 256 of them a row and one for 16 results:
+// rows beyond that go in turns of about equal size.
+template <class F>
+int in_turns(int64_t rows, int64_t width, const F& f) {
+  const int64_t most = std::min<int64_t>((int64_t)1 << 23, std::max<int64_t>(((int64_t)1 << 35) / width, 1));
+  const int64_t each = ceil_div(rows, std::max<int64_t>(ceil_div(rows, most), 1));
+  for (int64_t r = 0; r < rows; r += each) {
+    const int rc = f(r, std::min(each, rows - r));
+    if (rc != INF_OK) return rc;
+  }
+  return INF_OK;
+}
 
 // |x| as an unsigned number: orders like |x|, infinities and NaNs above everything finite,
 // so that a maximum keeps them (fmaxf drops a NaN)

@@ -111,10 +111,13 @@ static void restore_rows_any(const int8_t* q, int64_t ldq, const float* scale, i
 
 int launch_quantize_rows(const void* x, int dtype, int64_t rows, int k, int64_t ldx, int8_t* q, int64_t ldq,
                          float* scale, hipStream_t stream) {
-  if (dtype == INF_DTYPE_F32) quantize_rows_any((const float*)x, rows, k, ldx, q, ldq, scale, stream);
-  else quantize_rows_any((const bf16*)x, rows, k, ldx, q, ldq, scale, stream);
-  INF_LAUNCH_CHECK();
-  return INF_OK;
+  return in_turns(rows, 1, [&](int64_t r, int64_t count) {
+    int8_t* const to = q != nullptr ? q + r * ldq : nullptr;
+    if (dtype == INF_DTYPE_F32) quantize_rows_any((const float*)x + r * ldx, count, k, ldx, to, ldq, scale + r, stream);
+    else quantize_rows_any((const bf16*)x + r * ldx, count, k, ldx, to, ldq, scale + r, stream);
+    INF_LAUNCH_CHECK();
+    return INF_OK;
+  });
 }
 
 }  // namespace inf
@@ -144,10 +147,14 @@ int inf_restore_rows(const int8_t* q, int64_t ld_q, const float* scale, int64_t 
   if (rows == 0) return INF_OK;
   INF_CHECK_ARG(q != nullptr && scale != nullptr && out != nullptr && (uintptr_t)q % 16 == 0,
                 "restore_rows: null or unaligned argument");
-  if (out_dtype == INF_DTYPE_F32) restore_rows_any(q, ld_q, scale, rows, k, (float*)out, ld_out, (hipStream_t)stream);
-  else restore_rows_any(q, ld_q, scale, rows, k, (bf16*)out, ld_out, (hipStream_t)stream);
-  INF_LAUNCH_CHECK();
-  return INF_OK;
+  const hipStream_t st = (hipStream_t)stream;
+  return q8::in_turns(rows, 1, [&](int64_t r, int64_t count) {
+    const int8_t* const from = q + r * ld_q;
+    if (out_dtype == INF_DTYPE_F32) restore_rows_any(from, ld_q, scale + r, count, k, (float*)out + r * ld_out, ld_out, st);
+    else restore_rows_any(from, ld_q, scale + r, count, k, (bf16*)out + r * ld_out, ld_out, st);
+    INF_LAUNCH_CHECK();
+    return INF_OK;
+  });
 }
 
 int64_t inf_packed_weight_bytes(int n, int k) {
