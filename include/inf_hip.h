@@ -216,8 +216,11 @@ int inf_pack_weight(const int8_t* q, int64_t stride_n, int64_t stride_k, int n, 
  * be NULL.  x: fp32 / bf16 (put into 8 bits on the way), or INF_DTYPE_I8 rows
  * with x_scale, behind whose last row 128 bytes may be read (their values do not matter).
  * out: fp32 / bf16, or INF_DTYPE_I8 rows with out_scale (inf_quantize_rows of the result).
- * act 0 none, 1 ReLU, 2 sigmoid.  workspace: inf_linear_int_workspace_bytes bytes.        */
+ * act 0 none, 1 ReLU, 2 sigmoid.  workspace: inf_linear_int_call_workspace_bytes bytes, often
+ * none; inf_linear_int_workspace_bytes is enough for any act, with or without add.         */
 int64_t inf_linear_int_workspace_bytes(int64_t rows, int n, int k, int x_dtype, int out_dtype);
+int64_t inf_linear_int_call_workspace_bytes(int64_t rows, int n, int k, int x_dtype, int out_dtype, int act,
+                                            int with_add);
 int inf_linear_int(int64_t rows, int n, int k, const void* x, int x_dtype, int64_t ld_x, const float* x_scale,
                    const int8_t* w, const float* w_scale, const float* bias, const float* add, int64_t ld_add, int act,
                    void* out, int out_dtype, int64_t ld_out, float* out_scale, void* workspace, inf_stream_t stream);

@@ -535,8 +535,8 @@ int launch_rows(const Linear8Args& a, const X* x, int64_t ldx, hipStream_t strea
 // k up to 256 with up to 256 outputs, and rows for a turn of every CU.  (Fewer outputs than 33 are
 // bound by x's bytes whichever kernel reads them; a sigmoid or a sum to add to is a head's or a skip
 // layer's, one a network.)
-bool rows_walk(const Linear8Args& a) {
-  return a.rows >= 16384 && a.k <= 256 && a.n > 32 && a.n <= 256 && a.act != 2 && a.add == nullptr;
+bool rows_walk(int64_t rows, int n, int k, int act, bool with_add) {
+  return rows >= 16384 && k <= 256 && n > 32 && n <= 256 && act != 2 && !with_add;
 }
 
 template <typename X, typename T>
@@ -848,13 +848,22 @@ bool takes_long(int64_t rows, int n, int k, int x_dtype) {
 // whether a result in 8 bits is made by the product's own kernel
 bool rows_whole(int64_t rows, int n, int k) { return n <= 256 && !is_few(rows, k); }
 
+// Which kernel makes the products of a call: the workspace's size and the launch go by the same rule.
+// (Calls in several turns have thousands of rows in each, so that the rule names the same kernel for them.)
+enum class Form { FEW, WALK, LONG, TILES };
+Form form_of(int64_t rows, int n, int k, int x_dtype, int act, bool with_add) {
+  if (is_few(rows, k)) return Form::FEW;
+  if (rows_walk(rows, n, k, act, with_add)) return Form::WALK;
+  return takes_long(rows, n, k, x_dtype) ? Form::LONG : Form::TILES;
+}
+
 struct Workspace {
   int64_t q, qs, y, bytes;  // offsets: x in 8 bits, its scales, the fp32 rows that go into 8 bits
 };
 
-Workspace workspace_of(int64_t rows, int n, int k, int x_dtype, int out_dtype) {
+Workspace workspace_of(Form form, int64_t rows, int n, int k, int x_dtype, int out_dtype) {
   Workspace w{0, 0, 0, 0};
-  if (x_dtype != INF_DTYPE_I8 && !is_few(rows, k) && !takes_long(rows, n, k, x_dtype)) {
+  if (x_dtype != INF_DTYPE_I8 && form == Form::TILES) {
     w.q = w.bytes;
     w.bytes += round_up(rows * round_up(k, Q_ALIGN) + Q_SLACK, 256);
     w.qs = w.bytes;
@@ -873,7 +882,8 @@ int linear_rows(const Linear8Args& call, const void* x, int x_dtype, int out_dty
   const int64_t rows = a.rows, ld_x = a.ldq;
   const int n = a.n, k = a.k;
   const bool x8 = x_dtype == INF_DTYPE_I8;
-  const Workspace o = workspace_of(rows, n, k, x_dtype, out_dtype);
+  const Form form = form_of(rows, n, k, x_dtype, a.act, a.add != nullptr);
+  const Workspace o = workspace_of(form, rows, n, k, x_dtype, out_dtype);
   const bool put_after = out_dtype == INF_DTYPE_I8 && !rows_whole(rows, n, k);
   if (put_after) {
     a.out = wsp + o.y;
@@ -881,15 +891,15 @@ int linear_rows(const Linear8Args& call, const void* x, int x_dtype, int out_dty
   }
   const int product_dtype = put_after ? INF_DTYPE_F32 : out_dtype;
   int rc;
-  if (is_few(rows, k)) {
+  if (form == Form::FEW) {
     rc = x8 ? launch_few_out<int8_t>(a, product_dtype, x, ld_x, st)
             : x_dtype == INF_DTYPE_BF16 ? launch_few_out<bf16>(a, product_dtype, x, ld_x, st)
                                         : launch_few_out<float>(a, product_dtype, x, ld_x, st);
-  } else if (rows_walk(a)) {
+  } else if (form == Form::WALK) {
     rc = x8 ? launch_rows_out<int8_t>(a, product_dtype, x, ld_x, st)
             : x_dtype == INF_DTYPE_BF16 ? launch_rows_out<bf16>(a, product_dtype, x, ld_x, st)
                                         : launch_rows_out<float>(a, product_dtype, x, ld_x, st);
-  } else if (takes_long(rows, n, k, x_dtype)) {
+  } else if (form == Form::LONG) {
     rc = x_dtype == INF_DTYPE_BF16 ? launch_long<bf16>(a, product_dtype, x, ld_x, st)
                                    : launch_long<float>(a, product_dtype, x, ld_x, st);
   } else {
@@ -915,7 +925,13 @@ extern "C" {
 
 int64_t inf_linear_int_workspace_bytes(int64_t rows, int n, int k, int x_dtype, int out_dtype) {
   if (rows < 0 || n < 1 || k < 1) return -1;
-  return workspace_of(rows, n, k, x_dtype, out_dtype).bytes;
+  const Form form = form_of(rows, n, k, x_dtype, 2, true);  // (the only one that needs none because of them is WALK)
+  return workspace_of(form, rows, n, k, x_dtype, out_dtype).bytes;
+}
+
+int64_t inf_linear_int_call_workspace_bytes(int64_t rows, int n, int k, int x_dtype, int out_dtype, int act, int with_add) {
+  if (rows < 0 || n < 1 || k < 1) return -1;
+  return workspace_of(form_of(rows, n, k, x_dtype, act, with_add != 0), rows, n, k, x_dtype, out_dtype).bytes;
 }
 
 int inf_linear_int(int64_t rows, int n, int k, const void* x, int x_dtype, int64_t ld_x, const float* x_scale,
@@ -938,7 +954,7 @@ int inf_linear_int(int64_t rows, int n, int k, const void* x, int x_dtype, int64
                 "linear_int: int8 rows need their scales and rows that start on 16 bytes");
   INF_CHECK_ARG(!y8 || (out_scale != nullptr && ld_out % q8::Q_ALIGN == 0 && (uintptr_t)out % 16 == 0),
                 "linear_int: int8 output needs scales and rows that start on 16 bytes");
-  const Workspace o = workspace_of(rows, n, k, x_dtype, out_dtype);
+  const Workspace o = workspace_of(form_of(rows, n, k, x_dtype, act, add != nullptr), rows, n, k, x_dtype, out_dtype);
   INF_CHECK_ARG(o.bytes == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0),
                 "linear_int: null or unaligned workspace");
   const int64_t x_size = x8 ? 1 : x_dtype == INF_DTYPE_BF16 ? 2 : 4, out_size = y8 ? 1 : out_dtype == INF_DTYPE_BF16 ? 2 : 4;

@@ -305,10 +305,11 @@ def linear8(xs, weights, biases, act=None, out=torch.float32):
             else:
                 y = torch.empty((rows, n), dtype=out if s == last else torch.float32, device=device)
                 op, ldo, osc = y.data_ptr(), n, None
-            nws = lib.inf_linear_int_workspace_bytes(rows, n, w.k, xc, oc)
+            to = a if s == last else 0
+            nws = lib.inf_linear_int_call_workspace_bytes(rows, n, w.k, xc, oc, to, acc is not None)
             ws = torch.empty(nws, dtype=torch.uint8, device=device) if nws else None
             rt.check(lib.inf_linear_int(rows, n, w.k, q.data_ptr(), xc, q.stride(0), scale, w.packed.data_ptr(),
-                                        w.scale.data_ptr(), _at(b), _at(acc), n, a if s == last else 0, op, oc, ldo,
+                                        w.scale.data_ptr(), _at(b), _at(acc), n, to, op, oc, ldo,
                                         osc, _at(ws), _stream(device)), "linear_int")
             acc = y
     return y

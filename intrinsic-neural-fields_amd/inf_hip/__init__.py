@@ -90,6 +90,7 @@ _SIGNATURES = {
     "inf_packed_weight_bytes": (c_int64, [c_int, c_int]),
     "inf_pack_weight": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p]),
     "inf_linear_int_workspace_bytes": (c_int64, [c_int64, c_int, c_int, c_int, c_int]),
+    "inf_linear_int_call_workspace_bytes": (c_int64, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int]),
     "inf_linear_int": (c_int, [c_int64, c_int, c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                c_void_p, c_int64, c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p]),
     "inf_linear_ckpt_workspace_bytes": (c_int64, [c_int64, c_int, c_int, c_int, c_int]),
