@@ -323,8 +323,6 @@ struct LR {
   static_assert(LDS <= 160 * 1024, "LDS");
 };
 
-__device__ __forceinline__ float positive_nan(float v) { return v != v ? __uint_as_float(0x7fc00000u) : v; }
-
 template <typename X, typename T, int KS, int TJ>
 __global__ __launch_bounds__(64 * WALK_WAVES) void linear8_rows_kernel(Linear8Args a, const X* __restrict__ x,
                                                                                  int64_t ldx) {
@@ -350,8 +348,8 @@ __global__ __launch_bounds__(64 * WALK_WAVES) void linear8_rows_kernel(Linear8Ar
     }
   }
   for (int i = tid; i < TJ * 16; i += P::THREADS) {
-    sws[i] = i < a.n ? positive_nan(a.ws[i]) : 0.f;  // columns behind the last are zero
-    sws[TJ * 16 + i] = i < a.n && a.bias != nullptr ? positive_nan(a.bias[i]) : 0.f;
+    sws[i] = i < a.n ? a.ws[i] : 0.f;  // columns behind the last are zero
+    sws[TJ * 16 + i] = i < a.n && a.bias != nullptr ? a.bias[i] : 0.f;
   }
   __syncthreads();
 
@@ -383,10 +381,11 @@ __global__ __launch_bounds__(64 * WALK_WAVES) void linear8_rows_kernel(Linear8Ar
         }
     }
   };
-  // ReLU in one operation: as whole numbers, negative values lie below zero and a NaN (of positive sign:
-  // every one here is) above.  Without it the bound is below everything (and unknown to the compiler,
-  // which else selects: an operation more, 47.5 and 45.8 us from 8 bits into 8 bits).
-  int least = a.act == 1 ? 0 : (int)0x80000000;
+  // ReLU in one operation, the maximum that keeps a NaN (inf 0 and inf - inf, of scales, biases and
+  // overflows, have a negative sign here: a maximum of whole numbers would make zeros of them; three layers of
+  // 262,144 x 256 took 141 us with it, 144 so).  Without ReLU the bound is below everything (and unknown to
+  // the compiler, which else selects: an operation more).
+  int least = a.act == 1 ? 0 : (int)0xff800000;  // the bits of 0 and of minus infinity
   asm volatile("" : "+s"(least));
   int tile = (int)blockIdx.x * P::NW + wave;
   if (tile < tiles) fetch(tile);
@@ -397,7 +396,7 @@ __global__ __launch_bounds__(64 * WALK_WAVES) void linear8_rows_kernel(Linear8Ar
     if constexpr (sizeof(X) == 1) {
 #pragma unroll
       for (int b = 0; b < KS; ++b) xf[b] = __builtin_bit_cast(i32x4, raw[b][0]);
-      sx = positive_nan(a.qs[min(m, a.rows - 1)]);
+      sx = a.qs[min(m, a.rows - 1)];
     } else {
       unsigned top = 0;
       if constexpr (sizeof(X) == 2) {  // two values at a time: bf16 is the upper half of its fp32
@@ -471,7 +470,7 @@ __global__ __launch_bounds__(64 * WALK_WAVES) void linear8_rows_kernel(Linear8Ar
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         z[e] = combine(acc[j][e], sx, sw[e], bias[e]);
-        z[e] = __int_as_float(max(__float_as_int(z[e]), least));
+        z[e] = __builtin_elementwise_maximum(z[e], __int_as_float(least));
       }
       if constexpr (sizeof(T) == 1) {
 #pragma unroll
