@@ -13,7 +13,9 @@
 //   (lo lo would be a fourth matrix instruction beside three.)  A bf16 x is one piece, exact down to
 //   2^-31 of the row's largest: two products.  The powers of two leave the result exactly.
 //   dW: q is exact in bf16 and dz s is three bf16 pieces, all 24 bits of it: three products, no
-//   scale (a column of dz has no scale that a sum over its rows could be divided by).
+//   scale (a column of dz has no scale that a sum over its rows could be divided by): from dz s below 2^-110
+//   on its low pieces are subnormal, and a term is off by less than 2^-133 |q|, 2^-126 at most.
+// A row of x whose 8-bit scale is 0 (its largest value is below 2^-143) counts as a row of zeros.
 // A value that is not finite makes NaN of the rows (and columns) that it enters.
 #include <algorithm>
 #include <cstdlib>

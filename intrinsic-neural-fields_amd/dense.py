@@ -118,8 +118,10 @@ def linear(segments, weights, biases, act=None, checkpoint=None):
     A list names it for each segment: "int8", or the `Rows8` of that x_s where several layers
     read the same tensor.  Its products are not quite fp32's: a value counts to 2^-23 of itself, or
     to 2^-39 of the largest of its row (of x and dz; of W, its row forward, its column for dx) where
-    that is more, a product to 2^-21; their sums are fp32, in another order; a row with an infinity or a NaN gives NaN.  (As with every layer here: a backward
-    is captured into a graph only while no eager graph of the same leaves is alive.)"""
+    that is more, a product to 2^-21; a term of dW to 2^-24 of itself, or to 2^-126 where that is
+    more; their sums are fp32, in another order; a row of x with an infinity or a NaN gives NaN,
+    and one whose largest value is below 2^-143 counts as zeros.  (As with every layer here: a
+    backward is captured into a graph only while no eager graph of the same leaves is alive.)"""
     for t in [x for x, _, _ in segments] + list(weights) + list(biases):
         if not t.is_cuda:
             raise RuntimeError("the dense layers run on the HIP device only; there is no CPU fallback")
@@ -210,9 +212,10 @@ class Rows8:
 
 def quantize_rows(x):
     """x [rows, k] fp32 / bf16 in 8 bits: scale = max|x| / 127 of each row, q the whole number
-    nearest to 127 x / max|x| (ties to even).  Rows of zeros have scale 0; a row with an
-    infinity or a NaN has scale NaN, and whatever is made of it is NaN.  No gradient: x counts
-    as detached, and a dual tensor of forward-mode differentiation is refused."""
+    nearest to 127 x / max|x| (ties to even).  Rows of zeros have scale 0 (so have rows whose
+    largest value is below 2^-143); a row with an infinity or a NaN has scale NaN, and whatever
+    is made of it is NaN.  No gradient: x counts as detached, and a dual tensor of forward-mode
+    differentiation is refused."""
     rt = _rt()
     rt.require_hip(x)
     if _has_tangent(x):
