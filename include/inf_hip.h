@@ -203,7 +203,7 @@ int inf_adam_dense(int64_t n, float* param, const float* grad, float* exp_avg, f
  * bytes behind column k do not matter to any reader and may be written.                   */
 int inf_quantize_rows(const void* x, int x_dtype, int64_t rows, int k, int64_t ld_x, int8_t* q, int64_t ld_q,
                       float* scale, inf_stream_t stream);
-/* out[m][j] = q[m][j] scale[m], rounded once to fp32 / bf16. */
+/* out[m][j] = q[m][j] scale[m], rounded to fp32; bf16: that rounded again. */
 int inf_restore_rows(const int8_t* q, int64_t ld_q, const float* scale, int64_t rows, int k, void* out, int out_dtype,
                      int64_t ld_out, inf_stream_t stream);
 /* 8-bit weights q[n][k] (any strides) laid out for inf_linear_int; `packed` 16-byte aligned,
@@ -212,8 +212,8 @@ int64_t inf_packed_weight_bytes(int n, int k);
 int inf_pack_weight(const int8_t* q, int64_t stride_n, int64_t stride_k, int n, int k, int8_t* packed,
                     inf_stream_t stream);
 /* out = act(fl(fl(acc) fl(x_scale[m] w_scale[n])) + bias[n] + add[m][n]), acc the exact sum
- * of the 8-bit products (k <= 2^17), each operation rounded once to fp32; bias and add may
- * be NULL.  x: fp32 / bf16 (put into 8 bits on the way), or INF_DTYPE_I8 rows
+ * of the 8-bit products (k <= 2^17), each operation rounded once to fp32, a bf16 result once
+ * more; bias and add may be NULL.  x: fp32 / bf16 (put into 8 bits on the way), or INF_DTYPE_I8 rows
  * with x_scale, behind whose last row 128 bytes may be read (their values do not matter).
  * out: fp32 / bf16, or INF_DTYPE_I8 rows with out_scale (inf_quantize_rows of the result).
  * act 0 none, 1 ReLU, 2 sigmoid.  workspace: inf_linear_int_call_workspace_bytes bytes, often

@@ -1,7 +1,7 @@
 // A linear layer on rows and weights in 8-bit whole numbers (quant.hpp), for rendering:
 //   acc_mn = sum_k qx_mk qw_nk                              exact, in 32 bits (k <= 2^17)
 //   z_mn   = fl(fl(acc) fl(sx_m sw_n)) + bias_n + add_mn    each operation rounded once to fp32
-//   y      = act(z), as fp32, bf16, or in 8-bit rows again
+//   y      = act(z), as fp32, rounded again to bf16, or in 8-bit rows again
 // The roundings are written out one by one and never contracted: a row that goes into 8
 // bits again has the same numbers whichever kernel made it.
 //

@@ -1,6 +1,6 @@
 // Rows in 8 bits (quant.hpp): the quantiser, its inverse, and the packing of 8-bit weights.
 //   inf_quantize_rows: x [rows][k] fp32 / bf16 -> q int8, scale fp32
-//   inf_restore_rows:  q s, rounded once to fp32 / bf16
+//   inf_restore_rows:  q s, rounded to fp32, for bf16 then to that
 //   inf_pack_weight:   int8 weights of any strides -> rows of whole 128 bytes, zero behind k
 #include <algorithm>
 

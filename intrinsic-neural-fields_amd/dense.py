@@ -197,7 +197,7 @@ class Rows8:
         return self.q.device
 
     def restore(self, dtype=torch.float32):
-        """scale * q, rounded once to fp32 / bf16."""
+        """scale * q, rounded to fp32; bf16: that rounded again."""
         rt = _rt()
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"8-bit rows are restored to fp32 or bf16, not {dtype}")
@@ -211,8 +211,8 @@ class Rows8:
 
 
 def quantize_rows(x):
-    """x [rows, k] fp32 / bf16 in 8 bits: scale = max|x| / 127 of each row, q the whole number
-    nearest to 127 x / max|x| (ties to even).  Rows of zeros have scale 0 (so have rows whose
+    """x [rows, k] fp32 / bf16 in 8 bits: scale = fl(max|x| fl(1 / 127)) of each row, q the whole
+    number nearest to 127 x / max|x| (the ratio itself; ties to even).  Rows of zeros have scale 0 (so have rows whose
     largest value is below 2^-143); a row with an infinity or a NaN has scale NaN, and whatever
     is made of it is NaN.  No gradient: x counts as detached, and a dual tensor of forward-mode
     differentiation is refused."""
@@ -269,7 +269,8 @@ def linear8(xs, weights, biases, act=None, out=torch.float32):
 
     xs: for each segment a matrix fp32 / bf16 (put into 8 bits on the way) or a Rows8;
     weights: a Weight8 each; biases: fp32 [n], one for each of the first segments.
-    out: torch.float32, torch.bfloat16, or torch.int8 for a Rows8 of the result.
+    out: torch.float32, torch.bfloat16 (the fp32 result rounded again), or torch.int8 for a Rows8
+    of the fp32 result.
     For rendering: it has no gradient, and refuses inputs that ask for one, in forward mode too."""
     rt = _rt()
     i8 = rt.DTYPE_I8
