@@ -226,8 +226,9 @@ int inf_linear_int(int64_t rows, int n, int k, const void* x, int x_dtype, int64
                    void* out, int out_dtype, int64_t ld_out, float* out_scale, void* workspace, inf_stream_t stream);
 /* Linear layer that keeps its input in 8 bits: y = act(x W^T + bias + add) from x (fp32 / bf16) as
  * it is, W(n, k) = W[n stride_wn + k stride_wk]; a value counts to 2^-23 of itself or 2^-39 of its
- * row's largest, a product to 2^-21, sums are fp32.  bias and add may be NULL, add may be y.  q and scale: the rows of x in 8 bits, written; scale alone: x's own scales,
- * read (q made before); both NULL: nothing is kept.  mask (not NULL): bit j of
+ * row's largest, a product to 2^-21, sums are fp32.  bias and add may be NULL, add may be y.
+ * q and scale: the rows of x in 8 bits, written; scale alone: x's own scales, read (q made
+ * before); both NULL: nothing is kept.  mask (not NULL): bit j of
  * word w of row m (ceil(n / 32) words a row) = y[m][32 w + j] > 0.  workspace:
  * inf_linear_ckpt_workspace_bytes(.., 0) bytes.  n k below 2^29 (n and k padded to 256), rows
  * of x, dy and y less than 2^21 values apart.                                              */
@@ -244,6 +245,12 @@ int inf_linear_ckpt_backward(int64_t rows, int n, int k, const float* dy, int64_
                              int64_t ld_y, const uint32_t* mask, const int8_t* q, int64_t ld_q, const float* scale,
                              const float* W, int64_t stride_wn, int64_t stride_wk, void* dx, int dx_dtype,
                              int64_t ld_dx, float* dW, int64_t ld_dw, float* db, void* workspace, inf_stream_t stream);
+
+/* The bits of a ReLU (mask as above) from its output, and dz = dy where they are set: for the layer
+ * whose products are inf_dense_gemm's and whose inputs are kept in 8 bits.                     */
+int inf_relu_mask(int64_t rows, int n, const float* y, int64_t ld_y, uint32_t* mask, inf_stream_t stream);
+int inf_relu_mask_bwd(int64_t rows, int n, const float* dy, int64_t ld_dy, const uint32_t* mask, float* dz,
+                      int64_t ld_dz, inf_stream_t stream);
 
 /* ---- plan: one TextureField (model.py:12-112) + its training step ---------------- */
 typedef struct inf_plan inf_plan;

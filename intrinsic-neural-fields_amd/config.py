@@ -4,8 +4,8 @@ Same YAML keys and defaults.  Differences, all on the device side: the optimizer
 HIP Adam (inf_optim.Adam, a torch.optim.Adam subclass with the same state layout), the
 loss functions carry the tag the fused training step needs, and an optional
 `model.kernels` section ({mode: fp32|bf16, max_batch: N}) selects the GEMM arithmetic, and
-for the view-dependent field {dense_checkpoints: int8, dense_inference: int8} the 8-bit dense
-layers (the reference ignores unknown keys, so these YAMLs still load there).
+for the view-dependent field {dense_checkpoints: int8, dense_products: fp32, dense_inference:
+int8} the 8-bit dense layers (the reference ignores unknown keys, so these YAMLs still load there).
 """
 import os
 from shutil import copyfile

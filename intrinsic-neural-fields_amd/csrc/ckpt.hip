@@ -915,6 +915,32 @@ __global__ __launch_bounds__(256) void db_kernel(Dz d, int64_t rows, int n, floa
   if (threadIdx.x == 0) db[blockIdx.x] = part[0];
 }
 
+// ---- a ReLU's bits for the layer whose products are plain fp32 ------------------------------
+// A wave 64 neighbouring values of a row; bound by bytes.
+__global__ __launch_bounds__(256) void relu_mask_kernel(int64_t rows, int n, const float* __restrict__ y, int64_t ldy,
+                                                        uint32_t* __restrict__ mask) {
+  const int lane = threadIdx.x % 64, parts = (n + 63) / 64, words = (n + 31) / 32;
+  for (int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 64; i < rows * parts; i += (int64_t)gridDim.x * 4) {
+    const int64_t m = i / parts;
+    const int part = (int)(i % parts), c = part * 64 + lane;
+    const uint64_t bits = __ballot(c < n && y[m * ldy + min(c, n - 1)] > 0.f);
+    const int word = part * 2 + lane / 32;
+    if (lane % 32 == 0 && word < words) mask[m * words + word] = (uint32_t)(bits >> lane);
+  }
+}
+__global__ __launch_bounds__(256) void relu_mask_bwd_kernel(int64_t rows, int n, Dz d, float* __restrict__ dz,
+                                                            int64_t lddz) {
+  const int lane = threadIdx.x % 64, parts = (n + 63) / 64;
+  for (int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 64; i < rows * parts; i += (int64_t)gridDim.x * 4) {
+    const int64_t m = i / parts;
+    const int c = (int)(i % parts) * 64 + lane;
+    if (c < n) dz[m * lddz + c] = dz_at<DZ_RELU>(d, m, c);
+  }
+}
+unsigned mask_blocks(int64_t rows, int n) {
+  return (unsigned)std::min<int64_t>(ceil_div(rows * ceil_div(n, 64), 4), 1 << 16);
+}
+
 // ---- launches -------------------------------------------------------------------------
 template <int MODE, int ACT, typename X, typename T, int BM, int BN, int WM, int WN>
 int launch_tile(const SideArgs& a, hipStream_t stream) {
@@ -1192,6 +1218,26 @@ int inf_linear_ckpt_backward(int64_t rows, int n, int k, const float* dy, int64_
   backward<ACT>(rows, n, k, dz, q, ld_q, scale, W, stride_wn, stride_wk, dx, dx_dtype, ld_dx, dW, ld_dw, db, ws, st)
   return act == 1 ? INF_BACKWARD(DZ_RELU) : act == 2 ? INF_BACKWARD(DZ_SIGMOID) : INF_BACKWARD(DZ_NONE);
 #undef INF_BACKWARD
+}
+
+int inf_relu_mask(int64_t rows, int n, const float* y, int64_t ld_y, uint32_t* mask, inf_stream_t stream) {
+  INF_CHECK_ARG(rows >= 0 && n >= 1 && ld_y >= n && rows < (int64_t)1 << 31, "relu_mask: bad shape");
+  if (rows == 0) return INF_OK;
+  INF_CHECK_ARG(y != nullptr && mask != nullptr, "relu_mask: null argument");
+  relu_mask_kernel<<<mask_blocks(rows, n), 256, 0, (hipStream_t)stream>>>(rows, n, y, ld_y, mask);
+  INF_LAUNCH_CHECK();
+  return INF_OK;
+}
+
+int inf_relu_mask_bwd(int64_t rows, int n, const float* dy, int64_t ld_dy, const uint32_t* mask, float* dz, int64_t ld_dz,
+                      inf_stream_t stream) {
+  INF_CHECK_ARG(rows >= 0 && n >= 1 && ld_dy >= 0 && ld_dz >= n && rows < (int64_t)1 << 31, "relu_mask_bwd: bad shape");
+  if (rows == 0) return INF_OK;
+  INF_CHECK_ARG(dy != nullptr && mask != nullptr && dz != nullptr, "relu_mask_bwd: null argument");
+  const Dz d{dy, ld_dy, nullptr, 0, mask, (n + 31) / 32};
+  relu_mask_bwd_kernel<<<mask_blocks(rows, n), 256, 0, (hipStream_t)stream>>>(rows, n, d, dz, ld_dz);
+  INF_LAUNCH_CHECK();
+  return INF_OK;
 }
 
 }  // extern "C"

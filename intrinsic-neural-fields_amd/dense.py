@@ -11,7 +11,8 @@ allocates.
 
 In 8 bits (csrc/quant.hpp: whole numbers q and one scale s a row, x ~ s q):
 `linear(..., checkpoint="int8")` keeps the inputs in 8 bits between forward and backward
-(a quarter of the memory; ReLU's outputs as one bit each), `linear8` multiplies 8-bit rows
+(a quarter of the memory; ReLU's outputs as one bit each), with products in 16-bit pieces or, at
+products="fp32", as without; `linear8` multiplies 8-bit rows
 with 8-bit weights for rendering, and `quantize_rows` / `Rows8.restore` are the rows
 themselves.
 
@@ -48,6 +49,15 @@ def _gemm(M, N, K, A, sam, sak, B, sbn, sbk, bias, act, beta, C, ldc):
                                 rt.ptr(C), ldc, rt.stream_handle()), "dense_gemm")
 
 
+def _products(spec, act, xs, ws, bs, y):
+    """y = act(sum_s x_s W_s[:, c_s:]^T + sum bias), in fp32."""
+    rows, n = y.shape
+    for s, (wi, c0) in enumerate(spec):
+        x, W = xs[s], ws[wi]
+        _gemm(rows, n, x.shape[1], x, x.stride(0), x.stride(1), W[:, c0:], W.stride(0), W.stride(1),
+              bs[s] if s < len(bs) else None, act if s == len(spec) - 1 else 0, 0.0 if s == 0 else 1.0, y, n)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, spec, act, *tensors):
@@ -58,10 +68,7 @@ class _Linear(torch.autograd.Function):
         B = xs[0].shape[0]
         N = ws[0].shape[0]
         y = torch.empty((B, N), dtype=torch.float32, device=xs[0].device)
-        for s, (wi, c0) in enumerate(spec):
-            x, W = xs[s], ws[wi]
-            _gemm(B, N, x.shape[1], x, x.stride(0), x.stride(1), W[:, c0:], W.stride(0), W.stride(1),
-                  bs[s] if s < len(bs) else None, act if s == nseg - 1 else 0, 0.0 if s == 0 else 1.0, y, N)
+        _products(spec, act, xs, ws, bs, y)
         ctx.spec, ctx.act, ctx.nw, ctx.nb = spec, act, nw, len(bs)
         ctx.save_for_backward(*xs, *ws, y)
         return y
@@ -110,7 +117,7 @@ class _Linear(torch.autograd.Function):
         return (None, None, *dxs, *dws, *dbs)
 
 
-def linear(segments, weights, biases, act=None, checkpoint=None):
+def linear(segments, weights, biases, act=None, checkpoint=None, products=None):
     """segments: [(x_s, weight index, column offset)]; weights / biases: lists of tensors.
 
     checkpoint="int8": x_s (fp32, or bf16 taken as it is) is kept in 8 bits for the backward,
@@ -120,14 +127,17 @@ def linear(segments, weights, biases, act=None, checkpoint=None):
     to 2^-39 of the largest of its row (of x and dz; of W, its row forward, its column for dx) where
     that is more, a product to 2^-21; a term of dW to 2^-24 of itself, or to 2^-126 where that is
     more; their sums are fp32, in another order; a row of x with an infinity or a NaN gives NaN,
-    and one whose largest value is below 2^-143 counts as zeros.  (As with every layer here: a
+    and one whose largest value is below 2^-143 counts as zeros.  products="fp32" leaves all but dW
+    as it is without a checkpoint, bit for bit, and takes the time of those products.  (As with every layer here: a
     backward is captured into a graph only while no eager graph of the same leaves is alive.)"""
     for t in [x for x, _, _ in segments] + list(weights) + list(biases):
         if not t.is_cuda:
             raise RuntimeError("the dense layers run on the HIP device only; there is no CPU fallback")
+    if products not in (None, "fp32"):
+        raise ValueError(f'products are "fp32" or, with a checkpoint, its own (None), not {products!r}')
     spec = tuple((wi, c0) for _, wi, c0 in segments)
     if checkpoint is not None:
-        return _linear_ckpt(segments, spec, weights, biases, ACT[act], checkpoint)
+        return _linear_ckpt(segments, spec, weights, biases, ACT[act], checkpoint, products)
     xs = [x.to(torch.float32) for x, _, _ in segments]
     return _Linear.apply(spec, ACT[act], *xs, *weights, *biases)
 
@@ -421,12 +431,9 @@ class _LinearCkpt(torch.autograd.Function):
                 if needs[4 + s]:
                     grads[4 + s] = dx = torch.empty((rows, k), dtype=dtypes[s], device=device)
                 if needs[4 + nseg + wi]:
-                    g = grads[4 + nseg + wi]
-                    if g is None:
-                        covered = sum(kk for (wj, _), kk in zip(spec, widths) if wj == wi) == W.shape[1]
-                        g = grads[4 + nseg + wi] = (torch.empty if covered else torch.zeros)(
-                            W.shape, dtype=torch.float32, device=device)
-                    dw = g.data_ptr() + 4 * c0
+                    if grads[4 + nseg + wi] is None:
+                        grads[4 + nseg + wi] = _weight_gradient(spec, widths, wi, W)
+                    dw = grads[4 + nseg + wi].data_ptr() + 4 * c0
                 if s < nb and needs[4 + nseg + nw + s]:
                     grads[4 + nseg + nw + s] = db = torch.empty(n, dtype=torch.float32, device=device)
                 if dx is None and dw is None and db is None:
@@ -440,7 +447,82 @@ class _LinearCkpt(torch.autograd.Function):
         return tuple(grads)
 
 
-def _linear_ckpt(segments, spec, weights, biases, act, checkpoint):
+class _LinearKept(torch.autograd.Function):
+    """_Linear's products, with the inputs kept in 8 bits and a ReLU's output as bits for the backward."""
+
+    @staticmethod
+    def forward(ctx, spec, act, kept, recorded, *tensors):
+        # as _LinearCkpt; x fp32
+        rt = _rt()
+        lib = rt.lib
+        nseg = len(spec)
+        nw = max(w for w, _ in spec) + 1
+        xs, ws, bs = tensors[:nseg], tensors[nseg:nseg + nw], tensors[nseg + nw:]
+        needs = ctx.needs_input_grad
+        rows, n, device = xs[0].shape[0], ws[0].shape[0], xs[0].device
+        with _on(device):
+            y = torch.empty((rows, n), dtype=torch.float32, device=device)
+            _products(spec, act, xs, ws, bs, y)
+            if not recorded:
+                return y
+            kept = [(r or quantize_rows(x)) if needs[4 + nseg + wi] else None for r, x, (wi, _) in zip(kept, xs, spec)]
+            out = y if act == 2 else None
+            if act == 1 and any(needs):
+                out = torch.empty((rows, (n + 31) // 32), dtype=torch.int32, device=device)
+                rt.check(lib.inf_relu_mask(rows, n, y.data_ptr(), n, out.data_ptr(), _stream(device)), "relu_mask")
+        ctx.layer = (spec, act, nw, len(bs), rows, n, [x.shape[1] for x in xs], [r is not None for r in kept])
+        ctx.save_for_backward(out, *ws, *[t for r in kept if r is not None for t in (r.q, r.scale)])
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        rt = _rt()
+        lib = rt.lib
+        spec, act, nw, nb, rows, n, widths, has_rows = ctx.layer
+        nseg = len(spec)
+        out, ws = ctx.saved_tensors[0], ctx.saved_tensors[1:1 + nw]
+        rows8 = iter(ctx.saved_tensors[1 + nw:])
+        needs = ctx.needs_input_grad
+        dy = dy.to(torch.float32).contiguous()
+        device = dy.device
+        grads = [None] * (4 + nseg + nw + nb)
+        with _on(device):
+            st = _stream(device)
+            dz = dy if act == 0 else torch.empty_like(dy)
+            if act == 1:
+                rt.check(lib.inf_relu_mask_bwd(rows, n, dy.data_ptr(), n, out.data_ptr(), dz.data_ptr(), n, st),
+                         "relu_mask_bwd")
+            elif act == 2:
+                rt.check(lib.inf_dense_act_bwd(dz.numel(), out.data_ptr(), dy.data_ptr(), act, dz.data_ptr(), st),
+                         "dense_act_bwd")
+            work = _workspace(lib, rows, n, widths, 1, device) if any(has_rows) else None
+            for s, (wi, c0) in enumerate(spec):
+                W, k = ws[wi], widths[s]
+                if needs[4 + s]:
+                    grads[4 + s] = dx = torch.empty((rows, k), dtype=torch.float32, device=device)
+                    _gemm(rows, k, n, dz, n, 1, W[:, c0:], W.stride(1), W.stride(0), None, 0, 0.0, dx, k)
+                if has_rows[s]:
+                    q, scale = next(rows8), next(rows8)
+                    if grads[4 + nseg + wi] is None:
+                        grads[4 + nseg + wi] = _weight_gradient(spec, widths, wi, W)
+                    dw = grads[4 + nseg + wi].data_ptr() + 4 * c0
+                    rt.check(lib.inf_linear_ckpt_backward(
+                        rows, n, k, dz.data_ptr(), n, 0, None, n, None, q.data_ptr(), q.stride(0), scale.data_ptr(), None,
+                        0, 0, None, rt.DTYPE_F32, k, dw, W.shape[1], None, work.data_ptr(), st), "linear_ckpt_backward")
+                if s < nb and needs[4 + nseg + nw + s]:
+                    grads[4 + nseg + nw + s] = db = torch.empty(n, dtype=torch.float32, device=device)
+                    rt.check(lib.inf_colsum(rows, n, dz.data_ptr(), n, db.data_ptr(), 0, st), "colsum")
+        return tuple(grads)
+
+
+def _weight_gradient(spec, widths, wi, W):
+    """For the segments' columns of W to be written; zeros where no segment takes some of them."""
+    covered = sum(k for (wj, _), k in zip(spec, widths) if wj == wi) == W.shape[1]
+    return (torch.empty if covered else torch.zeros)(W.shape, dtype=torch.float32, device=W.device)
+
+
+def _linear_ckpt(segments, spec, weights, biases, act, checkpoint, products):
     kept = [checkpoint] * len(segments) if isinstance(checkpoint, str) else list(checkpoint)
     if len(kept) != len(segments) or any(not isinstance(c, Rows8) and c != "int8" for c in kept):
         raise ValueError('checkpoint is "int8", or for each segment "int8" or the Rows8 of its input')
@@ -471,8 +553,11 @@ def _linear_ckpt(segments, spec, weights, biases, act, checkpoint):
     for t in (*xs, *weights, *biases):
         if t.device != device:
             raise ValueError("linear takes its tensors on one device")
-    return _LinearCkpt.apply(spec, act, tuple(None if isinstance(c, str) else c for c in kept), torch.is_grad_enabled(),
-                             *xs, *weights, *biases)
+    layer = _LinearCkpt
+    if products == "fp32":
+        layer, xs = _LinearKept, [x.to(torch.float32) for x in xs]
+    return layer.apply(spec, act, tuple(None if isinstance(c, str) else c for c in kept), torch.is_grad_enabled(),
+                       *xs, *weights, *biases)
 
 
 def view_angles(unit_dirs, face_idxs, face_normals):

@@ -100,6 +100,8 @@ _SIGNATURES = {
     "inf_linear_ckpt_backward": (c_int, [c_int64, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p,
                                          c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int,
                                          c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    "inf_relu_mask": (c_int, [c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
+    "inf_relu_mask_bwd": (c_int, [c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
     "inf_plan_create": (c_int, [ctypes.POINTER(MlpDesc), c_int, ctypes.POINTER(c_void_p)]),
     "inf_plan_destroy": (None, [c_void_p]),
     "inf_plan_get_info": (c_int, [c_void_p, ctypes.POINTER(PlanInfo)]),

@@ -76,6 +76,7 @@ class LinearWithConcatAndActivation(nn.Module):
         self.Ly = nn.Linear(y_in_dim, out_dim)
         self.actn = activation()
         self.checkpoint = None  # None or "int8": what dense.linear keeps of x and y until the backward
+        self.products = None    # None or "fp32": its products with a checkpoint
         self.batchnorm = None
         if batchnorm:
             self.batchnorm = nn.BatchNorm1d(out_dim)
@@ -91,5 +92,5 @@ class LinearWithConcatAndActivation(nn.Module):
         lead = x.shape[:-1]
         out = dense.linear([(x.reshape(-1, x.shape[-1]), 0, 0), (y.reshape(-1, y.shape[-1]), 1, 0)],
                            [self.Lx.weight, self.Ly.weight], [self.Lx.bias, self.Ly.bias], "relu",
-                           checkpoint=self.checkpoint)
+                           checkpoint=self.checkpoint, products=self.products)
         return out.view(*lead, out.shape[-1])

@@ -9,10 +9,11 @@ into it), the kernels read packed GEMM-dtype copies that are refreshed whenever 
 parameter changes, and a batch whose features were not materialised is gathered inside
 the same launch sequence (mesh.py:313-324 fused into the forward).
 
-The layers outside the fused plan (the view-dependent field; dense.py) take two more keys of
+The layers outside the fused plan (the view-dependent field; dense.py) take more keys of
 `model_config["kernels"]`: `dense_checkpoints: int8` keeps their inputs in 8 bits between
-forward and backward, `dense_inference: int8` runs them on 8-bit rows and weights wherever no
-gradient is recorded (rendering, evaluation).
+forward and backward (with `dense_products: fp32` their products are those without it),
+`dense_inference: int8` runs them on 8-bit rows and weights wherever no gradient is recorded
+(rendering, evaluation).
 
 Kernel arithmetic mode: `model_config["kernels"]["mode"]` ("fp32" exact f32 MFMA, the
 default, or "bf16" MFMA with fp32 accumulation), overridable by INF_MODE.
@@ -114,6 +115,7 @@ class TextureField(nn.Module):
         self.kernel_mode = os.environ.get("INF_MODE", "fp32")
         self.max_batch_hint = 4096
         self.dense_checkpoints = None   # None or "int8": the dense layers' inputs until the backward
+        self.dense_products = None      # None or "fp32": the products of layers with checkpoints
         self._rt: _Runtime | None = None
 
     # ---- device binding ----------------------------------------------------------
@@ -225,12 +227,13 @@ class TextureField(nn.Module):
         for i, layer in enumerate(self.layers):
             if i == self.skip_layer_idx:
                 h = dense.linear([(h, 0, 0), (x, 1, 0)], [layer.Lx.weight, layer.Ly.weight],
-                                 [layer.Lx.bias, layer.Ly.bias], "relu", checkpoint=kept and [kept, kept_x])
+                                 [layer.Lx.bias, layer.Ly.bias], "relu", checkpoint=kept and [kept, kept_x],
+                                 products=self.dense_products)
             else:
                 lin = layer[0]
                 act = "relu" if i < n - 1 or not self.return_rgb else "sigmoid"
                 h = dense.linear([(h, 0, 0)], [lin.weight], [lin.bias], act,
-                                 checkpoint=kept and [kept if i else kept_x])
+                                 checkpoint=kept and [kept if i else kept_x], products=self.dense_products)
         return h
 
     def weights8(self):
@@ -396,13 +399,17 @@ class TextureFieldWithViewDependency(nn.Module):
                                              nn.Sigmoid())
         self.dense_inference = None   # None or "int8": the layers where no gradient is recorded
 
-    def set_dense_options(self, checkpoints=None, inference=None):
-        """checkpoints="int8": inputs kept in 8 bits until the backward (dense.linear);
-        inference="int8": 8-bit rows and weights where no gradient is recorded (dense.linear8)."""
+    def set_dense_options(self, checkpoints=None, inference=None, products=None):
+        """checkpoints="int8": inputs kept in 8 bits until the backward (dense.linear), and
+        products="fp32" the products of these layers as without it; inference="int8": 8-bit rows
+        and weights where no gradient is recorded (dense.linear8)."""
         for what in (checkpoints, inference):
             if what not in (None, "int8"):
                 raise ValueError(f'dense layers have "int8" or nothing for checkpoints and inference, not {what!r}')
+        if products not in (None, "fp32") or (products and not checkpoints):
+            raise ValueError(f'products are "fp32" or nothing, beside checkpoints, not {products!r}')
         self.spatial_mlp.dense_checkpoints = checkpoints
+        self.spatial_mlp.dense_products = products
         self.dense_inference = inference
 
     @contextlib.contextmanager
@@ -469,13 +476,13 @@ class TextureFieldWithViewDependency(nn.Module):
         import dense
         if self.dense_inference == "int8" and not torch.is_grad_enabled():
             return self._forward8(batch)
-        kept = self.spatial_mlp.dense_checkpoints
+        kept, products = self.spatial_mlp.dense_checkpoints, self.spatial_mlp.dense_products
         bottleneck = self.spatial_mlp(batch)
         view = self._get_embedded_view_dir(batch)
         l0, l2 = self.directional_mlp[0], self.directional_mlp[2]
         h = dense.linear([(bottleneck, 0, 0), (view, 0, self.bottleneck_vec_dim)], [l0.weight], [l0.bias], "relu",
-                         checkpoint=kept)
-        return dense.linear([(h, 0, 0)], [l2.weight], [l2.bias], "sigmoid", checkpoint=kept)
+                         checkpoint=kept, products=products)
+        return dense.linear([(h, 0, 0)], [l2.weight], [l2.bias], "sigmoid", checkpoint=kept, products=products)
 
 
 def init_weights(m):
@@ -522,12 +529,12 @@ def make_model(model_config, mesh=None):
                                                batchnorm=model_config.get("batchnorm", False), activation=nn.ReLU)
     model.apply(init_weights)
     kernels = model_config.get("kernels") or {}
-    dense_options = {k: kernels.get(f"dense_{k}") for k in ("checkpoints", "inference")}
+    dense_options = {k: kernels.get(f"dense_{k}") for k in ("checkpoints", "inference", "products")}
     if isinstance(model, TextureFieldWithViewDependency):
         model.set_dense_options(**dense_options)
     elif any(dense_options.values()):
-        raise ValueError("kernels.dense_checkpoints / dense_inference are for the view-dependent field; the others "
-                         "run on the fused plan (kernels.mode)")
+        raise ValueError("kernels.dense_checkpoints / dense_products / dense_inference are for the view-dependent field; "
+                         "the others run on the fused plan (kernels.mode)")
     model.kernel_mode = os.environ.get("INF_MODE", kernels.get("mode", "fp32"))
     if kernels.get("max_batch"):
         model.max_batch_hint = int(kernels["max_batch"])
