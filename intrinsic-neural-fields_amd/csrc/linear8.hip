@@ -531,9 +531,11 @@ int launch_rows(const Linear8Args& a, const X* x, int64_t ldx, hipStream_t strea
   return INF_OK;
 }
 
-// k up to 256 with up to 256 outputs, and rows for a turn of every CU.  (Fewer outputs than 33 are
-// bound by x's bytes whichever kernel reads them; a sigmoid or a sum to add to is a head's or a skip
-// layer's, one a network.)
+// k up to 256 with up to 256 outputs, from 16,384 rows on: half of the CUs then have a workgroup, of 128 rows
+// a turn.  256 x 256, us, here and in tiles: int8 into fp32 rows 9.4 and 6.0 for 8192 rows, 10.2 and 9.7 for 16,384,
+// 12.0 and 13.6 for 32,768; bf16 into bf16 10.5 and 9.2, 11.5 and 14.0, 12.6 and 22.5 (into 8 bits this is
+// ahead from fewer rows on: int8 8.1 and 12.5 for 8192).  Fewer outputs than 33 are bound by x's bytes whichever
+// kernel reads them; a sigmoid or a sum to add to is a head's or a skip layer's, one a network.
 bool rows_walk(int64_t rows, int n, int k, int act, bool with_add) {
   return rows >= 16384 && k <= 256 && n > 32 && n <= 256 && act != 2 && !with_add;
 }
