@@ -292,6 +292,7 @@ def linear8(xs, weights, biases, act=None, out=torch.float32):
         raise ValueError("linear8 takes one weight and at most one bias for each segment")
     rows, n, device = xs[0].shape[0], weights[0].n, xs[0].device
     acc, last, lib, a = None, len(xs) - 1, rt.lib, ACT[act]
+    recorded, dual = torch.is_grad_enabled(), forward_ad._current_level >= 0
     if device.type != "cuda":
         rt.require_hip(xs[0].q if isinstance(xs[0], Rows8) else xs[0])
     with _on(device):
@@ -299,7 +300,7 @@ def linear8(xs, weights, biases, act=None, out=torch.float32):
             if isinstance(x, Rows8):
                 q, scale, xc = x.q, x.scale.data_ptr(), i8
             else:
-                if (x.requires_grad and torch.is_grad_enabled()) or _has_tangent(x):
+                if (recorded and x.requires_grad) or (dual and _has_tangent(x)):
                     raise RuntimeError("linear8 has no gradient: call it under torch.no_grad(), or train with linear")
                 q, scale = _rows_of(x, "x"), None
                 xc = rt.dtype_code(q)
@@ -308,7 +309,7 @@ def linear8(xs, weights, biases, act=None, out=torch.float32):
             b = biases[s] if s < len(biases) else None
             if b is not None and (b.shape != (n,) or b.dtype != torch.float32 or not b.is_contiguous()):
                 raise ValueError("a bias is a contiguous fp32 [n] tensor")
-            if b is not None and ((b.requires_grad and torch.is_grad_enabled()) or _has_tangent(b)):
+            if b is not None and ((recorded and b.requires_grad) or (dual and _has_tangent(b))):
                 raise RuntimeError("linear8 has no gradient: call it under torch.no_grad(), or train with linear")
             if q.device != device or w.packed.device != device or (b is not None and b.device != device):
                 raise ValueError("linear8 takes its tensors on one device")
