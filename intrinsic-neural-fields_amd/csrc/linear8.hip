@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256) void linear8_few_kernel(Linear8Args a, const X
 // into 8 bits there, and so are the results, whose row maximum is two exchanges between lanes.
 // Bound by the vector operations, a wave's phases of which and of matrix instructions overlap in part (a value
 // in: 9 operations, none from 8 bits; a result: 6, 15 into 8 bits), and by bytes.  262,144 x 256 x 256, us: bf16
-// into 8 bits 60, 8 bits into 8 bits 46 (their bytes: 39, 26), 8 bits into bf16 47 (39).
+// into 8 bits 63, 8 bits into 8 bits 44 (their bytes: 39, 26), 8 bits into bf16 52 (39).
 //   k runs over KS blocks of 64.  Within a block, byte p of lane group g's 16 is k = G (4 p / G +
 //   g) + p % G with G = 16 bytes of x (4 fp32, 8 bf16, 16 int8 values): each load of 16 bytes then
 //   lies next to the neighbouring lane groups'.  The weight is laid out the same way on its way to
