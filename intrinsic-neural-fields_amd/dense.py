@@ -128,7 +128,8 @@ def linear(segments, weights, biases, act=None, checkpoint=None, products=None):
     that is more, a product to 2^-21; a term of dW to 2^-24 of itself, or to 2^-126 where that is
     more; their sums are fp32, in another order; a row of x with an infinity or a NaN gives NaN,
     and one whose largest value is below 2^-143 counts as zeros.  products="fp32" leaves all but dW
-    as it is without a checkpoint, bit for bit, and takes the time of those products.  (As with every layer here: a
+    as it is without a checkpoint, bit for bit, and takes the time of those products.  A weight has
+    less than 2^29 values (rows and columns counted in 256s).  (As with every layer here: a
     backward is captured into a graph only while no eager graph of the same leaves is alive.)"""
     for t in [x for x, _, _ in segments] + list(weights) + list(biases):
         if not t.is_cuda:
@@ -556,6 +557,10 @@ def _linear_ckpt(segments, spec, weights, biases, act, checkpoint, products):
             raise ValueError("linear takes its tensors on one device")
     layer = _LinearCkpt
     if products == "fp32":
+        for x in xs:  # what dW's product takes (include/inf_hip.h), before the backward finds out
+            k = x.shape[1]
+            if max(_round_up(n, 256) * _round_up(k, 64), _round_up(k, 256) * _round_up(n, 64)) >= 1 << 29:
+                raise RuntimeError(f"linear with a checkpoint: a weight of {n} x {k} is too large")
         layer, xs = _LinearKept, [x.to(torch.float32) for x in xs]
     return layer.apply(spec, act, tuple(None if isinstance(c, str) else c for c in kept), torch.is_grad_enabled(),
                        *xs, *weights, *biases)

@@ -153,3 +153,22 @@ def test_graph_replay_and_streams():
         want = step(sx, sdy, "relu") + step(sx, sdy, "sigmoid")
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("kw", [{}, {"products": "fp32"}])
+@pytest.mark.parametrize("n,k,taken", [(1 << 21, 1, False), (1, 1 << 21, False), ((1 << 21) - 63, 1, False),
+                                       ((1 << 21) - 64, 1, True), ((1 << 21) - 255, 1, True), (1, (1 << 21) - 64, True)])
+def test_weights_too_large_are_refused_by_the_forward(n, k, taken, kw):
+    """n k is counted with one side rounded up to 256 and the other to 64: of one column, 2^21 - 64 rows are the most."""
+    d = dense()
+    x, w = torch.ones((1, k), device="cuda"), torch.ones((n, k), device="cuda", requires_grad=True)
+
+    def call():
+        return d.linear([(x, 0, 0)], [w], [], "relu", checkpoint="int8", **kw)
+
+    if not taken:
+        with pytest.raises(RuntimeError, match="too large"):
+            call()
+        return
+    y = call()
+    assert (y == k).all() and (torch.autograd.grad(y.sum(), w)[0] == 1).all()
